@@ -227,12 +227,22 @@ def _workspace(nbytes):
     return _WORKSPACE["buf"].data_ptr()
 
 
+_LIBRARY = {}
+
+
+def _library(model):
+    """The package and a model's library, loaded once per program."""
+    if model not in _LIBRARY:
+        path = str(Path(__file__).resolve().parent.parent / "conflux-nova_amd")
+        if path not in sys.path:
+            sys.path.insert(0, path)
+        import nova_amd
+        _LIBRARY[model] = nova_amd, nova_amd.load(model)
+    return _LIBRARY[model]
+
+
 def _own(s):
-    path = str(Path(__file__).resolve().parent.parent / "conflux-nova_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    import nova_amd
-    nova = nova_amd.load(s.case["model"])
+    nova_amd, nova = _library(s.case["model"])
     st = torch.cuda.current_stream().cuda_stream
     kind = s.case["kind"]
     if kind == "cow":
