@@ -35,6 +35,8 @@ HIP_SOURCES = [
     "code/kernel/hip/attn_decode.hip",
     "code/kernel/hip/attn_prefill.hip",
     "code/kernel/hip/kv_pages.hip",
+    "code/kernel/hip/kv_q8.hip",
+    "code/kernel/hip/attn_q8.hip",
     "code/kernel/hip/rope.hip",
     "code/kernel/hip/q4k.hip",
 ]

@@ -11,7 +11,8 @@
 //   * Engine::cow_guard (src/model.cpp:171-191)
 // Differences, all MI355X-motivated:
 //   * pools are fp16 and sized by (n_slices, ctx) at run time, from one
-//     dev_alloc per pool; at 288 GB per GPU the pool is the dominant tenant
+//     dev_alloc per pool; at 288 GB per GPU the pool is the dominant tenant.
+//     The same layer serves one pool of 8-bit pages (init's q8)
 //   * page clears and COW copies are single launches (launch_kv_zero_pages,
 //     launch_kv_cow_apply) instead of 2*L memset/memcpy calls per page; the
 //     table patch rides in the same launch
@@ -39,16 +40,23 @@ namespace nova {
 
 class PagedKv {
 public:
-    // n_slices sessions of up to ctx tokens share NB = n_slices * ceil(ctx/16) pages
-    void init(int n_slices, int64_t ctx) {
+    // n_slices sessions of up to ctx tokens share NB = n_slices * ceil(ctx/16) pages.
+    // q8: one pool of 8-bit pages instead of the two fp16 pools; tables, page ids,
+    // refcounts and COW decisions are the same, and KvSlice::k, v stay null.
+    void init(int n_slices, int64_t ctx, bool q8 = false) {
         geo_ = nova_model_geometry();
         pool_.init(n_slices, ctx);
         nb_ = pool_.nb_total();
-        const uint64_t per_pool = (uint64_t)geo_.n_layers * (uint64_t)nb_ * (uint64_t)geo_.kv_block *
-                                  (uint64_t)geo_.nkv * (uint64_t)geo_.hd * 2ull;
-        k_ = static_cast<uint16_t*>(dev_alloc(per_pool));
-        v_ = static_cast<uint16_t*>(dev_alloc(per_pool));
-        pool_bytes_ = per_pool;
+        if (q8) {
+            pool_bytes_ = (uint64_t)geo_.n_layers * (uint64_t)nb_ * (uint64_t)kv_q8_page_bytes();
+            q8_ = static_cast<uint8_t*>(dev_alloc(pool_bytes_));
+        } else {
+            const uint64_t per_pool = (uint64_t)geo_.n_layers * (uint64_t)nb_ * (uint64_t)geo_.kv_block *
+                                      (uint64_t)geo_.nkv * (uint64_t)geo_.hd * 2ull;
+            k_ = static_cast<uint16_t*>(dev_alloc(per_pool));
+            v_ = static_cast<uint16_t*>(dev_alloc(per_pool));
+            pool_bytes_ = per_pool;
+        }
         tables_ = static_cast<int32_t*>(dev_alloc((uint64_t)(nb_ > 0 ? nb_ : 1) * 4ull));
         pool_.set_dev(tables_);
         stream_ = dev_stream_create();
@@ -58,9 +66,11 @@ public:
         if (stream_) dev_stream_sync(stream_);
         dev_free(k_);
         dev_free(v_);
+        dev_free(q8_);
         dev_free(tables_);
         if (stream_) dev_stream_destroy(stream_);
         k_ = v_ = nullptr;
+        q8_ = nullptr;
         tables_ = nullptr;
         stream_ = nullptr;
     }
@@ -79,7 +89,7 @@ public:
             std::vector<int32_t> pages(s->table.begin(), s->table.end());
             int32_t* d = static_cast<int32_t*>(dev_alloc(pages.size() * 4));
             dev_upload_async(d, pages.data(), pages.size() * 4, stream_);
-            launch_kv_zero_pages(k_, v_, nb_, d, (int)pages.size(), stream_);
+            zero_pages(d, (int)pages.size());
             dev_stream_sync(stream_);
             dev_free(d);
         }
@@ -113,7 +123,7 @@ public:
             }
             int32_t* d = static_cast<int32_t*>(dev_alloc(pages.size() * 4));
             dev_upload_async(d, pages.data(), pages.size() * 4, stream_);
-            launch_kv_zero_pages(k_, v_, nb_, d, (int)pages.size(), stream_);
+            zero_pages(d, (int)pages.size());
             dev_stream_sync(stream_);
             dev_free(d);
         }
@@ -164,7 +174,7 @@ public:
     int cow_guard(KvSlice& s, int64_t pos, nova_stream_t st) {
         nova_cow_op op;
         const int nb = decide(s, pos, &op);
-        if (nb >= 0) launch_kv_cow_apply(k_, v_, nb_, tables_, &op, 1, st);
+        if (nb >= 0) cow_apply(&op, 1, st);
         return nb;
     }
 
@@ -176,7 +186,7 @@ public:
             nova_cow_op op;
             if (decide(s, (int64_t)b * kKvBlockCfg, &op) >= 0) ops.push_back(op);
         }
-        if (!ops.empty()) launch_kv_cow_apply(k_, v_, nb_, tables_, ops.data(), (int)ops.size(), st);
+        if (!ops.empty()) cow_apply(ops.data(), (int)ops.size(), st);
     }
 
     // Many sessions' next writes at once: session i writes [pos0[i], pos0[i]+n[i]).
@@ -193,7 +203,7 @@ public:
                 if (decide(*ss[i], (int64_t)b * kKvBlockCfg, &op) >= 0) ops.push_back(op);
             }
         }
-        if (!ops.empty()) launch_kv_cow_apply(k_, v_, nb_, tables_, ops.data(), (int)ops.size(), st);
+        if (!ops.empty()) cow_apply(ops.data(), (int)ops.size(), st);
         return (int)ops.size();
     }
 
@@ -204,12 +214,23 @@ public:
     KvPool& pool() { return pool_; }
     uint16_t* k_base() const { return k_; }
     uint16_t* v_base() const { return v_; }
+    uint8_t* q8_base() const { return q8_; }           // null unless the pool holds 8-bit pages
     int32_t* tables() const { return tables_; }
     int nb() const { return nb_; }
     uint64_t pool_bytes() const { return pool_bytes_; }
     nova_stream_t stream() const { return stream_; }
 
 private:
+    void zero_pages(const int32_t* pages_dev, int n) {
+        if (q8_) launch_kv_q8_zero_pages(q8_, nb_, pages_dev, n, stream_);
+        else launch_kv_zero_pages(k_, v_, nb_, pages_dev, n, stream_);
+    }
+
+    void cow_apply(const nova_cow_op* ops, int n, nova_stream_t st) {
+        if (q8_) launch_kv_q8_cow_apply(q8_, nb_, tables_, ops, n, st);
+        else launch_kv_cow_apply(k_, v_, nb_, tables_, ops, n, st);
+    }
+
     int decide(KvSlice& s, int64_t pos, nova_cow_op* op) {
         const int nb = pool_.cow_slice(s, pos);
         if (nb == -2) {
@@ -230,6 +251,7 @@ private:
     int nb_ = 0;
     uint16_t* k_ = nullptr;
     uint16_t* v_ = nullptr;
+    uint8_t* q8_ = nullptr;
     int32_t* tables_ = nullptr;
     uint64_t pool_bytes_ = 0;
     nova_stream_t stream_ = nullptr;

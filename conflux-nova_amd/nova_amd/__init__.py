@@ -95,6 +95,16 @@ _SIGS = {
     "launch_kv_cow_apply": (None, [vp, vp, i32, vp, C.POINTER(CowOp), i32, vp]),
     "launch_kv_zero_pages": (None, [vp, vp, i32, vp, i32, vp]),
     "launch_table_patch": (None, [vp, vp, vp, i32, vp]),
+    "kv_q8_page_bytes": (sz, []),
+    "launch_kv_q8_store_batch": (None, [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]),
+    "launch_rope_kv_q8_store_batch": (None, [vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp]),
+    "launch_kv_q8_load_batch": (None, [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]),
+    "attn_decode_q8_workspace_bytes": (sz, [i32]),
+    "launch_attn_decode_q8_batch": (None, [vp, vp, vp, i32, vp, i32, i32, i32, vp, vp, vp]),
+    "attn_chunk_q8_workspace_bytes": (sz, [i32, i32, i32]),
+    "launch_attn_chunk_q8_batch": (None, [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "launch_kv_q8_cow_apply": (None, [vp, i32, vp, C.POINTER(CowOp), i32, vp]),
+    "launch_kv_q8_zero_pages": (None, [vp, i32, vp, i32, vp]),
     # nova_graph.h
     "nova_kvpool_new": (vp, [i32, i64]),
     "nova_kvpool_delete": (None, [vp]),
@@ -131,6 +141,8 @@ _SIGS = {
     "nova_registry_live": (i32, [vp]),
     "nova_registry_total": (i32, [vp]),
     "nova_paged_new": (vp, [i32, i64]),
+    "nova_paged_new_q8": (vp, [i32, i64]),
+    "nova_paged_pool_q8": (vp, [vp]),
     "nova_paged_delete": (None, [vp]),
     "nova_paged_pool": (vp, [vp]),
     "nova_paged_pool_k": (vp, [vp]),

@@ -67,6 +67,12 @@ int     nova_registry_total(nova_registry_t r);
  *      SessionManager::create/destroy session.h:84-142, session_attach*,
  *      session_cow session.h:156-180, Engine::cow_guard model.cpp:171-191) ---- */
 nova_paged_t  nova_paged_new(int n_slices, int64_t ctx);
+/* The same over one pool of 8-bit pages (nova_kernel.h): nova_paged_pool_q8 is
+ * its base and nova_paged_pool_k / _v are NULL; in a handle of nova_paged_new it
+ * is the other way round.  Every other call is the same: creating sessions
+ * clears 8-bit pages and the COW calls copy them. */
+nova_paged_t  nova_paged_new_q8(int n_slices, int64_t ctx);
+void*         nova_paged_pool_q8(nova_paged_t h);
 void          nova_paged_delete(nova_paged_t h);
 nova_kvpool_t nova_paged_pool(nova_paged_t h);          /* its KvPool, for the getters above */
 uint16_t*     nova_paged_pool_k(nova_paged_t h);

@@ -272,6 +272,80 @@ void launch_gemv4_q4k(const uint8_t* blocks, int64_t rows, int cols, const int8_
 void launch_gemv_q4k_f32(const uint8_t* const* blocks, const int64_t* rows, float* const* outs, int n_mat,
                          int cols, const float* x, nova_stream_t s);
 
+/* ---- 8-bit pages (no reference counterpart) ----
+ *
+ * A cache at 132 instead of 256 bytes per row of 128 values: int8 codes c with
+ * one fp32 scale s per token, kv head and K or V; value = c * s.  One pool
+ *     pool[layer][NB][NKV][4224]  (bytes; kv_q8_page_bytes() = NKV * 4224),
+ * 16-byte aligned, with the block tables, positions and page ids of the fp16
+ * pools (KB = 16 tokens per page).  The record of a page and kv head holds, for
+ * token t of the page and dim d:
+ *     K code  int8 at (t>>2)*512 + (d>>4)*64 + (t&3)*16 + (d&15)
+ *     V code  int8 at 2048 + d*16 + t
+ *     K scale fp32 at 4096 + 4t,  V scale fp32 at 4160 + 4t
+ * All-zero memory is a page of zeros.
+ *
+ * Quantiser, per row x of 128 values: s = fp32(max|x| / 127), codes the integers
+ * nearest to the exact quotients x / s, ties to even (s at most the largest
+ * number whose 127 s is finite).  A row whose s would be
+ * below the smallest normal fp32 number is stored as zeros; a row that holds an
+ * infinity or a NaN gets the scale NaN and reads back as NaN.
+ *
+ * Ragged calls: n_rows rows in all, session i owning rows
+ * [row_off[i], row_off[i+1]) of the flat arrays (row_off: device int32[n_sess+1],
+ * not decreasing, from 0 to at most n_rows), or n_rows / n_sess rows each where
+ * row_off is NULL.  A session may have no rows.  Rows behind the last session's
+ * are neither read nor written.  tables must hold n_sess rows of table_stride
+ * entries; positions past table_stride * 16 are left out, a table entry outside
+ * [0, nb) is not written through and reads page 0.  fp32 arrays and pools are
+ * read 16 bytes at a time and must be 16-byte aligned. */
+size_t kv_q8_page_bytes(void);
+/* Append: session i's rows go to positions pos0[i].. (pos0: device
+ * int32[n_sess]).  k, v: [n_rows][NKV][HD] fp32.  Tokens of a page that the call
+ * does not write keep their codes and scales.  The 8-bit form of
+ * launch_kv_store_paged_batch. */
+void launch_kv_q8_store_batch(uint8_t* pool, const int32_t* tables, int table_stride, const int32_t* pos0,
+                              const int32_t* row_off, int n_sess, int n_rows, int layer, int nb, const float* k,
+                              const float* v, nova_stream_t s);
+/* RoPE and append in one launch, the 8-bit form of
+ * launch_rope_kv_store_paged_batch: q [n_rows][NH][HD] is rotated in place, k is
+ * rotated and quantised with v (k's buffer is left as passed).  The values that
+ * are quantised and the rotated q have the bits of launch_rope_batch. */
+void launch_rope_kv_q8_store_batch(float* q, const float* k, const float* v, const float* cs, const float* sn,
+                                   uint8_t* pool, const int32_t* tables, int table_stride, const int32_t* n_past,
+                                   const int32_t* row_off, int n_sess, int n_rows, int layer, int nb,
+                                   nova_stream_t s);
+/* Read back: the values of positions pos0[i].. of each session as fp32
+ * [n_rows][NKV][HD], c * s rounded once. */
+void launch_kv_q8_load_batch(const uint8_t* pool, const int32_t* tables, int table_stride, const int32_t* pos0,
+                             const int32_t* row_off, int n_sess, int n_rows, int layer, int nb, float* k, float* v,
+                             nova_stream_t s);
+/* Decode attention: one query row per session over keys [0, n_keys[i]) (device
+ * int32[n_sess]; the new token already appended).  q, o: [n_sess][NH][HD] fp32.
+ * n_keys[i] == 0 gives a row of zeros.  workspace: from
+ * attn_decode_q8_workspace_bytes(n_sess), 16-byte aligned, no initial contents;
+ * calls that may overlap need one each. */
+size_t attn_decode_q8_workspace_bytes(int n_sess);
+void launch_attn_decode_q8_batch(const float* q, const uint8_t* pool, const int32_t* tables, int table_stride,
+                                 const int32_t* n_keys, int n_sess, int layer, int nb, float* o, void* workspace,
+                                 nova_stream_t s);
+/* Chunk attention: row r of session i sits at position n_past[i] + r and attends
+ * keys [0, n_past[i] + r] (the chunk already appended): prefill chunks of unequal
+ * lengths, or a few drafted tokens per session behind long contexts.  q, o:
+ * [n_rows][NH][HD] fp32, ragged as above.  max_q: no session has more rows (rows
+ * past it are left unwritten).  n_past[i] >= 0.  workspace as for the decode,
+ * from attn_chunk_q8_workspace_bytes with the same three counts. */
+size_t attn_chunk_q8_workspace_bytes(int n_sess, int n_rows, int max_q);
+void launch_attn_chunk_q8_batch(const float* q, const uint8_t* pool, const int32_t* tables, int table_stride,
+                                const int32_t* n_past, const int32_t* row_off, int n_sess, int n_rows, int max_q,
+                                int layer, int nb, float* o, void* workspace, nova_stream_t s);
+/* launch_kv_cow_apply and launch_kv_zero_pages for 8-bit pages.  The copies of
+ * one call run side by side: an op whose dst is another op's dst, or any op's
+ * src, aborts the call. */
+void launch_kv_q8_cow_apply(uint8_t* pool, int nb, int32_t* tables_dev, const nova_cow_op* ops, int n_ops,
+                            nova_stream_t s);
+void launch_kv_q8_zero_pages(uint8_t* pool, int nb, const int32_t* pages, int n_pages, nova_stream_t s);
+
 #ifdef __cplusplus
 }
 #endif
