@@ -26,14 +26,14 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int NH = Model::NH, NKV = Model::NKV, HD = Model::HD, G = Model::G;
 constexpr float kLog2e = 1.4426950408889634f;
 #ifndef Q8_WPS
-#define Q8_WPS (NB == 1 ? 2 : 1)
+#define Q8_WPS (NB == 1 || kWide ? 2 : 1)
 #endif
 constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
-constexpr float kUnset = -1e30f;               // running reference before a column's first key
+constexpr float kUnset = -1e30f;               // reference of a column without keys, where states are joined
 constexpr float kTop = 6.f, kLazy = 14.f;      // log2 of a column's largest weight: where it is put, where it may drift
 constexpr int kAccRow = HD + 4;                // floats per column in LDS: rows on different banks
 static_assert(HD == 128 && kTilePages == 4 && G <= 16, "tile layout");
@@ -73,7 +73,7 @@ __device__ __forceinline__ int scan_incl(int v) {
 // lane N of each row of 16
 template <int N>
 __device__ __forceinline__ float row_lane(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xf, 0xf, false));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + N, 0xf, 0xf, true));
 }
 
 // over lanes c, c + 16, c + 32, c + 48
@@ -252,13 +252,16 @@ __device__ __forceinline__ h8 codes_f16(uint32_t w0, uint32_t w1) {
     return __builtin_bit_cast(h8, r) + (_Float16)-1152.0f;
 }
 
-// weights e in fp16 terms hi + lo, 22 bits of them
+// weights e in fp16 terms hi + lo (hi cut off, lo the rest: 21 bits or more)
 __device__ __forceinline__ void split_f16(const float (&e)[8], h8& hi, h8& lo) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const _Float16 h = (_Float16)e[j];
-        hi[j] = h;
-        lo[j] = (_Float16)(e[j] - (float)h);
+    for (int j = 0; j < 8; j += 2) {
+        const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[j], e[j + 1]));
+        const h2 r = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[j] - (float)h[0], e[j + 1] - (float)h[1]));
+        hi[j] = h[0];
+        hi[j + 1] = h[1];
+        lo[j] = r[0];
+        lo[j + 1] = r[1];
     }
 }
 
@@ -272,9 +275,14 @@ __device__ __forceinline__ void split_f16(const float (&e)[8], h8& hi, h8& lo) {
 template <int NB, bool kCausal, bool kWide>
 __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
     constexpr int COLS = kGroupCols<NB, kWide>;
-    __shared__ __attribute__((aligned(16))) float s_acc[WAVES][16][kAccRow];
+    // in the wide form the query's digits stay in LDS, 1 KiB per operand, which the
+    // results overwrite at the end; otherwise they stay in registers
+    constexpr int kQOps = 6 * NB;
+    constexpr int kWaveLds = kWide && kQOps * 1024 > 16 * kAccRow * 4 ? kQOps * 1024 : 16 * kAccRow * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char s_wave[WAVES][kWaveLds];
     __shared__ float s_m[WAVES][16 * NB], s_l[WAVES][16 * NB];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    auto s_acc = [&](int w, int col, int d) { return reinterpret_cast<f4*>(s_wave[w] + (col * kAccRow + d) * 4); };
     const int kvh = blockIdx.x, slot = blockIdx.y;
     const Part p = find_part<kCausal, COLS>(a, slot);
     if (p.sess < 0) return;
@@ -336,7 +344,8 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
 
     QDigits q[NB];
     int seen[NB];              // keys that the column sees
-    float m[NB], l[NB];
+    // running reference and sum of the column; a score above `limit` moves the reference
+    float m[NB], l[NB], limit[NB];
     f4 acc[NB][DB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -353,59 +362,78 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
                 if (!real) x[h][j] = f4{0.f, 0.f, 0.f, 0.f};
             }
         q_digits(x, q[b]);
+        if constexpr (kWide)
+#pragma unroll
+            for (int e = 0; e < 6; ++e)
+                *reinterpret_cast<i4*>(s_wave[wave] + (6 * b + e) * 1024 + 16 * lane) = q[b].d[e / 2][e % 2];
         seen[b] = real ? min(p.s.past + r + 1, p.s.keys) : 0;
-        m[b] = kUnset;
-        l[b] = 0.f;
+        m[b] = l[b] = 0.f;
+        limit[b] = -INFINITY;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[b][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
 
-    for (int t = t0; t < t1; ++t) {
+    auto q_op = [&](int b, int d, int h) -> i4 {
+        if constexpr (kWide) return *reinterpret_cast<const i4*>(s_wave[wave] + (6 * b + 2 * d + h) * 1024 + 16 * lane);
+        else return q[b].d[d][h];
+    };
+    // The lowest digit's sum starts at the bits of 1.5 * 2^23, so that it is that
+    // float plus the sum without a conversion; the middle one starts 1.5 * 2^23 / 256
+    // lower, which takes it off again.
+    const i4 kLow = i4{0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000}, kMid = i4{-49152, -49152, -49152, -49152};
+    auto step = [&](auto mask_tag, int t) {
+        constexpr bool kMask = decltype(mask_tag)::value;
+        if constexpr (kWide) asm volatile("" ::: "memory");  // the digits are read anew, not kept in 48 registers
         const int key0 = t * TILE + 16 * g;
-        const bool masked = (t + 1) * TILE > clear_keys;
         // lane (g, c) has the scales of token c of page g; a key behind the last
         // one may hold anything
-        const bool there = key0 + c < p.s.keys;
-        const float sv = there ? (vs == 0.f ? 0x1p-20f : vs) : 1.f;
-        const float lv = __builtin_amdgcn_logf(sv), inv = 1.0f / sv;
+        float sv = vs == 0.f ? 0x1p-20f : vs;
+        if (kMask && key0 + c >= p.s.keys) sv = 1.f;
+        const float lv = __builtin_amdgcn_logf(sv), inv = __builtin_amdgcn_rcpf(sv);
         h8 hi[NB][2], lo[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             // scores: key block kb has row 4g + i = token 4 kb + i of page g
             float x[16];
-            float top = kUnset;
+            float top = -INFINITY;
             each<4>([&](auto kb) {
-                i4 z[3];
+                i4 z[3] = {i4{0, 0, 0, 0}, kMid, kLow};
 #pragma unroll
-                for (int d = 0; d < 3; ++d) {
-                    z[d] = i4{0, 0, 0, 0};
+                for (int d = 0; d < 3; ++d)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        z[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[2 * kb + h], q[b].d[d][h], z[d], 0, 0, 0);
-                }
+                        z[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[2 * kb + h], q_op(b, d, h), z[d], 0, 0, 0);
                 each<4>([&](auto i) {
                     constexpr int e = i, j = 4 * kb + i;
-                    const float w = fmaf((float)((z[0][e] << 8) + z[1][e]), 256.f, (float)z[2][e]) * row_lane<j>(ks);
-                    x[j] = fmaf(w, q[b].scale, row_lane<j>(lv));
-                    if (masked && key0 + j >= seen[b]) x[j] = -INFINITY;
+                    const float w = fmaf((float)((z[0][e] << 8) + z[1][e]), 256.f, __int_as_float(z[2][e])) * row_lane<j>(ks);
+                    x[j] = fmaf(w, q[b].scale, row_lane<j>(lv) - m[b]);
+                    if (kMask && key0 + j >= seen[b]) x[j] = -INFINITY;
                     top = fmaxf(top, x[j]);
                 });
             });
-            if (__builtin_amdgcn_ballot_w64(top > m[b] + kLazy)) {
+            if (__builtin_amdgcn_ballot_w64(top > limit[b])) {
+                // rare: a column's first keys, and a score more than kLazy above the
+                // reference, put it to kTop below the largest score
                 const float col_top = rows_max(top);
-                const float to = col_top > m[b] + kLazy ? col_top - kTop : m[b];
-                const float corr = __builtin_amdgcn_exp2f(m[b] - to);
-                m[b] = to;
+                const bool moves = col_top > limit[b];
+                const float by = moves ? col_top - kTop : 0.f;
+                const float corr = limit[b] == kLazy ? __builtin_amdgcn_exp2f(-by) : 0.f;
+                m[b] += by;
+                limit[b] = moves ? kLazy : limit[b];
                 l[b] *= corr;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] -= by;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[b][d] *= corr;
             }
             float e[2][8];
             each<16>([&](auto j) {
-                const float w = __builtin_amdgcn_exp2f(x[j] - m[b]);
+                const float w = __builtin_amdgcn_exp2f(x[j]);
                 e[j / 8][j % 8] = w;
-                const float share = w * row_lane<j>(inv);
-                l[b] += masked && key0 + j >= seen[b] ? 0.f : share;
+                // (the cross-lane read is not for the lanes of one side of a branch)
+                const float share = row_lane<j>(inv) * w;
+                if (kMask) l[b] += key0 + j >= seen[b] ? 0.f : share;
+                else l[b] += share;
             });
             split_f16(e[0], hi[b][0], lo[b][0]);
             split_f16(e[1], hi[b][1], lo[b][1]);
@@ -427,7 +455,10 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
                 }
             }
         if (more) load_v();
-    }
+    };
+    const int t_clear = max(min(t1, clear_keys / TILE), t0);
+    for (int t = t0; t < t_clear; ++t) step(std::false_type{}, t);
+    for (int t = t_clear; t < t1; ++t) step(std::true_type{}, t);
 
     // ---- the waves' results through LDS: each wave's own columns, or the four
     // states of the same columns joined; a lone part writes the output ----
@@ -447,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
     for (int b = 0; b < NB; ++b) {
         l[b] = rows_sum(l[b]);
         if (g == 0) {
-            s_m[wave][16 * b + c] = m[b];
+            s_m[wave][16 * b + c] = limit[b] == kLazy ? m[b] : kUnset;
             s_l[wave][16 * b + c] = l[b];
         }
     }
@@ -457,14 +488,14 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
         if (b > 0 && !kWide) __syncthreads();
         if (col0 + 16 * b + c < n_cols)
 #pragma unroll
-            for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(&s_acc[wave][c][16 * d + 4 * g]) = acc[b][d];
+            for (int d = 0; d < DB; ++d) *s_acc(wave, c, 16 * d + 4 * g) = acc[b][d];
         if constexpr (kWide) {
             wave_lds_sync();
 #pragma unroll
             for (int e = lane; e < 16 * (HD / 4); e += 64) {
                 const int cc = e / (HD / 4), d4 = e % (HD / 4), col = col0 + 16 * b + cc;
                 if (col < n_cols)
-                    put(col, d4, *reinterpret_cast<const f4*>(&s_acc[wave][cc][4 * d4]), s_m[wave][16 * b + cc],
+                    put(col, d4, *s_acc(wave, cc, 4 * d4), s_m[wave][16 * b + cc],
                         s_l[wave][16 * b + cc]);
             }
             wave_lds_sync();
@@ -482,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 const float f = __builtin_amdgcn_exp2f(s_m[w][col] - mm);
-                sum += *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]) * f;
+                sum += *s_acc(w, cc, 4 * d4) * f;
                 ll += s_l[w][col] * f;
             }
             put(col, d4, sum, mm, ll);
