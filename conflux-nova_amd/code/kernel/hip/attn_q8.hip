@@ -4,6 +4,7 @@
 // o_h = sum_t softmax_t(q_h . k_t / sqrt(HD)) v_t, k_t = ks_t * code, v_t = vs_t * code,
 // over keys [0, n_keys) or, for row r of a chunk, [0, n_past + r].
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 #include <utility>
@@ -142,17 +143,32 @@ constexpr int kGroupCols = 16 * NB * (kWide ? WAVES : 1);
 // ceil(rows * G / cols) column groups, which its t tiles cost each; with T tiles in
 // all and gw workgroups aimed at, each group is cut into ceil(t / share) parts,
 // share = max(ceil(T / gw), min_share), so that no workgroup has more than a share
-// whatever the lengths, and at most gw + (number of groups) slots are used.  A
-// session's last group, which sees the most keys, comes first.  Every wave works
-// it out for itself, 64 sessions at a time.
-template <bool kCausal, int kCols>
+// whatever the lengths, and at most gw + (number of groups) slots are used.  Every
+// wave works it out for itself, 64 sessions at a time.  The wide form, whose
+// workgroups are few and long, takes the sessions with the most keys first and a
+// session's last group, which sees the most of them, before its others, so that
+// the short ones fill the end.
+template <bool kCausal, int kCols, bool kSort>
 __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
     const int lane = threadIdx.x & 63;
     Session s{0, 0, 0, 0};
-    int tiles = 0, groups = 0;
+    int tiles = 0, groups = 0, index = lane;
     auto load = [&](int base) {
         s = Session{0, 0, 0, 0};
         if (base + lane < a.n_sess) s = session_of<kCausal>(a, base + lane);
+        if constexpr (kSort) {
+            const int n = min(a.n_sess - base, 64);
+            int rank = lane < n ? 0 : lane;
+            for (int j = 0; j < n; ++j) {
+                const int k = __builtin_amdgcn_readlane(s.keys, j);
+                if (lane < n) rank += k > s.keys || (k == s.keys && j < lane);
+            }
+            s.keys = __builtin_amdgcn_ds_permute(4 * rank, s.keys);
+            s.past = __builtin_amdgcn_ds_permute(4 * rank, s.past);
+            s.rows = __builtin_amdgcn_ds_permute(4 * rank, s.rows);
+            s.row0 = __builtin_amdgcn_ds_permute(4 * rank, s.row0);
+            index = __builtin_amdgcn_ds_permute(4 * rank, lane);
+        }
         tiles = (s.keys + TILE - 1) / TILE;
         groups = (s.rows * G + kCols - 1) / kCols;
     };
@@ -171,7 +187,7 @@ __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
         if (hit) {
             const int l = __builtin_ctzll(hit);
             Part p;
-            p.sess = base + l;
+            p.sess = base + __builtin_amdgcn_readlane(index, l);
             p.parts = __builtin_amdgcn_readlane(parts, l);
             const int n_groups = __builtin_amdgcn_readlane(groups, l);
             p.slot0 = __builtin_amdgcn_readlane(incl, l) - p.parts * n_groups;
@@ -284,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
     auto s_acc = [&](int w, int col, int d) { return reinterpret_cast<f4*>(s_wave[w] + (col * kAccRow + d) * 4); };
     const int kvh = blockIdx.x, slot = blockIdx.y;
-    const Part p = find_part<kCausal, COLS>(a, slot);
+    const Part p = find_part<kCausal, COLS, kWide>(a, slot);
     if (p.sess < 0) return;
     if (kvh == 0 && slot == p.slot0 && tid == 0) a.info[p.sess] = i4{p.slot0, p.parts, p.s.rows, p.s.row0};
     const int n_cols = p.s.rows * G;
@@ -521,51 +537,69 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
     }
 }
 
-// Joins the parts of a session's column that was cut: one workgroup per
-// (column, kv head, session), the waves taking every fourth part.
+// Joins the parts of the sessions that were cut.  Columns of all kv heads are
+// dealt out over the grid: a workgroup each, its waves taking every fourth part
+// (few columns, up to many parts), or a wave each (kWide: many columns).
+template <bool kWide>
 __global__ void __launch_bounds__(THREADS) q8_join_kernel(Q8Args a, int cols) {
     __shared__ f2 s_o[WAVES][64];
     __shared__ float s_l[WAVES], s_m[WAVES];
-    const int col = blockIdx.x, kvh = blockIdx.y, sess = blockIdx.z;
-    if (q8_count(a.rows, sess) == 0) return;
-    const i4 in = a.info[sess];
-    if (in[1] <= 1 || col >= in[2] * G) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int last_group = (in[2] * G - 1) / cols;
-    const int first = in[0] + (last_group - col / cols) * in[1];
-    if (first + in[1] > a.slots) return;                     // offsets that do not add up: more groups than rows allow
-    const int64_t base = ((int64_t)kvh * a.slots + first) * cols + col % cols;
-    float m = kUnset, l = 0.f;
-    f2 o = f2{0.f, 0.f};
-    for (int p = wave; p < in[1]; p += WAVES) {
-        const f2 x = a.ml[base + (int64_t)p * cols];
-        const f2 v = *reinterpret_cast<const f2*>(a.acc + (base + (int64_t)p * cols) * HD + 2 * lane);
-        const float to = fmaxf(m, x[0]);
-        const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
-        l = l * f0 + x[1] * f1;
-        o = o * f0 + v * f1;
-        m = to;
-    }
-    s_o[wave][lane] = o;
-    if (lane == 0) {
-        s_m[wave] = m;
-        s_l[wave] = l;
-    }
-    __syncthreads();
-    if (wave) return;
-    float mm = s_m[0];
+    const int first = kWide ? blockIdx.x * WAVES + wave : blockIdx.x, stride = kWide ? gridDim.x * WAVES : gridDim.x;
+    int64_t done = 0;                                        // columns of the sessions before this batch of 64
+    for (int base = 0; base < a.n_sess; base += 64) {
+        i4 in = i4{0, 0, 0, 0};
+        if (base + lane < a.n_sess && q8_count(a.rows, base + lane) > 0) in = a.info[base + lane];
+        const int mine = in[1] > 1 ? in[2] * NH : 0;
+        const int incl = scan_incl(mine);
+        const int all = __builtin_amdgcn_readlane(incl, 63);
+        int u = (int)((first + stride - done % stride) % stride);
+        for (; u < all; u += stride) {                       // uniform over the workgroup unless kWide
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > u));
+            const int e = u - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(mine, l));
+            const int slot0 = __builtin_amdgcn_readlane(in[0], l), parts = __builtin_amdgcn_readlane(in[1], l);
+            const int n_cols = __builtin_amdgcn_readlane(in[2], l) * G, row0 = __builtin_amdgcn_readlane(in[3], l);
+            const int kvh = e / n_cols, col = e % n_cols;
+            const int at = slot0 + ((n_cols - 1) / cols - col / cols) * parts;
+            if (at + parts > a.slots) continue;              // offsets that do not add up: more groups than rows allow
+            const int64_t from = ((int64_t)kvh * a.slots + at) * cols + col % cols;
+            float m = kUnset, ll = 0.f;
+            f2 o = f2{0.f, 0.f};
+            for (int p = kWide ? 0 : wave; p < parts; p += kWide ? 1 : WAVES) {
+                const f2 x = a.ml[from + (int64_t)p * cols];
+                const f2 v = *reinterpret_cast<const f2*>(a.acc + (from + (int64_t)p * cols) * HD + 2 * lane);
+                const float to = fmaxf(m, x[0]);
+                const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
+                ll = ll * f0 + x[1] * f1;
+                o = o * f0 + v * f1;
+                m = to;
+            }
+            if constexpr (!kWide) {
+                __syncthreads();                             // the last column has been read
+                s_o[wave][lane] = o;
+                if (lane == 0) {
+                    s_m[wave] = m;
+                    s_l[wave] = ll;
+                }
+                __syncthreads();
+                if (wave) continue;
+                m = s_m[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, s_m[w]);
-    f2 sum = f2{0.f, 0.f};
-    float ll = 0.f;
+                for (int w = 1; w < WAVES; ++w) m = fmaxf(m, s_m[w]);
+                o = f2{0.f, 0.f};
+                ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const float f = __builtin_amdgcn_exp2f(s_m[w] - mm);
-        sum += s_o[w][lane] * f;
-        ll += s_l[w] * f;
+                for (int w = 0; w < WAVES; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(s_m[w] - m);
+                    o += s_o[w][lane] * f;
+                    ll += s_l[w] * f;
+                }
+            }
+            const int r = col / G, hh = col - r * G;
+            *reinterpret_cast<f2*>(a.o + ((int64_t)(row0 + r) * NH + kvh * G + hh) * HD + 2 * lane) = o * (1.0f / ll);
+        }
+        done += all;
     }
-    const int r = col / G, hh = col - r * G;
-    *reinterpret_cast<f2*>(a.o + ((int64_t)(in[3] + r) * NH + kvh * G + hh) * HD + 2 * lane) = sum * (1.0f / ll);
 }
 
 // ---- host side ----
@@ -575,6 +609,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 constexpr int kFewCols = 64;                   // columns per session up to which a session's waves share them
 constexpr int kAimWgs = 512;                   // workgroups aimed at: two per CU
 constexpr int kMinShare = 4;                   // tiles: one per wave
+constexpr int kJoinWgs = 2048;                 // a launch full of the chip
 constexpr int kWideBlocks = 2;                 // 16-column blocks per wave of the wide form
 
 // What a call of these counts runs with: the columns of a workgroup and the
@@ -643,7 +678,10 @@ void launch(Q8Args a, void* workspace, hipStream_t s) {
     }
     if (f.blocks == 1) hipLaunchKernelGGL((q8_attn_kernel<1, kCausal, false>), grid, dim3(THREADS), 0, s, a);
     NOVA_LAUNCHED();
-    hipLaunchKernelGGL(q8_join_kernel, dim3(a.max_q * G, NKV, a.n_sess), dim3(THREADS), 0, s, a, f.cols);
+    const int64_t columns = (int64_t)a.rows.n_rows * NH;
+    const unsigned join = (unsigned)std::min<int64_t>(f.wide ? (columns + WAVES - 1) / WAVES : columns, kJoinWgs);
+    if (f.wide) hipLaunchKernelGGL(q8_join_kernel<true>, dim3(join), dim3(THREADS), 0, s, a, f.cols);
+    else hipLaunchKernelGGL(q8_join_kernel<false>, dim3(join), dim3(THREADS), 0, s, a, f.cols);
     NOVA_LAUNCHED();
 }
 
