@@ -26,14 +26,13 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int NH = Model::NH, NKV = Model::NKV, HD = Model::HD, G = Model::G;
 constexpr float kLog2e = 1.4426950408889634f;
-#ifndef Q8_WPS
-#define Q8_WPS (NB == 1 || kWide ? 2 : 1)
-#endif
 constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
+constexpr int kMinPiece = 4;                   // tiles of a group that is cut
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
+constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -1e30f;               // reference of a column without keys, where states are joined
 constexpr float kTop = 6.f, kLazy = 14.f;      // log2 of a column's largest weight: where it is put, where it may drift
 constexpr int kAccRow = HD + 4;                // floats per column in LDS: rows on different banks
@@ -49,11 +48,11 @@ struct Q8Args {
     int max_q;
     int n_sess;
     int nb;
-    int gw;                    // workgroups aimed at per kv head
+    int gw;                    // few columns: workgroups aimed at per kv head; many: workgroups per kv head
     int min_share;             // fewest tiles of a workgroup that shares a session
-    int slots;                 // workgroups launched per kv head
+    int slots;                 // partial results per kv head
     float* o;
-    i4* info;                  // [n_sess] {first slot, parts, rows, first row}
+    i4* info;                  // few: [n_sess] {first slot, parts, rows, first row}; many: [2 gw] pieces
     f2* ml;                    // [NKV][slots][cols] {reference, sum}
     float* acc;                // [NKV][slots][cols][HD]
 };
@@ -69,6 +68,29 @@ __device__ __forceinline__ int scan_incl(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row 0 -> 1, 2 -> 3
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // rows 0, 1 -> 2, 3
     return v;
+}
+
+// the same of doubles, whole numbers here, by their halves
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, kRows, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), kCtrl, kRows, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double scan_incl(double v) {
+    v += dpp<0x111, 0xf>(v);
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xa>(v);
+    v += dpp<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ double read_lane(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 // lane N of each row of 16
@@ -120,7 +142,7 @@ __device__ __forceinline__ Session session_of(const Q8Args& a, int i) {
     Session s;
     s.rows = min(q8_count(a.rows, i), a.max_q);
     s.row0 = q8_row0(a.rows, i);
-    const int n = max(a.n_keys[i], 0);
+    const int n = min(max(a.n_keys[i], 0), 1 << 30);
     const int64_t most = a.table_stride * kKvBlock, all = (int64_t)n + (kCausal ? s.rows : 0);
     s.keys = (int)(all < most ? all : most);
     s.past = kCausal ? n : s.keys - 1;
@@ -129,71 +151,47 @@ __device__ __forceinline__ Session session_of(const Q8Args& a, int i) {
 
 struct Part {
     int sess;                  // < 0: nothing to do
-    int index, parts;          // part `index` of `parts` of a column group's keys
-    int group;                 // column group of the session
-    int slot0;                 // the session's first slot
+    int index, parts;          // part `index` of `parts` of the session's keys
     Session s;
 };
 
-// columns of a workgroup: in the wide form each wave has its own
-template <int NB, bool kWide>
-constexpr int kGroupCols = 16 * NB * (kWide ? WAVES : 1);
-
-// The session, column group and part of a slot.  A session has
-// ceil(rows * G / cols) column groups, which its t tiles cost each; with T tiles in
-// all and gw workgroups aimed at, each group is cut into ceil(t / share) parts,
+// Few columns: the session and part of a slot.  With T tiles in the batch and gw
+// workgroups aimed at, a session of t tiles is cut into ceil(t / share) parts,
 // share = max(ceil(T / gw), min_share), so that no workgroup has more than a share
-// whatever the lengths, and at most gw + (number of groups) slots are used.  Every
-// wave works it out for itself, 64 sessions at a time.  The wide form, whose
-// workgroups are few and long, takes the sessions with the most keys first and a
-// session's last group, which sees the most of them, before its others, so that
-// the short ones fill the end.
-template <bool kCausal, int kCols, bool kSort>
+// whatever the lengths, and at most gw + n_sess slots are used.  Every wave works it
+// out for itself, 64 sessions at a time.
+template <bool kCausal>
 __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
     const int lane = threadIdx.x & 63;
     Session s{0, 0, 0, 0};
-    int tiles = 0, groups = 0, index = lane;
+    int tiles = 0;
     auto load = [&](int base) {
         s = Session{0, 0, 0, 0};
         if (base + lane < a.n_sess) s = session_of<kCausal>(a, base + lane);
-        if constexpr (kSort) {
-            const int n = min(a.n_sess - base, 64);
-            int rank = lane < n ? 0 : lane;
-            for (int j = 0; j < n; ++j) {
-                const int k = __builtin_amdgcn_readlane(s.keys, j);
-                if (lane < n) rank += k > s.keys || (k == s.keys && j < lane);
-            }
-            s.keys = __builtin_amdgcn_ds_permute(4 * rank, s.keys);
-            s.past = __builtin_amdgcn_ds_permute(4 * rank, s.past);
-            s.rows = __builtin_amdgcn_ds_permute(4 * rank, s.rows);
-            s.row0 = __builtin_amdgcn_ds_permute(4 * rank, s.row0);
-            index = __builtin_amdgcn_ds_permute(4 * rank, lane);
-        }
-        tiles = (s.keys + TILE - 1) / TILE;
-        groups = (s.rows * G + kCols - 1) / kCols;
+        tiles = s.rows > 0 ? (s.keys + TILE - 1) / TILE : 0;
     };
     int total = 0;
     for (int base = 0; base < a.n_sess; base += 64) {
         load(base);
-        total += __builtin_amdgcn_readlane(scan_incl(tiles * groups), 63);
+        total += __builtin_amdgcn_readlane(scan_incl(tiles), 63);
     }
-    const int share = max((total + a.gw - 1) / a.gw, a.min_share);
+    // Whole tiles for each wave (nine tiles last as long as twelve), and no more parts
+    // than workgroups that run at once: one that has to wait doubles the time.
+    int share = (max((total + a.gw - 1) / a.gw, a.min_share) + WAVES - 1) / WAVES * WAVES;
+    if (a.n_sess <= 64)
+        while (__builtin_amdgcn_readlane(scan_incl((tiles + share - 1) / share), 63) > a.gw && share < total) share += WAVES;
     int before = 0;
     for (int base = 0; base < a.n_sess; base += 64) {
         if (a.n_sess > 64) load(base);
-        const int parts = max((tiles + share - 1) / share, 1);
-        const int incl = before + scan_incl(parts * groups);
+        const int parts = s.rows > 0 ? max((tiles + share - 1) / share, 1) : 0;
+        const int incl = before + scan_incl(parts);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > slot);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             Part p;
-            p.sess = base + __builtin_amdgcn_readlane(index, l);
+            p.sess = base + l;
             p.parts = __builtin_amdgcn_readlane(parts, l);
-            const int n_groups = __builtin_amdgcn_readlane(groups, l);
-            p.slot0 = __builtin_amdgcn_readlane(incl, l) - p.parts * n_groups;
-            const int e = slot - p.slot0;
-            p.group = n_groups - 1 - e / p.parts;
-            p.index = e % p.parts;
+            p.index = slot - (__builtin_amdgcn_readlane(incl, l) - p.parts);
             p.s.keys = __builtin_amdgcn_readlane(s.keys, l);
             p.s.past = __builtin_amdgcn_readlane(s.past, l);
             p.s.rows = __builtin_amdgcn_readlane(s.rows, l);
@@ -202,7 +200,96 @@ __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
         }
         before = __builtin_amdgcn_readlane(incl, 63);
     }
-    return Part{-1, 0, 0, 0, 0, {0, 0, 0, 0}};
+    return Part{-1, 0, 0, {0, 0, 0, 0}};
+}
+
+// Many columns: a session's columns in groups of C = kManyCols, group g over the keys up to its
+// last row's.  The batch's work is one line, group after group, of which each
+// workgroup gets the same length, so a group may be shared by workgroups that
+// follow each other, and each of them has at most two groups in part.  The cost of
+// group g is counted as G past + C (g + 1) (G times the keys its last row sees,
+// where rows do not end inside a group), whose sums have a closed form; everything
+// is in whole numbers, so that neighbours agree on where one stops and the other begins.
+struct Place {
+    int sess, group, tile;     // sess == n_sess: the end
+};
+
+__device__ __forceinline__ Place uniform(const Place& p) {
+    return Place{__builtin_amdgcn_readfirstlane(p.sess), __builtin_amdgcn_readfirstlane(p.group),
+                 __builtin_amdgcn_readfirstlane(p.tile)};
+}
+
+__device__ __forceinline__ int n_groups(const Session& s) {
+    return (s.rows * G + kManyCols - 1) / kManyCols;
+}
+// tiles of group g
+__device__ __forceinline__ int group_tiles(const Session& s, int g) {
+    return (min(s.past + (min((g + 1) * kManyCols, s.rows * G) - 1) / G + 1, s.keys) + TILE - 1) / TILE;
+}
+// Cost of the first n groups, in a double: whole numbers below 2^53, exact.
+__device__ __forceinline__ double groups_cost(const Session& s, int n) {
+    return (double)n * ((double)G * s.past) + 0.5 * kManyCols * ((double)n * (n + 1));
+}
+
+// where cost x of the line lies in session s, which begins at x = 0
+__device__ __forceinline__ void place_in(const Session& s, double x, Place& p) {
+    const double half = 0.5 * kManyCols, b = (double)G * s.past + half;
+    int g = (int)((__builtin_sqrt(b * b + 4.0 * half * x) - b) / (2.0 * half));      // an estimate
+    g = min(max(g, 0), n_groups(s) - 1);
+    while (g > 0 && groups_cost(s, g) > x) --g;
+    while (g + 1 < n_groups(s) && groups_cost(s, g + 1) <= x) ++g;
+    const double lo = groups_cost(s, g), cost = groups_cost(s, g + 1) - lo;
+    const int tiles = group_tiles(s, g);
+    // no piece of fewer than kMinPiece tiles: it would cost more than it evens out
+    int t = min((int)(((x - lo) * tiles) / cost), tiles);
+    t = t < kMinPiece ? 0 : tiles - t < kMinPiece ? tiles : t;
+    p.group = g;
+    p.tile = t;
+}
+
+// The stretch of workgroup w: from `from` to before `to`.  The grid's gw workgroups
+// are all used where each gets min_share tiles or more.
+__device__ __forceinline__ void find_stretch(const Q8Args& a, int w, Place& from, Place& to) {
+    const int lane = threadIdx.x & 63;
+    Session s{0, 0, 0, 0};
+    double incl = 0;
+    auto load = [&](int base) {                              // costs up to and with the lane's session
+        s = Session{0, 0, 0, 0};
+        if (base + lane < a.n_sess) s = session_of<true>(a, base + lane);
+        incl = scan_incl(groups_cost(s, n_groups(s)));
+    };
+    double total = 0;
+    for (int base = 0; base < a.n_sess; base += 64) {
+        load(base);
+        total += read_lane(incl, 63);
+    }
+    const int use = (int)fmin((double)a.gw, fmax(total / ((double)(G * TILE) * a.min_share), 1.0));
+    from = to = Place{a.n_sess, 0, 0};
+    if (w >= use) return;
+    // whole numbers, the same for the workgroup that stops here and the one that starts
+    const double x0 = __builtin_floor((total * w) / use), x1 = __builtin_floor((total * (w + 1)) / use);
+    double before = 0;
+    for (int base = 0; base < a.n_sess; base += 64) {
+        if (a.n_sess > 64) load(base);
+        auto find = [&](double x, Place& p) {
+            x -= before;
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > x);
+            if (x < 0 || !hit) return;
+            const int l = __builtin_ctzll(hit);
+            Session t;
+            t.keys = __builtin_amdgcn_readlane(s.keys, l);
+            t.past = __builtin_amdgcn_readlane(s.past, l);
+            t.rows = __builtin_amdgcn_readlane(s.rows, l);
+            t.row0 = 0;
+            p.sess = base + l;
+            place_in(t, x - (read_lane(incl, l) - groups_cost(t, n_groups(t))), p);
+        };
+        find(x0, from);
+        find(x1, to);
+        before += read_lane(incl, 63);
+    }
+    from = uniform(from);
+    to = uniform(to);
 }
 
 // ---- operands ----
@@ -233,26 +320,25 @@ __device__ __forceinline__ void q_digits(const f4 (&x)[2][4], QDigits& out) {
     int ex = 0;
     const float m = live ? frexpf(__uint_as_float(top), &ex) : 1.f;    // largest = m 2^ex, m in [1/2, 1)
     constexpr float kUnit = 127.f * 65536.f;
-    const float f = kUnit / m;
+    // the factor in two steps, so that neither leaves fp32 (the first is a power of two)
+    const float f0 = live ? ldexpf(1.f, min(max(-ex, -126), 126)) : 0.f, f1 = live ? ldexpf(kUnit / m, -ex - min(max(-ex, -126), 126)) : 0.f;
     out.scale = finite ? ldexpf(m * (kScale * kLog2e / kUnit), ex) : __builtin_nanf("");
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            uint32_t y[4];
+            uint32_t y[4];                                   // digits plus 128 in bytes 2, 1, 0
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float v = live ? ldexpf(x[h][j][e], -ex) * f : 0.f;
-                y[e] = (uint32_t)((int)__builtin_rintf(v) + 0x808080);   // digits plus 128
+                const float v = finite ? x[h][j][e] * f0 * f1 : 0.f;
+                y[e] = (uint32_t)((int)__builtin_rintf(v) + 0x808080);
             }
-            // byte 2, 1, 0 of the four integers, 128 taken off again
-#pragma unroll
-            for (int d = 0; d < 3; ++d) {
-                const int sh = 16 - 8 * d;
-                const uint32_t w = ((y[0] >> sh) & 255) | ((y[1] >> sh) & 255) << 8 | ((y[2] >> sh) & 255) << 16 |
-                                   ((y[3] >> sh) & 255) << 24;
-                out.d[d][h][j] = (int)(w ^ 0x80808080u);
-            }
+            // bytes of (y0, y1) and of (y2, y3) side by side, then the four of a digit
+            const uint32_t a = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), b = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+            const uint32_t c = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), d = __builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u);
+            out.d[0][h][j] = (int)(__builtin_amdgcn_perm(d, c, 0x05040100u) ^ 0x80808080u);
+            out.d[1][h][j] = (int)(__builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u);
+            out.d[2][h][j] = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
         }
 }
 
@@ -273,7 +359,8 @@ __device__ __forceinline__ void split_f16(const float (&e)[8], h8& hi, h8& lo) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[j], e[j + 1]));
-        const h2 r = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(e[j] - (float)h[0], e[j + 1] - (float)h[1]));
+        const float r0 = __builtin_fmaf((float)h[0], -1.f, e[j]), r1 = __builtin_fmaf((float)h[1], -1.f, e[j + 1]);
+        const h2 r = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(r0, r1));
         hi[j] = h[0];
         hi[j + 1] = h[1];
         lo[j] = r[0];
@@ -281,184 +368,229 @@ __device__ __forceinline__ void split_f16(const float (&e)[8], h8& hi, h8& lo) {
     }
 }
 
-// ---- the kernel ----
-//
-// A wave has NB blocks of 16 columns (query rows x heads of a kv head) and takes
-// 64 keys at a time.  Few columns (!kWide): the workgroup's waves share the
-// session's columns and each takes its own keys, so K and V are read once and
-// bound everything.  Many columns (kWide): each wave has its own 16 NB columns and
-// all go over the same keys.
-template <int NB, bool kCausal, bool kWide>
-__global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
-    constexpr int COLS = kGroupCols<NB, kWide>;
-    // in the wide form the query's digits stay in LDS, 1 KiB per operand, which the
-    // results overwrite at the end; otherwise they stay in registers
-    constexpr int kQOps = 6 * NB;
-    constexpr int kWaveLds = kWide && kQOps * 1024 > 16 * kAccRow * 4 ? kQOps * 1024 : 16 * kAccRow * 4;
-    __shared__ __attribute__((aligned(16))) unsigned char s_wave[WAVES][kWaveLds];
-    __shared__ float s_m[WAVES][16 * NB], s_l[WAVES][16 * NB];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
-    auto s_acc = [&](int w, int col, int d) { return reinterpret_cast<f4*>(s_wave[w] + (col * kAccRow + d) * 4); };
-    const int kvh = blockIdx.x, slot = blockIdx.y;
-    const Part p = find_part<kCausal, COLS, kWide>(a, slot);
-    if (p.sess < 0) return;
-    if (kvh == 0 && slot == p.slot0 && tid == 0) a.info[p.sess] = i4{p.slot0, p.parts, p.s.rows, p.s.row0};
-    const int n_cols = p.s.rows * G;
-    const int col0 = kWide ? p.group * COLS + wave * 16 * NB : 0;            // this wave's columns
-    // the group's tiles, the part's of them, and this wave's of those
-    const int group_keys = kCausal && kWide ? min(p.s.past + min(p.group * COLS + COLS - 1, n_cols - 1) / G + 1, p.s.keys) : p.s.keys;
-    const int tiles = (group_keys + TILE - 1) / TILE;
-    const int t_lo = (int)((int64_t)tiles * p.index / p.parts), t_hi = (int)((int64_t)tiles * (p.index + 1) / p.parts);
-    int t0 = t_lo, t1 = t_hi;
-    if constexpr (kWide) {
-        const int wave_keys = min(p.s.past + min(col0 + 16 * NB - 1, n_cols - 1) / G + 1, p.s.keys);
-        t1 = col0 < n_cols ? min(t_hi, (wave_keys + TILE - 1) / TILE) : t_lo;
-    } else {
-        t0 = t_lo + (t_hi - t_lo) * wave / WAVES;
-        t1 = t_lo + (t_hi - t_lo) * (wave + 1) / WAVES;
-    }
-    const int clear_keys = min(p.s.past + col0 / G + 1, p.s.keys);             // keys below: seen by all of the wave's columns
-    const int32_t* table = a.tables + p.sess * a.table_stride;
-    const int last_page = (p.s.keys - 1) >> kKvBlockShift;
-
-    // Pages of a tile: lane (g, c) reads K rows of page c >> 2 and V columns and
-    // scales of page g.  64 table entries at a time stay in a register.
-    int win = -64, win_pages = 0;
-    auto phys = [&](int pg) {                                // pg: per lane, within the window
-        const int v = __shfl(win_pages, min(pg, last_page) - win, 64);
-        return (unsigned)v < (unsigned)a.nb ? v : 0;
-    };
-    const uint8_t* k_at;
-    const uint8_t* v_at;
-    auto locate = [&](int t) {
-        const int pg = t * kTilePages;
-        if (pg + kTilePages > win + 64) {                    // uniform
-            win = pg;
-            win_pages = table[min(pg + lane, last_page)];
+// The query rows of a block's column, lane (g, c) its dims 64 h + 16 g .. + 15.
+__device__ __forceinline__ void load_q(const Q8Args& a, const Session& s, int kvh, int col, QDigits& out, int& seen) {
+    const bool real = col < s.rows * G;
+    const int r = real ? col / G : 0, hh = real ? col - r * G : 0;
+    const float* src = a.q + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + 16 * ((threadIdx.x & 63) >> 4);
+    f4 x[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[h][j] = *reinterpret_cast<const f4*>(src + 64 * h + 4 * j);
+            if (!real) x[h][j] = f4{0.f, 0.f, 0.f, 0.f};
         }
-        const uint8_t* head = a.pool + kvh * kQ8Rec;
-        k_at = head + phys(pg + (c >> 2)) * kQ8Page + g * 64 + (c & 3) * 16;
-        v_at = head + phys(pg + g) * kQ8Page;
-    };
-    i4 kr[8], vr[DB];
-    float ks, vs;
-    auto load_k = [&] {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) kr[u] = *reinterpret_cast<const i4*>(k_at + 256 * u);
-        ks = *reinterpret_cast<const float*>(v_at + kQ8KsOff + 4 * c);
-    };
-    auto load_v = [&] {
-        vs = *reinterpret_cast<const float*>(v_at + kQ8VsOff + 4 * c);
-#pragma unroll
-        for (int u = 0; u < DB; ++u) vr[u] = *reinterpret_cast<const i4*>(v_at + kQ8VOff + 256 * u + 16 * c);
-    };
-    if (t0 < t1) {
-        locate(t0);
-        load_k();
-        load_v();
-    }
+    q_digits(x, out);
+    seen = real ? min(s.past + r + 1, s.keys) : 0;
+}
 
-    QDigits q[NB];
-    int seen[NB];              // keys that the column sees
-    // running reference and sum of the column; a score above `limit` moves the reference
-    float m[NB], l[NB], limit[NB];
-    f4 acc[NB][DB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int col = col0 + 16 * b + c;
-        const bool real = col < n_cols;
-        const int r = real ? col / G : 0, hh = real ? col - r * G : 0;
-        const float* src = a.q + ((int64_t)(p.s.row0 + r) * NH + kvh * G + hh) * HD + 16 * g;
-        f4 x[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[h][j] = *reinterpret_cast<const f4*>(src + 64 * h + 4 * j);
-                if (!real) x[h][j] = f4{0.f, 0.f, 0.f, 0.f};
-            }
-        q_digits(x, q[b]);
-        if constexpr (kWide)
-#pragma unroll
-            for (int e = 0; e < 6; ++e)
-                *reinterpret_cast<i4*>(s_wave[wave] + (6 * b + e) * 1024 + 16 * lane) = q[b].d[e / 2][e % 2];
-        seen[b] = real ? min(p.s.past + r + 1, p.s.keys) : 0;
-        m[b] = l[b] = 0.f;
-        limit[b] = -INFINITY;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) acc[b][d] = f4{0.f, 0.f, 0.f, 0.f};
+// Table entries, 64 at a time in a register: page pg (per lane, not before the
+// last call's) of the session.
+struct Pages {
+    const int32_t* table;
+    int last, nb;              // the last page with a key; pages of the pool
+    int win, held;
+    __device__ __forceinline__ Pages(const Q8Args& a, int sess, int keys)
+        : table(a.tables + sess * a.table_stride), last((keys - 1) >> kKvBlockShift), nb(a.nb), win(-64), held(0) {}
+    __device__ __forceinline__ void reach(int pg) {          // uniform: pages pg .. pg + 3 come next
+        if (pg + kTilePages > win + 64) {
+            win = pg;
+            held = table[min(pg + (int)(threadIdx.x & 63), last)];
+        }
     }
+    // page of the pool; an entry outside it reads page 0
+    __device__ __forceinline__ int operator[](int pg) const {
+        const int v = __shfl(held, min(pg, last) - win, 64);
+        return (unsigned)v < (unsigned)nb ? v : 0;
+    }
+};
 
-    auto q_op = [&](int b, int d, int h) -> i4 {
-        if constexpr (kWide) return *reinterpret_cast<const i4*>(s_wave[wave] + (6 * b + 2 * d + h) * 1024 + 16 * lane);
-        else return q[b].d[d][h];
-    };
+// A block's state over the keys seen so far: lane (g, c) holds the reference, its
+// share of the sum and dims 16 d + 4 g .. + 3 of column c.  A score above `limit`
+// moves the reference (a column's first one always).
+struct State {
+    float m, l, limit;
+    f4 acc[DB];
+    __device__ __forceinline__ void clear() {
+        m = l = 0.f;
+        limit = -INFINITY;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ float reference() const { return limit == kLazy ? m : kUnset; }
+    __device__ __forceinline__ void scale_acc(float f) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] *= f;
+    }
+};
+
+// The weights meet V's codes as 2^(s - m) vs, which have to stay inside fp16.  So V's
+// scales are taken relative to a power of two, `unit`, the same for all columns of a
+// wave: it moves up (and the accumulators with it) when a scale passes twice its
+// size, and stands at the first tile's largest scale to begin with.
+struct ValueUnit {
+    float unit, most;          // most: the scale that moves it
+    __device__ __forceinline__ void clear() {
+        unit = 1.f;
+        most = 0.f;
+    }
+    // vs: scale of the lane's key, 0 where there is none; returns it in units
+    template <int NB>
+    __device__ __forceinline__ float take(float vs, State (&st)[NB]) {
+        if (__builtin_amdgcn_ballot_w64(vs > most)) {        // rare
+            float top = vs;                                  // (a NaN does not count)
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            int ex;
+            (void)frexpf(top, &ex);
+            const float to = ldexpf(1.f, ex);                // top < to
+            const float f = most == 0.f ? 0.f : unit / to;   // before the first scale there is nothing to keep
+#pragma unroll
+            for (int b = 0; b < NB; ++b) st[b].scale_acc(f);
+            unit = to;
+            most = 2.f * to;
+        }
+        return vs * (1.f / unit);
+    }
+};
+
+// Scores, weights and sum of one tile and block.  k_op(u): K operand u = 2 kb + h
+// (dims 64 h .. of key block kb), q_op(d, h): the query's; ks and vs: the K scale of
+// the lane's key and its V scale in units; key0: first key of the lane's page.  The
+// weights come out in two fp16 terms, so that V's codes can follow as they are.
+template <bool kMask, class K, class Q>
+__device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float ks, float vs, int key0, int seen, State& st,
+                                      h8 (&hi)[2], h8 (&lo)[2]) {
     // The lowest digit's sum starts at the bits of 1.5 * 2^23, so that it is that
     // float plus the sum without a conversion; the middle one starts 1.5 * 2^23 / 256
     // lower, which takes it off again.
     const i4 kLow = i4{0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000}, kMid = i4{-49152, -49152, -49152, -49152};
+    float x[16];
+    float top = -INFINITY;
+    // row 4g + i of key block kb: token 4 kb + i of page g.  The matrix instructions
+    // of a key block go out before the vector instructions of the one before it.
+    each<4>([&](auto kb) {
+        i4 z[3] = {i4{0, 0, 0, 0}, kMid, kLow};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const i4 k = k_op(2 * kb + h);
+#pragma unroll
+            for (int d = 0; d < 3; ++d) z[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q_op(d, h), z[d], 0, 0, 0);
+        }
+        each<4>([&](auto i) {
+            constexpr int e = i, j = 4 * kb + i;
+            const float w = fmaf((float)((z[0][e] << 8) + z[1][e]), 256.f, __int_as_float(z[2][e])) * row_lane<j>(ks);
+            x[j] = fmaf(w, q_scale, -st.m);
+            if (kMask && key0 + j >= seen) x[j] = -INFINITY;
+            top = fmaxf(top, x[j]);
+        });
+    });
+    if (__builtin_amdgcn_ballot_w64(top > st.limit)) {
+        // rare: a column's first keys, and a score more than kLazy above the
+        // reference, put it to kTop below the largest score
+        const float col_top = rows_max(top);
+        const bool moves = col_top > st.limit;
+        const float by = moves ? col_top - kTop : 0.f;
+        const float corr = st.limit == kLazy ? __builtin_amdgcn_exp2f(-by) : 0.f;
+        st.m += by;
+        st.limit = moves ? kLazy : st.limit;
+        st.l *= corr;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] -= by;
+        st.scale_acc(corr);
+    }
+    float e[2][8];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    each<16>([&](auto j) {
+        const float w = __builtin_amdgcn_exp2f(x[j]);
+        sum[j / 4] += w;
+        // (the cross-lane read is not for the lanes of one side of a branch)
+        const float y = w * row_lane<j>(vs);
+        e[j / 8][j % 8] = kMask && key0 + j >= seen ? 0.f : y;   // a hidden value may be NaN
+    });
+    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    split_f16(e[0], hi[0], lo[0]);
+    split_f16(e[1], hi[1], lo[1]);
+}
+
+template <bool kOnce>
+__device__ __forceinline__ i4 page_load(const uint8_t* p) {
+    if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const i4*>(p));
+    else return *reinterpret_cast<const i4*>(p);
+}
+
+// ---- few columns ----
+//
+// Up to 16 NB columns (query rows x heads of a kv head) of a session: the
+// workgroup's waves share them and each takes its own keys, 64 at a time, so K and
+// V are read once and bound everything.  The operands come straight from the
+// pages; the next tile's K loads go out behind the scores, V's behind the
+// products, into the registers that these have just read.  kOnce: non-temporal
+// loads, for pools that no cache holds until the next step (see launch()).
+template <int NB, bool kCausal, bool kOnce>
+__global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q8_few_kernel(Q8Args a) {
+    constexpr int COLS = 16 * NB;
+    __shared__ __attribute__((aligned(16))) float s_acc[WAVES][16][kAccRow];
+    __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int kvh = blockIdx.x, slot = blockIdx.y;
+    const Part p = find_part<kCausal>(a, slot);
+    if (p.sess < 0) return;
+    if (kvh == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
+    const int n_cols = p.s.rows * G;
+    // the part's tiles, and this wave's of them
+    const int tiles = (p.s.keys + TILE - 1) / TILE;
+    const int t_lo = (int)((int64_t)tiles * p.index / p.parts), t_hi = (int)((int64_t)tiles * (p.index + 1) / p.parts);
+    const int t0 = t_lo + (t_hi - t_lo) * wave / WAVES, t1 = t_lo + (t_hi - t_lo) * (wave + 1) / WAVES;
+    const int clear_keys = min(p.s.past + 1, p.s.keys);      // keys below: seen by all columns
+
+    // lane (g, c) reads K rows of page c >> 2 and V columns and scales of page g
+    Pages pages(a, p.sess, p.s.keys);
+    const uint8_t *k_at = nullptr, *v_at = nullptr;
+    i4 kr[8], vr[DB];
+    float ks = 0.f, vs = 0.f;
+    auto load_k = [&](int t) {
+        const int pg = t * kTilePages;
+        pages.reach(pg);
+        const uint8_t* head = a.pool + kvh * kQ8Rec;
+        k_at = head + pages[pg + (c >> 2)] * kQ8Page + g * 64 + (c & 3) * 16;
+        v_at = head + pages[pg + g] * kQ8Page;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) kr[u] = page_load<kOnce>(k_at + 256 * u);
+        ks = *reinterpret_cast<const float*>(v_at + kQ8KsOff + 4 * c);
+        vs = *reinterpret_cast<const float*>(v_at + kQ8VsOff + 4 * c);
+    };
+    auto load_v = [&] {
+#pragma unroll
+        for (int u = 0; u < DB; ++u) vr[u] = page_load<kOnce>(v_at + kQ8VOff + 256 * u + 16 * c);
+    };
+    if (t0 < t1) {
+        load_k(t0);
+        load_v();
+    }
+    QDigits q[NB];
+    int seen[NB];              // keys that the column sees
+    State st[NB];
+    ValueUnit unit;
+    unit.clear();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        load_q(a, p.s, kvh, 16 * b + c, q[b], seen[b]);
+        st[b].clear();
+    }
     auto step = [&](auto mask_tag, int t) {
         constexpr bool kMask = decltype(mask_tag)::value;
-        if constexpr (kWide) asm volatile("" ::: "memory");  // the digits are read anew, not kept in 48 registers
         const int key0 = t * TILE + 16 * g;
-        // lane (g, c) has the scales of token c of page g; a key behind the last
-        // one may hold anything
-        float sv = vs == 0.f ? 0x1p-20f : vs;
-        if (kMask && key0 + c >= p.s.keys) sv = 1.f;
-        const float lv = __builtin_amdgcn_logf(sv), inv = __builtin_amdgcn_rcpf(sv);
+        // (a key behind the last one may hold anything)
+        const float sv = unit.take(!kMask || key0 + c < p.s.keys ? vs : 0.f, st);
         h8 hi[NB][2], lo[NB][2];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            // scores: key block kb has row 4g + i = token 4 kb + i of page g
-            float x[16];
-            float top = -INFINITY;
-            each<4>([&](auto kb) {
-                i4 z[3] = {i4{0, 0, 0, 0}, kMid, kLow};
-#pragma unroll
-                for (int d = 0; d < 3; ++d)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        z[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[2 * kb + h], q_op(b, d, h), z[d], 0, 0, 0);
-                each<4>([&](auto i) {
-                    constexpr int e = i, j = 4 * kb + i;
-                    const float w = fmaf((float)((z[0][e] << 8) + z[1][e]), 256.f, __int_as_float(z[2][e])) * row_lane<j>(ks);
-                    x[j] = fmaf(w, q[b].scale, row_lane<j>(lv) - m[b]);
-                    if (kMask && key0 + j >= seen[b]) x[j] = -INFINITY;
-                    top = fmaxf(top, x[j]);
-                });
-            });
-            if (__builtin_amdgcn_ballot_w64(top > limit[b])) {
-                // rare: a column's first keys, and a score more than kLazy above the
-                // reference, put it to kTop below the largest score
-                const float col_top = rows_max(top);
-                const bool moves = col_top > limit[b];
-                const float by = moves ? col_top - kTop : 0.f;
-                const float corr = limit[b] == kLazy ? __builtin_amdgcn_exp2f(-by) : 0.f;
-                m[b] += by;
-                limit[b] = moves ? kLazy : limit[b];
-                l[b] *= corr;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] -= by;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[b][d] *= corr;
-            }
-            float e[2][8];
-            each<16>([&](auto j) {
-                const float w = __builtin_amdgcn_exp2f(x[j]);
-                e[j / 8][j % 8] = w;
-                // (the cross-lane read is not for the lanes of one side of a branch)
-                const float share = row_lane<j>(inv) * w;
-                if (kMask) l[b] += key0 + j >= seen[b] ? 0.f : share;
-                else l[b] += share;
-            });
-            split_f16(e[0], hi[b][0], lo[b][0]);
-            split_f16(e[1], hi[b][1], lo[b][1]);
-        }
+        for (int b = 0; b < NB; ++b)
+            weigh<kMask>([&](int u) { return kr[u]; }, [&](int d, int h) { return q[b].d[d][h]; }, q[b].scale, ks, sv, key0, seen[b], st[b], hi[b],
+                         lo[b]);
         const bool more = t + 1 < t1;
-        if (more) {
-            locate(t + 1);
-            load_k();
-        }
+        if (more) load_k(t + 1);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -466,8 +598,8 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
                 const h8 v = codes_f16((uint32_t)vr[d][2 * u], (uint32_t)vr[d][2 * u + 1]);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    acc[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[b][u], acc[b][d], 0, 0, 0);
-                    acc[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[b][u], acc[b][d], 0, 0, 0);
+                    st[b].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[b][u], st[b].acc[d], 0, 0, 0);
+                    st[b].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[b][u], st[b].acc[d], 0, 0, 0);
                 }
             }
         if (more) load_v();
@@ -476,76 +608,57 @@ __global__ void __launch_bounds__(THREADS, Q8_WPS) q8_attn_kernel(Q8Args a) {
     for (int t = t0; t < t_clear; ++t) step(std::false_type{}, t);
     for (int t = t_clear; t < t1; ++t) step(std::true_type{}, t);
 
-    // ---- the waves' results through LDS: each wave's own columns, or the four
-    // states of the same columns joined; a lone part writes the output ----
-    const bool lone = p.parts == 1;
-    auto put = [&](int col, int d4, f4 sum, float mm, float ll) {            // col of the session
-        if (lone) {
-            const int r = col / G, hh = col - r * G;
-            const float n = p.s.keys > 0 ? 1.0f / ll : 0.f;
-            *reinterpret_cast<f4*>(a.o + ((int64_t)(p.s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d4) = sum * n;
-        } else {
-            const int64_t at = ((int64_t)kvh * a.slots + slot) * COLS + col - p.group * COLS;
-            *reinterpret_cast<f4*>(a.acc + at * HD + 4 * d4) = sum;
-            if (d4 == 0) a.ml[at] = f2{mm, ll};
-        }
-    };
+    // the four waves' states joined in LDS; a lone part writes the output
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        l[b] = rows_sum(l[b]);
+        const float l = rows_sum(st[b].l);
+        st[b].scale_acc(unit.unit);
         if (g == 0) {
-            s_m[wave][16 * b + c] = limit[b] == kLazy ? m[b] : kUnset;
-            s_l[wave][16 * b + c] = l[b];
+            s_m[wave][16 * b + c] = st[b].reference();
+            s_l[wave][16 * b + c] = l;
         }
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        if (col0 + 16 * b >= n_cols) break;                  // the same for all waves unless kWide
-        if (b > 0 && !kWide) __syncthreads();
-        if (col0 + 16 * b + c < n_cols)
+        if (16 * b >= n_cols) break;                         // uniform
+        if (b > 0) __syncthreads();
+        if (16 * b + c < n_cols)
 #pragma unroll
-            for (int d = 0; d < DB; ++d) *s_acc(wave, c, 16 * d + 4 * g) = acc[b][d];
-        if constexpr (kWide) {
-            wave_lds_sync();
-#pragma unroll
-            for (int e = lane; e < 16 * (HD / 4); e += 64) {
-                const int cc = e / (HD / 4), d4 = e % (HD / 4), col = col0 + 16 * b + cc;
-                if (col < n_cols)
-                    put(col, d4, *s_acc(wave, cc, 4 * d4), s_m[wave][16 * b + cc],
-                        s_l[wave][16 * b + cc]);
-            }
-            wave_lds_sync();
-            continue;
-        }
+            for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(&s_acc[wave][c][16 * d + 4 * g]) = st[b].acc[d];
         __syncthreads();
         for (int e = tid; e < 16 * (HD / 4); e += THREADS) {
             const int cc = e / (HD / 4), d4 = e % (HD / 4), col = 16 * b + cc;
             if (col >= n_cols) continue;
-            float mm = s_m[0][col];
+            float m = s_m[0][col];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, s_m[w][col]);
+            for (int w = 1; w < WAVES; ++w) m = fmaxf(m, s_m[w][col]);
             f4 sum = f4{0.f, 0.f, 0.f, 0.f};
-            float ll = 0.f;
+            float l = 0.f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(s_m[w][col] - mm);
-                sum += *s_acc(w, cc, 4 * d4) * f;
-                ll += s_l[w][col] * f;
+                const float f = __builtin_amdgcn_exp2f(s_m[w][col] - m);
+                sum += *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]) * f;
+                l += s_l[w][col] * f;
             }
-            put(col, d4, sum, mm, ll);
+            if (p.parts == 1) {
+                const int r = col / G, hh = col - r * G;
+                const float n = p.s.keys > 0 ? 1.0f / l : 0.f;
+                *reinterpret_cast<f4*>(a.o + ((int64_t)(p.s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d4) = sum * n;
+            } else {
+                const int64_t at = ((int64_t)kvh * a.slots + slot) * COLS + col;
+                *reinterpret_cast<f4*>(a.acc + at * HD + 4 * d4) = sum;
+                if (d4 == 0) a.ml[at] = f2{m, l};
+            }
         }
     }
 }
 
-// Joins the parts of the sessions that were cut.  Columns of all kv heads are
-// dealt out over the grid: a workgroup each, its waves taking every fourth part
-// (few columns, up to many parts), or a wave each (kWide: many columns).
-template <bool kWide>
-__global__ void __launch_bounds__(THREADS) q8_join_kernel(Q8Args a, int cols) {
+// Joins the parts of the sessions that were cut: a workgroup per column of all kv
+// heads, its waves taking every fourth part.
+__global__ void __launch_bounds__(THREADS) q8_few_join_kernel(Q8Args a, int cols) {
     __shared__ f2 s_o[WAVES][64];
     __shared__ float s_l[WAVES], s_m[WAVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int first = kWide ? blockIdx.x * WAVES + wave : blockIdx.x, stride = kWide ? gridDim.x * WAVES : gridDim.x;
     int64_t done = 0;                                        // columns of the sessions before this batch of 64
     for (int base = 0; base < a.n_sess; base += 64) {
         i4 in = i4{0, 0, 0, 0};
@@ -553,19 +666,18 @@ __global__ void __launch_bounds__(THREADS) q8_join_kernel(Q8Args a, int cols) {
         const int mine = in[1] > 1 ? in[2] * NH : 0;
         const int incl = scan_incl(mine);
         const int all = __builtin_amdgcn_readlane(incl, 63);
-        int u = (int)((first + stride - done % stride) % stride);
-        for (; u < all; u += stride) {                       // uniform over the workgroup unless kWide
+        int u = (int)((blockIdx.x + gridDim.x - done % gridDim.x) % gridDim.x);
+        for (; u < all; u += gridDim.x) {                    // uniform over the workgroup
             const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > u));
             const int e = u - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(mine, l));
             const int slot0 = __builtin_amdgcn_readlane(in[0], l), parts = __builtin_amdgcn_readlane(in[1], l);
             const int n_cols = __builtin_amdgcn_readlane(in[2], l) * G, row0 = __builtin_amdgcn_readlane(in[3], l);
             const int kvh = e / n_cols, col = e % n_cols;
-            const int at = slot0 + ((n_cols - 1) / cols - col / cols) * parts;
-            if (at + parts > a.slots) continue;              // offsets that do not add up: more groups than rows allow
-            const int64_t from = ((int64_t)kvh * a.slots + at) * cols + col % cols;
+            if (slot0 + parts > a.slots) continue;           // offsets that do not add up
+            const int64_t from = ((int64_t)kvh * a.slots + slot0) * cols + col;
             float m = kUnset, ll = 0.f;
             f2 o = f2{0.f, 0.f};
-            for (int p = kWide ? 0 : wave; p < parts; p += kWide ? 1 : WAVES) {
+            for (int p = wave; p < parts; p += WAVES) {
                 const f2 x = a.ml[from + (int64_t)p * cols];
                 const f2 v = *reinterpret_cast<const f2*>(a.acc + (from + (int64_t)p * cols) * HD + 2 * lane);
                 const float to = fmaxf(m, x[0]);
@@ -574,26 +686,24 @@ __global__ void __launch_bounds__(THREADS) q8_join_kernel(Q8Args a, int cols) {
                 o = o * f0 + v * f1;
                 m = to;
             }
-            if constexpr (!kWide) {
-                __syncthreads();                             // the last column has been read
-                s_o[wave][lane] = o;
-                if (lane == 0) {
-                    s_m[wave] = m;
-                    s_l[wave] = ll;
-                }
-                __syncthreads();
-                if (wave) continue;
-                m = s_m[0];
+            __syncthreads();                                 // the last column has been read
+            s_o[wave][lane] = o;
+            if (lane == 0) {
+                s_m[wave] = m;
+                s_l[wave] = ll;
+            }
+            __syncthreads();
+            if (wave) continue;
+            m = s_m[0];
 #pragma unroll
-                for (int w = 1; w < WAVES; ++w) m = fmaxf(m, s_m[w]);
-                o = f2{0.f, 0.f};
-                ll = 0.f;
+            for (int w = 1; w < WAVES; ++w) m = fmaxf(m, s_m[w]);
+            o = f2{0.f, 0.f};
+            ll = 0.f;
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(s_m[w] - m);
-                    o += s_o[w][lane] * f;
-                    ll += s_l[w] * f;
-                }
+            for (int w = 0; w < WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(s_m[w] - m);
+                o += s_o[w][lane] * f;
+                ll += s_l[w] * f;
             }
             const int r = col / G, hh = col - r * G;
             *reinterpret_cast<f2*>(a.o + ((int64_t)(row0 + r) * NH + kvh * G + hh) * HD + 2 * lane) = o * (1.0f / ll);
@@ -602,30 +712,258 @@ __global__ void __launch_bounds__(THREADS) q8_join_kernel(Q8Args a, int cols) {
     }
 }
 
+// ---- many columns ----
+
+// LDS byte address of a __shared__ location
+__device__ __forceinline__ uint32_t lds_addr(const unsigned char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
+}
+
+// 2 KiB from a wave-uniform address straight to LDS, 16 B per lane: bytes 16 lane of
+// each half.  In inline asm so that the compiler's own counts do not see the loads
+// (it would drain them before every LDS read): the pipeline below waits for them.
+// m0 holds the LDS address; the statement saves and restores it, and the scalar
+// copy of the base settles a base that a vector instruction wrote and is the wait
+// state that m0 needs before an LDS load.
+__device__ __forceinline__ void page_to_lds(const void* base, uint32_t lane16, uint32_t lds) {
+    uint32_t saved;
+    uint64_t from;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %4\n\ts_mov_b64 %1, %2\n\tglobal_load_lds_dwordx4 %3, %1\n\t"
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %1\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved), "=&s"(from)
+        : "s"(base), "v"(lane16), "s"(lds), "s"(lds + 1024u), "v"(lane16 + 1024u)
+        : "memory");
+}
+
+// Each wave has its own 16 columns of a group, and all go over the same keys.
+// Wave w brings page w of a tile: K straight to LDS, the
+// pages 64 B further apart than they are long so that the operand reads are free of
+// bank conflicts; V and the scales through registers, the codes turned into fp16 in
+// operand order, two tiles of everything.  A tile's loads go
+// out at the start of the tile before it and are waited for at its end; one barrier
+// per tile.
+__global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
+    constexpr int COLS = kManyCols;
+    constexpr int kPageLds = kQ8KBytes + 64, kStage = kTilePages * kPageLds;
+    constexpr int kOut = 16 * kAccRow * 4;                   // a block's results, per wave
+    constexpr int kVTile = 2 * DB * 1024;
+    static_assert(kTilePages == WAVES, "a page per wave");
+    static_assert(WAVES * kOut <= 2 * kStage + 2 * kVTile, "the results overwrite the tiles");
+    __shared__ __attribute__((aligned(16))) unsigned char s_mem[2 * kStage + 2 * kVTile];
+    __shared__ float s_scale[2][2][TILE];                    // K scale, V scale
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, c = lane & 15;
+    const int kvh = blockIdx.x, w = blockIdx.y;
+
+    Place at, to;
+    find_stretch(a, w, at, to);
+    i4 piece[2] = {i4{-1, 0, 0, 0}, i4{-1, 0, 0, 0}};        // the group begun before this stretch; the one it leaves open
+    for (;;) {
+        if (at.sess >= a.n_sess || at.sess > to.sess ||
+            (at.sess == to.sess && (at.group > to.group || (at.group == to.group && at.tile >= to.tile))))
+            break;
+        Session s = session_of<true>(a, at.sess);
+        s = Session{__builtin_amdgcn_readfirstlane(s.keys), __builtin_amdgcn_readfirstlane(s.past),
+                    __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.row0)};
+        if (at.group >= n_groups(s)) {
+            at = Place{at.sess + 1, 0, 0};
+            continue;
+        }
+        const int sess = at.sess, group = at.group;
+        const int tiles = __builtin_amdgcn_readfirstlane(group_tiles(s, group));
+        const int t_lo = __builtin_amdgcn_readfirstlane(at.tile);
+        const int t_hi = __builtin_amdgcn_readfirstlane(sess == to.sess && group == to.group ? to.tile : tiles);
+        at = Place{sess, group + 1, 0};
+        if (t_lo >= t_hi) continue;
+
+        const int n_cols = s.rows * G, col0 = group * COLS + wave * 16;
+        const int wave_keys = col0 < n_cols ? min(s.past + min(col0 + 15, n_cols - 1) / G + 1, s.keys) : 0;
+        const int t1 = __builtin_amdgcn_readfirstlane(min(t_hi, (wave_keys + TILE - 1) / TILE));   // this wave's last tile
+        const int t_clear = __builtin_amdgcn_readfirstlane(min(s.past + col0 / G + 1, s.keys) / TILE);   // tiles below: seen by all its columns
+
+        // ---- a tile's way into LDS ----
+        const int32_t* table = a.tables + sess * a.table_stride;
+        const int last_page = (s.keys - 1) >> kKvBlockShift;
+        int win = -64, held = 0;                             // 64 table entries from `win` on
+        i4 vr[2];
+        float scale = 0.f;
+        auto load = [&](int t) {                             // page `wave` of tile t
+            const int pg = t * kTilePages;
+            if (pg + kTilePages > win + 64) {
+                win = pg;
+                held = table[min(pg + lane, last_page)];
+            }
+            const int e = __builtin_amdgcn_readlane(held, min(pg + wave, last_page) - win);
+            const int phys = (unsigned)e < (unsigned)a.nb ? e : 0;           // an entry outside the pool reads page 0
+            const uint8_t* rec = a.pool + phys * kQ8Page + kvh * kQ8Rec;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) vr[u] = *reinterpret_cast<const i4*>(rec + kQ8VOff + 1024 * u + 16 * lane);
+            scale = *reinterpret_cast<const float*>(rec + kQ8KsOff + 4 * (lane & 31));
+            page_to_lds(rec, 16 * lane, __builtin_amdgcn_readfirstlane(lds_addr(s_mem) + (t & 1) * kStage + wave * kPageLds));
+        };
+        auto put = [&](int t) {                              // waits for every load of the wave
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            unsigned char* dst = s_mem + 2 * kStage + (t & 1) * kVTile + g * 2048 + (16 * wave + c) * 16;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)                  // dims 64 u + 16 g + c, tokens 8 e .. + 7
+                    *reinterpret_cast<h8*>(dst + u * 8192 + e * 1024) = codes_f16((uint32_t)vr[u][2 * e], (uint32_t)vr[u][2 * e + 1]);
+            // (a key behind the last one may hold anything: its V scale is none)
+            if (lane >= 16 && t * TILE + 16 * wave + c >= s.keys) scale = 0.f;
+            if (lane < 32) s_scale[t & 1][lane >> 4][16 * wave + c] = scale;
+        };
+        // the workgroup's LDS writes are done; loads in flight stay there
+        auto barrier = [&] {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        load(t_lo);
+        QDigits q;
+        int seen;
+        State st[1];
+        load_q(a, s, kvh, col0 + c, q, seen);
+        st[0].clear();
+        put(t_lo);
+        barrier();
+        ValueUnit unit;
+        unit.clear();
+        const uint32_t k_off = (uint32_t)((c >> 2) * kPageLds + g * 64 + (c & 3) * 16);
+        auto tile = [&](auto mask_tag, int t) {
+            constexpr bool kMask = decltype(mask_tag)::value;
+            const int key0 = t * TILE + 16 * g;
+            const unsigned char* k_at = s_mem + (t & 1) * kStage + k_off;
+            const unsigned char* v_at = s_mem + 2 * kStage + (t & 1) * kVTile + 16 * lane;
+            const float ks = s_scale[t & 1][0][lane], vs = unit.take(s_scale[t & 1][1][lane], st);
+            h8 hi[2], lo[2];
+            weigh<kMask>([&](int u) { return *reinterpret_cast<const i4*>(k_at + 256 * u); },
+                         [&](int d, int h) { return q.d[d][h]; }, q.scale, ks, vs, key0, seen, st[0], hi, lo);
+#pragma unroll
+            for (int e = 0; e < 2 * DB / 4; ++e) {           // two 16-dim blocks, two halves of their tokens
+                h8 v[2][2];
+#pragma unroll
+                for (int d = 0; d < 2; ++d)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) v[d][u] = *reinterpret_cast<const h8*>(v_at + 1024 * (2 * (2 * e + d) + u));
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            f4& o = st[0].acc[2 * e + d];
+                            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[d][u], k ? lo[u] : hi[u], o, 0, 0, 0);
+                        }
+            }
+        };
+        // every wave goes through all tiles of the stretch, for its page of them and the
+        // barrier; its own columns need the first ones, up to t_clear without a mask
+        auto round = [&](int t, auto&& compute) {
+            if (t + 1 < t_hi) load(t + 1);
+            compute();
+            if (t + 1 < t_hi) put(t + 1);
+            barrier();
+        };
+        int t = t_lo;
+        for (; t < min(t1, t_clear); ++t) round(t, [&] { tile(std::false_type{}, t); });
+        for (; t < t1; ++t) round(t, [&] { tile(std::true_type{}, t); });
+        for (; t < t_hi; ++t) round(t, [] {});
+
+        // results through LDS (every wave is past its tiles), rows in address order:
+        // the output, or a piece of a group that others have the rest of
+        const bool whole = t_lo == 0 && t_hi == tiles;
+        const int slot = 2 * w + (t_lo > 0 ? 0 : 1);
+        if (!whole) piece[t_lo > 0 ? 0 : 1] = i4{sess, group, t_hi == tiles, 0};
+        unsigned char* mine = s_mem + wave * kOut;
+        if (col0 < n_cols) {
+            const float l = rows_sum(st[0].l), m = st[0].reference();
+            st[0].scale_acc(unit.unit);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(mine + (c * kAccRow + 16 * d + 4 * g) * 4) = st[0].acc[d];
+            wave_lds_sync();
+#pragma unroll
+            for (int e = 0; e < 16 * (HD / 4) / 64; ++e) {
+                const int cc = 2 * e + lane / 32, d4 = lane % 32, col = col0 + cc;
+                const f4 sum = *reinterpret_cast<const f4*>(mine + (cc * kAccRow + 4 * d4) * 4);
+                const float cl = __shfl(l, cc, 64), cm = __shfl(m, cc, 64);
+                if (col >= n_cols) continue;
+                if (whole) {
+                    const int r = col / G, hh = col - r * G;
+                    *reinterpret_cast<f4*>(a.o + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d4) = sum * (1.0f / cl);
+                } else {
+                    const int64_t to_at = ((int64_t)kvh * a.slots + slot) * COLS + wave * 16 + cc;
+                    *reinterpret_cast<f4*>(a.acc + to_at * HD + 4 * d4) = sum;
+                    if (d4 == 0) a.ml[to_at] = f2{cm, cl};
+                }
+            }
+        }
+        barrier();                                           // the next group's tiles come where the results were
+    }
+    if (kvh == 0 && tid < 2) a.info[2 * w + tid] = tid ? piece[1] : piece[0];
+}
+
+// Joins the pieces of groups that several workgroups had: the one that began a
+// group names it, the next ones follow until one has its end.  A workgroup per
+// (stretch, kv head, 16 columns), 16 lanes per column.
+__global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
+    constexpr int COLS = kManyCols;
+    const int w = blockIdx.x, kvh = blockIdx.y;
+    const i4 begun = a.info[2 * w + 1];
+    if (begun[0] < 0) return;
+    const Session s = session_of<true>(a, begun[0]);
+    const int cc = blockIdx.z * 16 + threadIdx.x / 16, d8 = 8 * (threadIdx.x % 16), col = begun[1] * COLS + cc;
+    if (col >= s.rows * G) return;
+    auto slot_at = [&](int slot) { return ((int64_t)kvh * a.slots + slot) * COLS + cc; };
+    int64_t at = slot_at(2 * w + 1);
+    f2 x = a.ml[at];
+    float m = x[0], l = x[1];
+    f4 o0 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8), o1 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8 + 4);
+    for (int v = w + 1; v < a.gw; ++v) {
+        const i4 next = a.info[2 * v];
+        if (next[0] != begun[0] || next[1] != begun[1]) continue;            // a stretch too short to have a tile of it
+        at = slot_at(2 * v);
+        x = a.ml[at];
+        const f4 p0 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8), p1 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8 + 4);
+        const float to = fmaxf(m, x[0]);
+        const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
+        l = l * f0 + x[1] * f1;
+        o0 = o0 * f0 + p0 * f1;
+        o1 = o1 * f0 + p1 * f1;
+        m = to;
+        if (next[2]) break;
+    }
+    const int r = col / G, hh = col - r * G;
+    float* out = a.o + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + d8;
+    *reinterpret_cast<f4*>(out) = o0 * (1.0f / l);
+    *reinterpret_cast<f4*>(out + 4) = o1 * (1.0f / l);
+}
+
 // ---- host side ----
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr int kFewCols = 64;                   // columns per session up to which a session's waves share them
+constexpr int kFewCols = 32;                   // columns per session up to which a workgroup's waves share them
 constexpr int kAimWgs = 512;                   // workgroups aimed at: two per CU
 constexpr int kMinShare = 4;                   // tiles: one per wave
-constexpr int kJoinWgs = 2048;                 // a launch full of the chip
-constexpr int kWideBlocks = 2;                 // 16-column blocks per wave of the wide form
+constexpr int kSoloPages = 48;            // see launch()
+constexpr int kJoinWgs = 2048;                 // a launch that fills the chip
 
-// What a call of these counts runs with: the columns of a workgroup and the
-// workgroups per kv head.
+// What a call of these counts runs with: the columns of a workgroup and the partial
+// results per kv head.
 struct Shape {
-    int blocks, cols, slots;
-    bool wide;
+    bool many;
+    int cols, slots;
 };
-Shape shape(int n_sess, int n_rows, int max_q) {
+Shape shape(int n_sess, int max_q) {
     Shape f{};
     const int64_t cols = (int64_t)max_q * G;
-    f.wide = cols > kFewCols;
-    f.blocks = f.wide ? kWideBlocks : cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-    f.cols = 16 * f.blocks * (f.wide ? WAVES : 1);
-    const int64_t groups = f.wide ? (int64_t)n_rows * G / f.cols + n_sess : n_sess;
-    f.slots = (int)(kAimWgs / NKV + groups);
+    f.many = cols > kFewCols;
+    f.cols = f.many ? kManyCols : cols <= 16 ? 16 : 32;
+    f.slots = f.many ? 2 * (kAimWgs / NKV) : kAimWgs / NKV + n_sess;
     return f;
 }
 
@@ -635,7 +973,7 @@ struct Layout {
 Layout layout(const Shape& f, int n_sess) {
     Layout w{};
     const size_t rows = (size_t)NKV * f.slots * f.cols;
-    w.ml = ((size_t)n_sess * sizeof(i4) + 255) / 256 * 256;
+    w.ml = ((size_t)(f.many ? f.slots : n_sess) * sizeof(i4) + 255) / 256 * 256;
     w.acc = w.ml + (rows * sizeof(f2) + 255) / 256 * 256;
     w.total = w.acc + rows * HD * sizeof(float);
     return w;
@@ -663,25 +1001,46 @@ Q8Args attn_args(const float* q, const uint8_t* pool, const int32_t* tables, int
 
 template <bool kCausal>
 void launch(Q8Args a, void* workspace, hipStream_t s) {
-    const Shape f = shape(a.n_sess, a.rows.n_rows, a.max_q);
+    const Shape f = shape(a.n_sess, a.max_q);
     const Layout w = layout(f, a.n_sess);
     char* ws = static_cast<char*>(workspace);
     a.slots = f.slots;
     a.info = reinterpret_cast<i4*>(ws + w.info);
     a.ml = reinterpret_cast<f2*>(ws + w.ml);
     a.acc = reinterpret_cast<float*>(ws + w.acc);
-    const dim3 grid(NKV, f.slots);
     if constexpr (kCausal) {
-        if (f.wide) hipLaunchKernelGGL((q8_attn_kernel<kWideBlocks, true, true>), grid, dim3(THREADS), 0, s, a);
-        else if (f.blocks == 4) hipLaunchKernelGGL((q8_attn_kernel<4, true, false>), grid, dim3(THREADS), 0, s, a);
-        else if (f.blocks == 2) hipLaunchKernelGGL((q8_attn_kernel<2, true, false>), grid, dim3(THREADS), 0, s, a);
+        if (f.many) {
+            hipLaunchKernelGGL(q8_many_kernel, dim3(NKV, a.gw), dim3(THREADS), 0, s, a);
+            NOVA_LAUNCHED();
+            hipLaunchKernelGGL(q8_many_join_kernel, dim3(a.gw, NKV, WAVES), dim3(THREADS), 0, s, a);
+            NOVA_LAUNCHED();
+            return;
+        }
     }
-    if (f.blocks == 1) hipLaunchKernelGGL((q8_attn_kernel<1, kCausal, false>), grid, dim3(THREADS), 0, s, a);
+    // Tables this short: a workgroup per session and kv head, nothing to join (24
+    // sessions of up to 600 keys, 7B: 9.6 us instead of 10.7 in two launches).
+    const bool solo = a.table_stride <= kSoloPages;
+    if (solo) a.min_share = kSoloPages;
+    const dim3 grid(NKV, solo ? a.n_sess : f.slots);
+    // The pages of a pool larger than the 256 MB memory-side cache (all layers of it,
+    // as a step walks through them) come from HBM: non-temporal loads, 8 x 32768 keys
+    // of the 14B model 103 -> 90 us, 16 ragged sessions of the 7B model whose pages
+    // are in no cache 23.7 -> 22.6.  Where a cache still has them plain loads are
+    // faster: the same 16 sessions 20.7 instead of 22.0.
+    const bool once = (int64_t)Model::L * a.nb * kQ8Page > (int64_t)256 << 20;
+    auto run = [&](auto once_tag) {
+        constexpr bool kOnce = decltype(once_tag)::value;
+        if (f.cols == 16) hipLaunchKernelGGL((q8_few_kernel<1, kCausal, kOnce>), grid, dim3(THREADS), 0, s, a);
+        if constexpr (kCausal)
+            if (f.cols == 32) hipLaunchKernelGGL((q8_few_kernel<2, true, kOnce>), grid, dim3(THREADS), 0, s, a);
+    };
+    if (once) run(std::true_type{});
+    else run(std::false_type{});
     NOVA_LAUNCHED();
+    if (solo) return;
     const int64_t columns = (int64_t)a.rows.n_rows * NH;
-    const unsigned join = (unsigned)std::min<int64_t>(f.wide ? (columns + WAVES - 1) / WAVES : columns, kJoinWgs);
-    if (f.wide) hipLaunchKernelGGL(q8_join_kernel<true>, dim3(join), dim3(THREADS), 0, s, a, f.cols);
-    else hipLaunchKernelGGL(q8_join_kernel<false>, dim3(join), dim3(THREADS), 0, s, a, f.cols);
+    hipLaunchKernelGGL(q8_few_join_kernel, dim3((unsigned)std::min<int64_t>(columns, kJoinWgs)), dim3(THREADS), 0, s, a,
+                       f.cols);
     NOVA_LAUNCHED();
 }
 
@@ -694,12 +1053,12 @@ extern "C" {
 
 size_t attn_decode_q8_workspace_bytes(int n_sess) {
     NOVA_REQUIRE(n_sess >= 1 && n_sess <= 65535);
-    return layout(shape(n_sess, n_sess, 1), n_sess).total;
+    return layout(shape(n_sess, 1), n_sess).total;
 }
 
 size_t attn_chunk_q8_workspace_bytes(int n_sess, int n_rows, int max_q) {
     NOVA_REQUIRE(n_sess >= 1 && n_sess <= 65535 && n_rows >= 0 && max_q >= 0 && max_q <= n_rows);
-    return layout(shape(n_sess, n_rows, max_q), n_sess).total;
+    return layout(shape(n_sess, max_q), n_sess).total;
 }
 
 void launch_attn_decode_q8_batch(const float* q, const uint8_t* pool, const int32_t* tables, int table_stride,
