@@ -677,14 +677,26 @@ __global__ void __launch_bounds__(THREADS) q8_few_join_kernel(Q8Args a, int cols
             const int64_t from = ((int64_t)kvh * a.slots + slot0) * cols + col;
             float m = kUnset, ll = 0.f;
             f2 o = f2{0.f, 0.f};
-            for (int p = wave; p < parts; p += WAVES) {
-                const f2 x = a.ml[from + (int64_t)p * cols];
-                const f2 v = *reinterpret_cast<const f2*>(a.acc + (from + (int64_t)p * cols) * HD + 2 * lane);
-                const float to = fmaxf(m, x[0]);
-                const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
-                ll = ll * f0 + x[1] * f1;
-                o = o * f0 + v * f1;
-                m = to;
+            for (int p = wave; p < parts; p += 4 * WAVES) {  // four parts' loads at a time
+                f2 x[4], v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[k] = f2{kUnset, 0.f};
+                    v[k] = f2{0.f, 0.f};
+                    if (p + k * WAVES < parts) {
+                        const int64_t at = from + (int64_t)(p + k * WAVES) * cols;
+                        x[k] = a.ml[at];
+                        v[k] = *reinterpret_cast<const f2*>(a.acc + at * HD + 2 * lane);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float to = fmaxf(m, x[k][0]);
+                    const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[k][0] - to);
+                    ll = ll * f0 + x[k][1] * f1;
+                    o = o * f0 + v[k] * f1;
+                    m = to;
+                }
             }
             __syncthreads();                                 // the last column has been read
             s_o[wave][lane] = o;
@@ -908,38 +920,63 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
 
 // Joins the pieces of groups that several workgroups had: the one that began a
 // group names it, the next ones follow until one has its end.  A workgroup per
-// (stretch, kv head, 16 columns), 16 lanes per column.
+// (stretch, kv head, 8 columns), 32 lanes per column.  Which of the next 64
+// stretches have a piece is read at once, and the pieces eight at a time: the launch
+// lasts as long as its memory latencies in a row.
+constexpr int kJoinCols = THREADS / (HD / 4);
 __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
-    constexpr int COLS = kManyCols;
-    const int w = blockIdx.x, kvh = blockIdx.y;
+    constexpr int COLS = kManyCols, kAtOnce = 8;
+    const int w = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 63;
+    const int cc = blockIdx.z * kJoinCols + threadIdx.x / (HD / 4), d4 = 4 * (threadIdx.x % (HD / 4));
+    auto at = [&](int slot) { return ((int64_t)kvh * a.slots + slot) * COLS + cc; };
+    i4 next = i4{-1, 0, 0, 0};
+    if (w + 1 + lane < a.gw) next = a.info[2 * (w + 1 + lane)];
     const i4 begun = a.info[2 * w + 1];
     if (begun[0] < 0) return;
     const Session s = session_of<true>(a, begun[0]);
-    const int cc = blockIdx.z * 16 + threadIdx.x / 16, d8 = 8 * (threadIdx.x % 16), col = begun[1] * COLS + cc;
-    if (col >= s.rows * G) return;
-    auto slot_at = [&](int slot) { return ((int64_t)kvh * a.slots + slot) * COLS + cc; };
-    int64_t at = slot_at(2 * w + 1);
-    f2 x = a.ml[at];
-    float m = x[0], l = x[1];
-    f4 o0 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8), o1 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8 + 4);
-    for (int v = w + 1; v < a.gw; ++v) {
-        const i4 next = a.info[2 * v];
-        if (next[0] != begun[0] || next[1] != begun[1]) continue;            // a stretch too short to have a tile of it
-        at = slot_at(2 * v);
-        x = a.ml[at];
-        const f4 p0 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8), p1 = *reinterpret_cast<const f4*>(a.acc + at * HD + d8 + 4);
+    const int col = begun[1] * COLS + cc;
+    if (begun[1] * COLS + (int)blockIdx.z * kJoinCols >= s.rows * G) return;
+    float m = kUnset, l = 0.f;
+    f4 o = f4{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const f2 x, const f4 p) {
         const float to = fmaxf(m, x[0]);
         const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
         l = l * f0 + x[1] * f1;
-        o0 = o0 * f0 + p0 * f1;
-        o1 = o1 * f0 + p1 * f1;
+        o = o * f0 + p * f1;
         m = to;
-        if (next[2]) break;
+    };
+    const f2 x0 = a.ml[at(2 * w + 1)];
+    const f4 a0 = *reinterpret_cast<const f4*>(a.acc + at(2 * w + 1) * HD + d4);
+    for (int base = w + 1;;) {
+        const bool ours = next[0] == begun[0] && next[1] == begun[1];        // others: too short to have a tile of it
+        uint64_t todo = __builtin_amdgcn_ballot_w64(ours);
+        const bool closed = __builtin_amdgcn_ballot_w64(ours && next[2]) != 0;
+        while (todo) {                                       // uniform over the workgroup
+            f2 x[kAtOnce];
+            f4 p[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                x[k] = f2{kUnset, 0.f};
+                p[k] = f4{0.f, 0.f, 0.f, 0.f};
+                if (todo) {
+                    const int64_t from = at(2 * (base + __builtin_ctzll(todo)));
+                    x[k] = a.ml[from];
+                    p[k] = *reinterpret_cast<const f4*>(a.acc + from * HD + d4);
+                    todo &= todo - 1;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) add(x[k], p[k]);
+        }
+        base += 64;
+        if (closed || base >= a.gw) break;
+        next = i4{-1, 0, 0, 0};
+        if (base + lane < a.gw) next = a.info[2 * (base + lane)];
     }
+    add(x0, a0);
+    if (col >= s.rows * G) return;
     const int r = col / G, hh = col - r * G;
-    float* out = a.o + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + d8;
-    *reinterpret_cast<f4*>(out) = o0 * (1.0f / l);
-    *reinterpret_cast<f4*>(out + 4) = o1 * (1.0f / l);
+    *reinterpret_cast<f4*>(a.o + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + d4) = o * (1.0f / l);
 }
 
 // ---- host side ----
@@ -1012,7 +1049,8 @@ void launch(Q8Args a, void* workspace, hipStream_t s) {
         if (f.many) {
             hipLaunchKernelGGL(q8_many_kernel, dim3(NKV, a.gw), dim3(THREADS), 0, s, a);
             NOVA_LAUNCHED();
-            hipLaunchKernelGGL(q8_many_join_kernel, dim3(a.gw, NKV, WAVES), dim3(THREADS), 0, s, a);
+            hipLaunchKernelGGL(q8_many_join_kernel, dim3(a.gw, NKV, kManyCols / kJoinCols), dim3(THREADS),
+                               0, s, a);
             NOVA_LAUNCHED();
             return;
         }
