@@ -190,14 +190,20 @@ __global__ void __launch_bounds__(QT) q8_store_kernel(RowArgs a) {
         }
     }
     const int head = blockIdx.y;
+    f4 x0{}, x1{}, y0{}, y1{};                                               // the rows, requested beside the table entry
+    if (real) {
+        const float* src = a.k + (row * NKV + head) * HD + 4 * j;
+        x0 = *reinterpret_cast<const f4*>(src);
+        x1 = *reinterpret_cast<const f4*>(src + HALF);
+        src = a.v + (row * NKV + head) * HD + 4 * j;
+        y0 = *reinterpret_cast<const f4*>(src);
+        y1 = *reinterpret_cast<const f4*>(src + HALF);
+    }
     const int phys = a.tables[it.sess * a.table_stride + it.page];
     if ((unsigned)phys >= (unsigned)a.nb) return;                            // no such page: nothing is written
     uint8_t* rec = a.pool + ((int64_t)a.layer * a.nb + phys) * kQ8Page + head * kQ8Rec;
     uint32_t v0 = 0, v1 = 0;
-    float vs = 0.f;
     if (real) {
-        const float* src = a.k + (row * NKV + head) * HD + 4 * j;
-        f4 x0 = *reinterpret_cast<const f4*>(src), x1 = *reinterpret_cast<const f4*>(src + HALF);
         if constexpr (kRope) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -212,8 +218,7 @@ __global__ void __launch_bounds__(QT) q8_store_kernel(RowArgs a) {
         uint8_t* dk = rec + (t >> 2) * 512 + (j >> 2) * 64 + (t & 3) * 16 + (j & 3) * 4;
         *reinterpret_cast<uint32_t*>(dk) = k0;
         *reinterpret_cast<uint32_t*>(dk + 256) = k1;
-        src = a.v + (row * NKV + head) * HD + 4 * j;
-        vs = quantise(*reinterpret_cast<const f4*>(src), *reinterpret_cast<const f4*>(src + HALF), v0, v1);
+        const float vs = quantise(y0, y1, v0, v1);
         if (j == 0) {
             *reinterpret_cast<float*>(rec + kQ8KsOff + 4 * t) = ks;
             *reinterpret_cast<float*>(rec + kQ8VsOff + 4 * t) = vs;
@@ -252,21 +257,28 @@ __global__ void __launch_bounds__(QT) q8_load_kernel(RowArgs a) {
     const int t = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
     const int first = max(it.pos0 - it.page * kKvBlock, 0);
     const int last = min(it.pos0 + it.n - it.page * kKvBlock, kKvBlock);
-    if (t < first || t >= last) return;
-    const int64_t row = it.row0 + it.page * kKvBlock + t - it.pos0;
     const int head = blockIdx.y;
     const int phys = q8_phys(a.tables + it.sess * a.table_stride, it.page, a.nb);
     const uint8_t* rec = a.pool + ((int64_t)a.layer * a.nb + phys) * kQ8Page + head * kQ8Rec;
+    // every read of the record goes out before the first wait; V's codes, dim by dim
+    // in the page, are read 16 B per lane and turned in LDS (reading them byte by
+    // byte instead: 9.6 us for 8 x 512 rows of the 7B model, so 6.4)
     const uint8_t* pk = rec + (t >> 2) * 512 + (j >> 2) * 64 + (t & 3) * 16 + (j & 3) * 4;
     const uint32_t k0 = *reinterpret_cast<const uint32_t*>(pk), k1 = *reinterpret_cast<const uint32_t*>(pk + 256);
+    const float ks = *reinterpret_cast<const float*>(rec + kQ8KsOff + 4 * t);
+    const float vs = *reinterpret_cast<const float*>(rec + kQ8VsOff + 4 * t);
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[HD * kKvBlock];
+    if (threadIdx.x < HD)
+        *reinterpret_cast<u4*>(s_v + 16 * threadIdx.x) = *reinterpret_cast<const u4*>(rec + kQ8VOff + 16 * threadIdx.x);
+    __syncthreads();
+    if (t < first || t >= last) return;
+    const int64_t row = it.row0 + it.page * kKvBlock + t - it.pos0;
     uint32_t v0 = 0, v1 = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        v0 |= (uint32_t)rec[kQ8VOff + (4 * j + e) * kKvBlock + t] << (8 * e);
-        v1 |= (uint32_t)rec[kQ8VOff + (HALF + 4 * j + e) * kKvBlock + t] << (8 * e);
+        v0 |= (uint32_t)s_v[(4 * j + e) * kKvBlock + t] << (8 * e);
+        v1 |= (uint32_t)s_v[(HALF + 4 * j + e) * kKvBlock + t] << (8 * e);
     }
-    const float ks = *reinterpret_cast<const float*>(rec + kQ8KsOff + 4 * t);
-    const float vs = *reinterpret_cast<const float*>(rec + kQ8VsOff + 4 * t);
     float* k = a.k_out + (row * NKV + head) * HD + 4 * j;
     float* v = a.v_out + (row * NKV + head) * HD + 4 * j;
     *reinterpret_cast<f4*>(k) = values(k0, ks);

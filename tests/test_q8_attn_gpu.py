@@ -392,3 +392,92 @@ def test_sessions_on_8_bit_pages():
     step([44, 46], [60, 2], "chunk and draft")
     step([104, 48], [1, 1], "token")
     nova.nova_paged_delete(h)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_non_finite_query_stays_in_its_row_and_head(bad):
+    d = Decode("qwen25_7b", [70, 900], seed=61)
+    c = Chunk("qwen25_7b", [30, 500], [70, 3], seed=62, behind=0)
+    for x, row, head in ((d, 1, 9), (c, 40, 27)):
+        x.q[row, head, 77] = bad
+        x.nova.dev_upload(x.dq.ptr, x.q.ctypes.data, x.q.nbytes)
+        x.launch()
+        x.nova.dev_sync()
+        wrong = ~np.isfinite(x.result())
+        assert wrong[row, head].all()
+        wrong[row, head] = False
+        assert not wrong.any()
+
+
+def test_attention_beyond_32_bit_offsets():
+    """the last layer and the last pages of a pool of 5 GB: append, decode, chunk"""
+    nova = _nova("qwen25_7b")
+    nb, layer, n = 11000, 27, 40
+    rng = np.random.default_rng(63)
+    dev = nova.alloc((layer + 1) * nb * nova.kv_q8_page_bytes())
+    k, v = (rng.standard_normal((n, nova.nkv, HD)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((n, nova.nh, HD)).astype(np.float32)
+    table, zero, keys = np.array([[nb - 1, 3, nb - 2]], np.int32), np.zeros(1, np.int32), np.array([n], np.int32)
+    dt, dz, dn, dk, dv, dq = (nova.upload(x) for x in (table, zero, keys, k, v, q))
+    nova.launch_kv_q8_store_batch(dev.ptr, dt.ptr, 3, dz.ptr, None, 1, n, layer, nb, dk.ptr, dv.ptr, None)
+    o, o1 = nova.alloc(q.nbytes), nova.alloc(q[:1].nbytes)
+    ws = nova.alloc(nova.attn_chunk_q8_workspace_bytes(1, n, n))
+    nova.launch_attn_chunk_q8_batch(dq.ptr, dev.ptr, dt.ptr, 3, dz.ptr, None, 1, n, n, layer, nb, o.ptr, ws.ptr, None)
+    ws1 = nova.alloc(nova.attn_decode_q8_workspace_bytes(1))
+    nova.launch_attn_decode_q8_batch(dq.ptr, dev.ptr, dt.ptr, 3, dn.ptr, 1, layer, nb, o1.ptr, ws1.ptr, None)
+    nova.dev_sync()
+    kk, vv = (c.astype(np.float64) * s[..., None] for c, s in map(quantise, (k, v)))
+    ref, tol = attention(q, kk, vv, 1, nova.group)
+    assert_within(o.numpy(q.shape, np.float32), ref, tol, "chunk")
+    ref, tol = attention(q[:1], kk, vv, n, nova.group)
+    assert_within(o1.numpy(q[:1].shape, np.float32), ref, tol, "decode")
+
+
+@pytest.mark.parametrize("n_keys", [[33, 500, 1], [1], [767, 768]])
+def test_short_tables(n_keys):
+    """tables of up to 48 pages take one launch without a join"""
+    d = Decode("qwen25_7b", n_keys, seed=64)
+    assert d.table.shape[1] <= 51
+    d.table = np.ascontiguousarray(d.table[:, :48])
+    d.dt = d.nova.upload(d.table)
+    d.launch()
+    d.nova.dev_sync()
+    d.check("short")
+
+
+def test_keys_behind_the_table_are_left_out():
+    """a session said to hold more keys than its table has entries for"""
+    d = Decode("qwen25_1p5b", [64, 40], seed=65)
+    d.table = np.ascontiguousarray(d.table[:, :3])           # 48 tokens each
+    d.dt = d.nova.upload(d.table)
+    d.n_keys = np.array([48, 40], np.int32)                  # what is left of [64, 40]
+    d.launch()
+    d.nova.dev_sync()
+    d.check("cut")
+
+
+def test_rows_behind_max_q_are_left_unwritten():
+    c = Chunk("qwen25_7b", [100, 20], [9, 4], seed=66, max_q=5, behind=0)
+    c.launch()
+    c.nova.dev_sync()
+    got = c.result()
+    assert (got[5:9] == 3).all()
+    for i, (a, n) in enumerate(((0, 5), (9, 4))):
+        # the session's keys end with its last row that counts
+        k, v = values(c.pool.rec, c.table[i], int(c.past[i]) + n)
+        ref, tol = attention(c.q[a:a + n], k, v, int(c.past[i]) + 1, c.nova.group)
+        assert_within(got[a:a + n], ref, tol, f"session {i}")
+
+
+def test_workspace_is_enough():
+    """nothing is written behind the workspace's size, whatever it held before"""
+    for x in (Decode("qwen25_1p5b", [5000, 3, 900], seed=67), Chunk("qwen25_14b", [3000, 0], [6, 3], seed=68),
+              Chunk("qwen25_7b", [2000, 0], [50, 200], seed=69)):
+        n = x.nova
+        size = x.ws.nbytes
+        guard = n.upload(np.full(size + 65536, 0xff, np.uint8))              # NaN bits
+        x.ws = guard
+        x.launch()
+        n.dev_sync()
+        x.check("poisoned workspace")
+        assert (n.download(guard, (65536,), np.uint8, size) == 0xff).all()
