@@ -30,7 +30,8 @@ constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
-constexpr int kMinPiece = 4;                   // tiles of a group that is cut
+constexpr int kMinPiece = 3;                   // tiles of a group that is cut
+constexpr int kGroupTiles = 4;                 // what a group costs beside its tiles, in tiles
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -1e30f;               // reference of a column without keys, where states are joined
@@ -208,8 +209,9 @@ __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
 // workgroup gets the same length, so a group may be shared by workgroups that
 // follow each other, and each of them has at most two groups in part.  The cost of
 // group g is counted as G past + C (g + 1) (G times the keys its last row sees,
-// where rows do not end inside a group), whose sums have a closed form; everything
-// is in whole numbers, so that neighbours agree on where one stops and the other begins.
+// where rows do not end inside a group) and as much as kGroupTiles tiles for its
+// start and end, whose sums have a closed form; everything is in whole numbers, so
+// that neighbours agree on where one stops and the other begins.
 struct Place {
     int sess, group, tile;     // sess == n_sess: the end
 };
@@ -227,13 +229,14 @@ __device__ __forceinline__ int group_tiles(const Session& s, int g) {
     return (min(s.past + (min((g + 1) * kManyCols, s.rows * G) - 1) / G + 1, s.keys) + TILE - 1) / TILE;
 }
 // Cost of the first n groups, in a double: whole numbers below 2^53, exact.
+__device__ __forceinline__ double flat_cost(const Session& s) { return (double)G * s.past + G * TILE * kGroupTiles; }
 __device__ __forceinline__ double groups_cost(const Session& s, int n) {
-    return (double)n * ((double)G * s.past) + 0.5 * kManyCols * ((double)n * (n + 1));
+    return (double)n * flat_cost(s) + 0.5 * kManyCols * ((double)n * (n + 1));
 }
 
 // where cost x of the line lies in session s, which begins at x = 0
 __device__ __forceinline__ void place_in(const Session& s, double x, Place& p) {
-    const double half = 0.5 * kManyCols, b = (double)G * s.past + half;
+    const double half = 0.5 * kManyCols, b = flat_cost(s) + half;
     int g = (int)((__builtin_sqrt(b * b + 4.0 * half * x) - b) / (2.0 * half));      // an estimate
     g = min(max(g, 0), n_groups(s) - 1);
     while (g > 0 && groups_cost(s, g) > x) --g;
