@@ -30,6 +30,7 @@ constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
+constexpr int kAimWgs = 512;                   // workgroups aimed at: two per CU
 constexpr int kMinPiece = 3;                   // tiles of a group that is cut
 constexpr int kGroupTiles = 4;                 // what a group costs beside its tiles, in tiles
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
@@ -892,7 +893,7 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
         // the output, or a piece of a group that others have the rest of
         const bool whole = t_lo == 0 && t_hi == tiles;
         const int slot = 2 * w + (t_lo > 0 ? 0 : 1);
-        if (!whole) piece[t_lo > 0 ? 0 : 1] = i4{sess, group, t_hi == tiles, 0};
+        if (!whole) piece[t_lo > 0 ? 0 : 1] = i4{sess, group, t_hi == tiles, min(n_cols - group * COLS, COLS)};
         unsigned char* mine = s_mem + wave * kOut;
         if (col0 < n_cols) {
             const float l = rows_sum(st[0].l), m = st[0].reference();
@@ -922,64 +923,124 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
 }
 
 // Joins the pieces of groups that several workgroups had: the one that began a
-// group names it, the next ones follow until one has its end.  A workgroup per
-// (stretch, kv head, 8 columns), 32 lanes per column.  Which of the next 64
-// stretches have a piece is read at once, and the pieces eight at a time: the launch
-// lasts as long as its memory latencies in a row.
-constexpr int kJoinCols = THREADS / (HD / 4);
+// group names it, the next ones follow until one has its end.  32 lanes per column,
+// and as many teams of them share a column's pieces as there are workgroups for.
+// Which of the next 64 stretches have a piece is read at once, and a team's pieces
+// eight at a time: the launch lasts as long as its memory latencies in a row.
+constexpr int kJoinRows = THREADS / (HD / 4);
+static_assert(kJoinRows == 8, "columns or teams of a workgroup");
 __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
-    constexpr int COLS = kManyCols, kAtOnce = 8;
-    const int w = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 63;
-    const int cc = blockIdx.z * kJoinCols + threadIdx.x / (HD / 4), d4 = 4 * (threadIdx.x % (HD / 4));
-    auto at = [&](int slot) { return ((int64_t)kvh * a.slots + slot) * COLS + cc; };
-    i4 next = i4{-1, 0, 0, 0};
-    if (w + 1 + lane < a.gw) next = a.info[2 * (w + 1 + lane)];
-    const i4 begun = a.info[2 * w + 1];
-    if (begun[0] < 0) return;
-    const Session s = session_of<true>(a, begun[0]);
-    const int col = begun[1] * COLS + cc;
-    if (begun[1] * COLS + (int)blockIdx.z * kJoinCols >= s.rows * G) return;
-    float m = kUnset, l = 0.f;
-    f4 o = f4{0.f, 0.f, 0.f, 0.f};
-    auto add = [&](const f2 x, const f4 p) {
-        const float to = fmaxf(m, x[0]);
-        const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
-        l = l * f0 + x[1] * f1;
-        o = o * f0 + p * f1;
-        m = to;
-    };
-    const f2 x0 = a.ml[at(2 * w + 1)];
-    const f4 a0 = *reinterpret_cast<const f4*>(a.acc + at(2 * w + 1) * HD + d4);
-    for (int base = w + 1;;) {
-        const bool ours = next[0] == begun[0] && next[1] == begun[1];        // others: too short to have a tile of it
-        uint64_t todo = __builtin_amdgcn_ballot_w64(ours);
-        const bool closed = __builtin_amdgcn_ballot_w64(ours && next[2]) != 0;
-        while (todo) {                                       // uniform over the workgroup
-            f2 x[kAtOnce];
-            f4 p[kAtOnce];
+    constexpr int COLS = kManyCols, kAtOnce = 8, kBatches = (kAimWgs / NKV + 63) / 64;
+    __shared__ f4 s_o[kJoinRows][HD / 4];
+    __shared__ f2 s_ml[kJoinRows];
+    const int lane = threadIdx.x & 63, row = threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4);
+    i4 begun[kBatches];                                      // the groups that stretch 64 b + lane leaves open
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                x[k] = f2{kUnset, 0.f};
-                p[k] = f4{0.f, 0.f, 0.f, 0.f};
-                if (todo) {
-                    const int64_t from = at(2 * (base + __builtin_ctzll(todo)));
-                    x[k] = a.ml[from];
-                    p[k] = *reinterpret_cast<const f4*>(a.acc + from * HD + d4);
-                    todo &= todo - 1;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) add(x[k], p[k]);
-        }
-        base += 64;
-        if (closed || base >= a.gw) break;
-        next = i4{-1, 0, 0, 0};
-        if (base + lane < a.gw) next = a.info[2 * (base + lane)];
+    for (int b = 0; b < kBatches; ++b) {
+        begun[b] = i4{-1, 0, 0, 0};
+        if (64 * b + lane < a.gw) begun[b] = a.info[2 * (64 * b + lane) + 1];
     }
-    add(x0, a0);
-    if (col >= s.rows * G) return;
-    const int r = col / G, hh = col - r * G;
-    *reinterpret_cast<f4*>(a.o + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + d4) = o * (1.0f / l);
+    // Columns of a workgroup: 8, or fewer for a group of more than 8 pieces, so that a
+    // team has up to 8 (as many stretches lie before the next open group at most).
+    int log[kBatches], later = a.gw;
+#pragma unroll
+    for (int b = kBatches - 1; b >= 0; --b) {
+        const uint64_t open = __builtin_amdgcn_ballot_w64(begun[b][0] >= 0), behind = open >> lane >> 1;
+        const int run = behind ? __builtin_ctzll(behind) + 1 : later - (64 * b + lane);
+        log[b] = run <= 8 ? 3 : run <= 16 ? 2 : run <= 32 ? 1 : 0;
+        if (open) later = 64 * b + __builtin_ctzll(open);
+    }
+    // a workgroup's units, up to and with stretch 64 b + lane's; no more than workgroups
+    int incl[kBatches], units = 0;
+    auto count = [&](int more) {
+        units = 0;
+#pragma unroll
+        for (int b = 0; b < kBatches; ++b) {
+            log[b] = min(log[b] + more, 3);
+            incl[b] = units + scan_incl(begun[b][0] >= 0 ? ((begun[b][3] + (1 << log[b]) - 1) >> log[b]) * NKV : 0);
+            units = __builtin_amdgcn_readlane(incl[b], 63);
+        }
+    };
+    count(0);
+    for (int i = 0; i < 3 && units > (int)gridDim.x; ++i) count(1);
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {    // uniform over the workgroup
+        int w = -1, e = 0, sess = 0, group = 0, cols = 0, wide_log = 3;
+#pragma unroll
+        for (int b = 0; b < kBatches; ++b) {
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(incl[b] > u);
+            if (w >= 0 || !hit) continue;
+            const int l = __builtin_ctzll(hit);
+            w = 64 * b + l;
+            sess = __builtin_amdgcn_readlane(begun[b][0], l);
+            group = __builtin_amdgcn_readlane(begun[b][1], l);
+            cols = __builtin_amdgcn_readlane(begun[b][3], l);
+            wide_log = __builtin_amdgcn_readlane(log[b], l);
+            e = u - (__builtin_amdgcn_readlane(incl[b], l) - ((cols + (1 << wide_log) - 1) >> wide_log) * NKV);
+        }
+        const int wide = 1 << wide_log, teams = kJoinRows >> wide_log, team = row & (teams - 1);
+        const int per = (cols + wide - 1) >> wide_log, kvh = e / per, cc = min(e % per * wide + (row >> __builtin_ctz(teams)), COLS - 1);
+        const int64_t at = (int64_t)kvh * a.slots * COLS + cc;
+        const Session s = session_of<true>(a, sess);
+        float m = kUnset, l = 0.f;
+        f4 o = f4{0.f, 0.f, 0.f, 0.f};
+        if (team == 0 && cc < cols) {
+            const int64_t from = at + (int64_t)(2 * w + 1) * COLS;
+            const f2 x = a.ml[from];
+            o = *reinterpret_cast<const f4*>(a.acc + from * HD + 4 * d);
+            m = x[0];
+            l = x[1];
+        }
+        auto add = [&](const f2 x, const f4 p) {
+            const float to = fmaxf(m, x[0]);
+            const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
+            l = l * f0 + x[1] * f1;
+            o = o * f0 + p * f1;
+            m = to;
+        };
+        for (int base = w + 1; base < a.gw; base += 64) {
+            i4 next = i4{-1, 0, 0, 0};
+            if (base + lane < a.gw) next = a.info[2 * (base + lane)];
+            const bool ours = next[0] == sess && next[1] == group;           // others: too short to have a tile of it
+            const uint64_t all = __builtin_amdgcn_ballot_w64(ours);
+            const int rank = __builtin_popcountll(all & (((uint64_t)1 << lane) - 1));
+            uint64_t todo = 0;                               // this team's
+            for (int t = 0; t < teams; ++t) {
+                const uint64_t x = __builtin_amdgcn_ballot_w64(ours && (rank & (teams - 1)) == t);
+                if (t == team) todo = x;
+            }
+            if (cc >= cols) todo = 0;
+            while (__builtin_amdgcn_ballot_w64(todo != 0)) {
+                f2 x[kAtOnce];
+                f4 p[kAtOnce];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    x[k] = f2{kUnset, 0.f};
+                    p[k] = f4{0.f, 0.f, 0.f, 0.f};
+                    if (todo) {
+                        const int64_t from = at + (int64_t)(2 * (base + __builtin_ctzll(todo))) * COLS;
+                        x[k] = a.ml[from];
+                        p[k] = *reinterpret_cast<const f4*>(a.acc + from * HD + 4 * d);
+                        todo &= todo - 1;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) add(x[k], p[k]);
+            }
+            if (__builtin_amdgcn_ballot_w64(ours && next[2])) break;         // the group's end
+        }
+        if (teams > 1) {
+            __syncthreads();                                 // the last unit has been read
+            s_o[row][d] = o;
+            if (d == 0) s_ml[row] = f2{m, l};
+            __syncthreads();
+            if (team) continue;
+            for (int t = 1; t < teams; ++t) add(s_ml[row + t], s_o[row + t][d]);
+        }
+        const int col = group * COLS + cc;
+        if (cc >= cols || col >= s.rows * G) continue;
+        const int r = col / G, hh = col - r * G;
+        *reinterpret_cast<f4*>(a.o + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d) = o * (1.0f / l);
+    }
 }
 
 // ---- host side ----
@@ -987,7 +1048,6 @@ __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr int kFewCols = 32;                   // columns per session up to which a workgroup's waves share them
-constexpr int kAimWgs = 512;                   // workgroups aimed at: two per CU
 constexpr int kMinShare = 4;                   // tiles: one per wave
 constexpr int kSoloPages = 48;            // see launch()
 constexpr int kJoinWgs = 2048;                 // a launch that fills the chip
@@ -1048,12 +1108,12 @@ void launch(Q8Args a, void* workspace, hipStream_t s) {
     a.info = reinterpret_cast<i4*>(ws + w.info);
     a.ml = reinterpret_cast<f2*>(ws + w.ml);
     a.acc = reinterpret_cast<float*>(ws + w.acc);
+    const unsigned join_wgs = (unsigned)std::min<int64_t>((int64_t)a.rows.n_rows * NH, kJoinWgs);
     if constexpr (kCausal) {
         if (f.many) {
             hipLaunchKernelGGL(q8_many_kernel, dim3(NKV, a.gw), dim3(THREADS), 0, s, a);
             NOVA_LAUNCHED();
-            hipLaunchKernelGGL(q8_many_join_kernel, dim3(a.gw, NKV, kManyCols / kJoinCols), dim3(THREADS),
-                               0, s, a);
+            hipLaunchKernelGGL(q8_many_join_kernel, dim3(join_wgs), dim3(THREADS), 0, s, a);
             NOVA_LAUNCHED();
             return;
         }
@@ -1079,9 +1139,7 @@ void launch(Q8Args a, void* workspace, hipStream_t s) {
     else run(std::false_type{});
     NOVA_LAUNCHED();
     if (solo) return;
-    const int64_t columns = (int64_t)a.rows.n_rows * NH;
-    hipLaunchKernelGGL(q8_few_join_kernel, dim3((unsigned)std::min<int64_t>(columns, kJoinWgs)), dim3(THREADS), 0, s, a,
-                       f.cols);
+    hipLaunchKernelGGL(q8_few_join_kernel, dim3(join_wgs), dim3(THREADS), 0, s, a, f.cols);
     NOVA_LAUNCHED();
 }
 

@@ -481,3 +481,29 @@ def test_workspace_is_enough():
         n.dev_sync()
         x.check("poisoned workspace")
         assert (n.download(guard, (65536,), np.uint8, size) == 0xff).all()
+
+
+@pytest.mark.parametrize("model,past,count", [
+    ("qwen25_7b", [30000], [8]),                             # one group in as many pieces as there are stretches
+    ("qwen25_1p5b", [20000], [9]),
+    ("qwen25_14b", [9000, 9000, 70], [12, 7, 9]),
+    ("qwen25_7b", [12000] + [40] * 12, [5] + [6] * 12),      # one long, many short
+    ("qwen25_7b", [5000, 2500, 1200, 600, 300], [30, 9, 20, 6, 40]),
+], ids=["one", "one small", "two of three", "one of many", "halves"])
+def test_groups_in_many_pieces(model, past, count):
+    """the joining launch gives a group's columns one to eight teams, by its pieces"""
+    c = Chunk(model, past, count, seed=60 + len(past))
+    c.launch()
+    c.nova.dev_sync()
+    print(f"  {c.check(f'{model} pieces'):.3f} of the bound")
+
+
+@pytest.mark.parametrize("model", MODELS)
+def test_many_tiny_sessions(model):
+    """more groups than tiles: a workgroup has few of them, or none"""
+    rng = np.random.default_rng(61)
+    count = [10] + rng.integers(0, 11, 299).tolist()
+    c = Chunk(model, rng.integers(0, 4, 300).tolist(), count, seed=62)
+    c.launch()
+    c.nova.dev_sync()
+    print(f"  {c.check(f'{model} tiny'):.3f} of the bound")
