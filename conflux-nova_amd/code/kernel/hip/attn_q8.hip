@@ -3,6 +3,32 @@
 //
 // o_h = sum_t softmax_t(q_h . k_t / sqrt(HD)) v_t, k_t = ks_t * code, v_t = vs_t * code,
 // over keys [0, n_keys) or, for row r of a chunk, [0, n_past + r].
+//
+// Numbers.  The codes are exact operands: the query goes into three signed digits of
+// base 256 against K's int8 codes (products and sums are exact integers), and a
+// weight times V's scale into two fp16 terms against V's codes, which fp16 holds
+// exactly; sums are fp32.  So the result has fp32's accuracy: 3e-7 to 6e-7 relative
+// to 64 bits, where fp32 arithmetic on the decoded values has 4e-7 to 2e-6.  That
+// costs one and a half fp16 products for the scores and two for the output.
+//
+// One pass over the keys with the running maximum and sum of the softmax.  The
+// maximum is a reference that follows lazily: weights are 2^(s - m) with m up to
+// kLazy below the true maximum, which fp32 and the two fp16 terms have room for, so
+// that almost no tile rescales its sums.
+//
+// Two kernels, by the columns (query rows x heads of a kv head) that a session may
+// have.  Up to 32: the waves of a workgroup share them and split the keys; K and V
+// go from the pages to registers once and HBM bounds it.  8 x 32768 keys of the 14B
+// model, 554 MB: 90 us, 6.2 TB/s; 16 sessions of 512 to 8192 keys (7B), 66 MB: 21.7 us
+// in two launches.  Above: 64 columns a workgroup, K and V through LDS, the
+// matrix instructions and the softmax's vector instructions bound it, of which a SIMD
+// overlaps a part only (a 16x16x32 product and 4 vector instructions take 16 and 16
+// clocks alone, 28 together).  8 x 512 tokens behind up to 4096 (7B), 122 GFLOP: 272 us, 450
+// TFLOP/s of the result's own products, twice that with the digits and terms.  A wave with
+// 32 columns, whose bigger products leave the vector unit more room, was 10 to 20%
+// slower: its operands and sums fill the 256 registers of two waves per SIMD, and
+// nothing is loaded ahead.  Three waves per SIMD, loads two tiles ahead and the scores of a tile
+// under the products of the one before it came out within 2% or slower.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cstdint>
@@ -31,8 +57,13 @@ constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
 constexpr int kAimWgs = 512;                   // workgroups aimed at: two per CU
-constexpr int kMinPiece = 3;                   // tiles of a group that is cut
-constexpr int kGroupTiles = 4;                 // what a group costs beside its tiles, in tiles
+// Many columns, 12 prompts of up to 300 tokens (1.5B) / 8 x 512 tokens behind up to
+// 4096 (7B), us.  Fewest tiles of a piece of a group: 2 37.3 / 266, 3 36.0 / 266, 4 39.0 / 272.
+constexpr int kMinPiece = 3;
+// What a group costs beside its tiles, in tiles: 0 43.2 / 277, 2 36.6 / 276, 4 39.0 / 272,
+// 8 35.7 / 279 with pieces of 4; short sessions need it most (8 of 19 rows, 7B: 0 135, 2 17.6,
+// 4 11.8, 8 12.0), as a workgroup is given several of them.
+constexpr int kGroupTiles = 4;
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -1e30f;               // reference of a column without keys, where states are joined
@@ -54,7 +85,7 @@ struct Q8Args {
     int min_share;             // fewest tiles of a workgroup that shares a session
     int slots;                 // partial results per kv head
     float* o;
-    i4* info;                  // few: [n_sess] {first slot, parts, rows, first row}; many: [2 gw] pieces
+    i4* info;                  // few: [n_sess] {first slot, parts, rows, first row}; many: [2 gw] {session, group, its end, columns}
     f2* ml;                    // [NKV][slots][cols] {reference, sum}
     float* acc;                // [NKV][slots][cols][HD]
 };
@@ -754,7 +785,8 @@ __device__ __forceinline__ void page_to_lds(const void* base, uint32_t lane16, u
         : "memory");
 }
 
-// Each wave has its own 16 columns of a group, and all go over the same keys.
+// Each wave has its own 16 columns of a group, and all go over the same keys: V's
+// conversion to fp16 is done once for 64 columns, and a tile's loads once.
 // Wave w brings page w of a tile: K straight to LDS, the
 // pages 64 B further apart than they are long so that the operand reads are free of
 // bank conflicts; V and the scales through registers, the codes turned into fp16 in
@@ -926,7 +958,9 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
 // group names it, the next ones follow until one has its end.  32 lanes per column,
 // and as many teams of them share a column's pieces as there are workgroups for.
 // Which of the next 64 stretches have a piece is read at once, and a team's pieces
-// eight at a time: the launch lasts as long as its memory latencies in a row.
+// eight at a time: the launch lasts as long as its memory latencies in a row, 2.5 us
+// each (8 rows behind 30000 keys, 7B, 128 pieces a group: the call takes 59 us with one
+// team, 28 with eight; without teams, 16 and 32 pieces at a time 56 and 58).
 constexpr int kJoinRows = THREADS / (HD / 4);
 static_assert(kJoinRows == 8, "columns or teams of a workgroup");
 __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
@@ -1047,8 +1081,14 @@ __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr int kFewCols = 32;                   // columns per session up to which a workgroup's waves share them
-constexpr int kMinShare = 4;                   // tiles: one per wave
+// Columns per session up to which a workgroup's waves share them.  At 17 to 32 columns
+// the other kernel is faster behind many long sessions (9 x 4400 keys, 4 rows, 7B: 29.5
+// instead of 35.3 us; 24 x 3000: 38.1, 44.5) and slower for few or short ones (1 x 30000: 57.3,
+// 37.3; 16 x 600: 19.8, 17.5; 32 x 100: 14.0, 11.5); the host knows the columns, not the keys.
+constexpr int kFewCols = 32;
+// Tiles of a workgroup that shares a session: one per wave.  Many columns, 12 prompts
+// of up to 300 tokens (1.5B): 2 42.9 us, 4 43.1, 6 44.3, 8 57.4.
+constexpr int kMinShare = 4;
 constexpr int kSoloPages = 48;            // see launch()
 constexpr int kJoinWgs = 2048;                 // a launch that fills the chip
 

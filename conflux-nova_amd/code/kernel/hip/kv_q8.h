@@ -2,12 +2,12 @@
 //
 // A cached row x (128 values of one token and kv head, K or V) is held as int8
 // codes c with one fp32 scale s, value = c * s.  A page of one layer is a record
-// of kRecBytes per kv head, [layer][NB][NKV][kRecBytes]:
+// of kQ8Rec bytes per kv head, [layer][NB][NKV][kQ8Rec]:
 //
 //   K codes   token t, dim d at (t >> 2) * 512 + (d >> 4) * 64 + (t & 3) * 16 + (d & 15)
-//   V codes   token t, dim d at kVOff + d * 16 + t
-//   K scales  token t at kKsOff + 4 t
-//   V scales  token t at kVsOff + 4 t
+//   V codes   token t, dim d at kQ8VOff + d * 16 + t
+//   K scales  token t at kQ8KsOff + 4 t
+//   V scales  token t at kQ8VsOff + 4 t
 //
 // The layout is what the matrix instructions of attn_q8.hip read, 16 B per lane
 // with nothing to move afterwards.  The score product is K . Q^T over 64 dims
