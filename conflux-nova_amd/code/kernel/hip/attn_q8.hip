@@ -7,8 +7,9 @@
 // Numbers.  The codes are exact operands: the query goes into three signed digits of
 // base 256 against K's int8 codes (products and sums are exact integers), and a
 // weight times V's scale into two fp16 terms against V's codes, which fp16 holds
-// exactly; sums are fp32.  So the result has fp32's accuracy: 3e-7 to 6e-7 relative
-// to 64 bits, where fp32 arithmetic on the decoded values has 4e-7 to 2e-6.  That
+// exactly; sums are fp32.  So the result has fp32's accuracy: 1e-7 (a handful of
+// keys) to 6e-7 (tens of thousands) relative to 64 bits, where fp32 operations on
+// the decoded values have 2e-8 to 2e-6.  That
 // costs one and a half fp16 products for the scores and two for the output.
 //
 // One pass over the keys with the running maximum and sum of the softmax.  The
