@@ -957,7 +957,8 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
 
 // Joins the pieces of groups that several workgroups had: the one that began a
 // group names it, the next ones follow until one has its end.  32 lanes per column,
-// and as many teams of them share a column's pieces as there are workgroups for.
+// and up to eight teams of them share a column's pieces, as many as its pieces need
+// and there are workgroups for.
 // Which of the next 64 stretches have a piece is read at once, and a team's pieces
 // eight at a time: the launch lasts as long as its memory latencies in a row, 2.5 us
 // each (8 rows behind 30000 keys, 7B, 128 pieces a group: the call takes 59 us with one
@@ -1091,7 +1092,9 @@ constexpr int kFewCols = 32;
 // of up to 300 tokens (1.5B): 2 42.9 us, 4 43.1, 6 44.3, 8 57.4.
 constexpr int kMinShare = 4;
 constexpr int kSoloPages = 48;            // see launch()
-constexpr int kJoinWgs = 2048;                 // a launch that fills the chip
+// A joining launch that fills the chip (4096: 16 sessions of 1 to 8 rows, 7B, 34.8 us instead
+// of 34.4; 12 prompts of up to 300 tokens, 1.5B, 38.5, 37.4).
+constexpr int kJoinWgs = 2048;
 
 // What a call of these counts runs with: the columns of a workgroup and the partial
 // results per kv head.
