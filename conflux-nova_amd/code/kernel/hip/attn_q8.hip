@@ -12,10 +12,11 @@
 // the decoded values have 2e-8 to 2e-6.  That
 // costs one and a half fp16 products for the scores and two for the output.
 //
-// One pass over the keys with the running maximum and sum of the softmax.  The
-// maximum is a reference that follows lazily: weights are 2^(s - m) with m up to
-// kLazy below the true maximum, which fp32 and the two fp16 terms have room for, so
-// that almost no tile rescales its sums.
+// One pass over the keys with a running reference and sum of the softmax.  The
+// reference m of the weights 2^(s - m) follows the largest weight times V scale, lazily:
+// that product may drift from 2^kTop to 2^kLazy, which the two fp16 terms have room
+// for, so that almost no tile rescales its sums (kTop 2: 268 instead of 275 us for the
+// 8 x 512 tokens below, and 4 bits less for the small products).
 //
 // Two kernels, by the columns (query rows x heads of a kv head) that a session may
 // have.  Up to 32: the waves of a workgroup share them and split the keys; K and V
@@ -68,7 +69,10 @@ constexpr int kGroupTiles = 4;
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -1e30f;               // reference of a column without keys, where states are joined
-constexpr float kTop = 6.f, kLazy = 14.f;      // log2 of a column's largest weight: where it is put, where it may drift
+constexpr float kTop = 6.f, kLazy = 15.9f;      // log2 of a column's largest weight times value scale: where it is put, where it may drift
+constexpr int kUnitLow = -44, kUnitHigh = 35;  // log2 of the units of value scales
+constexpr float kHighFrom = 0x1p42f;           // the scale from which the high one is needed
+constexpr float kFloor = -82.f;                // log2 of the smallest scale, in units, that the reference follows
 constexpr int kAccRow = HD + 4;                // floats per column in LDS: rows on different banks
 static_assert(HD == 128 && kTilePages == 4 && G <= 16, "tile layout");
 
@@ -145,6 +149,15 @@ __device__ __forceinline__ float rows_sum(float v) {
     v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+
+// over all lanes
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, true)));   // row_ror 8, 4, 2, 1
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x124, 0xf, 0xf, true)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x122, 0xf, 0xf, true)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x121, 0xf, 0xf, true)));
+    return rows_max(v);
 }
 
 template <int... I, class F>
@@ -442,9 +455,23 @@ struct Pages {
     }
 };
 
+// 2^d, d <= 0, for a state moved to a reference -d higher: in halves for the sum of
+// weights, as these are 2^98 at most and the largest of a column 2^-80 at least, so
+// that a factor below fp32 may leave a sum that counts.  The sums of products
+// stand at one size and need no such care.
+struct Factor {
+    float half, all;
+    __device__ __forceinline__ explicit Factor(float d) : half(__builtin_amdgcn_exp2f(0.5f * d)), all(half * half) {}
+    __device__ __forceinline__ float of_weights(float l) const { return l * half * half; }
+};
+
 // A block's state over the keys seen so far: lane (g, c) holds the reference, its
-// share of the sum and dims 16 d + 4 g .. + 3 of column c.  A score above `limit`
-// moves the reference (a column's first one always).
+// share of the sum and dims 16 d + 4 g .. + 3 of column c.  Weights are 2^(s - m).
+// They meet V's codes as 2^(s - m) vs in two fp16 terms, which end at 2^-24, so the
+// reference follows the largest of these products among the keys that the column
+// sees, not the largest score: what a key may lose is 2^-30 of the largest one, whatever
+// the scales of keys that are hidden or weigh nothing.  A score above `limit` may move
+// the reference (a column's first one always does).
 struct State {
     float m, l, limit;
     f4 acc[DB];
@@ -454,49 +481,63 @@ struct State {
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ float reference() const { return limit == kLazy ? m : kUnset; }
+    __device__ __forceinline__ bool unset() const { return limit == -INFINITY; }
+    __device__ __forceinline__ float reference() const { return unset() ? kUnset : m; }
     __device__ __forceinline__ void scale_acc(float f) {
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] *= f;
     }
 };
 
-// The weights meet V's codes as 2^(s - m) vs, which have to stay inside fp16.  So V's
-// scales are taken relative to a power of two, `unit`, the same for all columns of a
-// wave: it moves up (and the accumulators with it) when a scale passes twice its
-// size, and stands at the first tile's largest scale to begin with.
+// V's scales in units, so that weights (from 2^(kTop - log2 vs) for the largest
+// product) stay inside fp32 with their tails: a unit serves scales of 2^-82 to 2^86 of
+// its own size.  The low one's are 2^-126 (the quantiser's smallest) to 2^42; a larger scale takes the
+// wave to the high one, 2^-47 to 2^121 (the largest).  There, beside values of
+// 2^49 and more, a column whose values are all below 2^-40 loses bits.
 struct ValueUnit {
-    float unit, most;          // most: the scale that moves it
+    float inv;                 // 1 / unit
+    float most, cap;           // no scale so far is larger; its log2 in units, or kFloor
+    __device__ __forceinline__ bool low() const { return inv > 1.f; }
+    __device__ __forceinline__ float unit() const { return low() ? ldexpf(1.f, kUnitLow) : ldexpf(1.f, kUnitHigh); }
     __device__ __forceinline__ void clear() {
-        unit = 1.f;
+        inv = ldexpf(1.f, -kUnitLow);
         most = 0.f;
+        cap = kFloor;
     }
     // vs: scale of the lane's key, 0 where there is none; returns it in units
     template <int NB>
     __device__ __forceinline__ float take(float vs, State (&st)[NB]) {
         if (__builtin_amdgcn_ballot_w64(vs > most)) {        // rare
-            float top = vs;                                  // (a NaN does not count)
+            const float top = wave_max(vs);                  // (a NaN does not count)
+            if (low() && top >= kHighFrom) {
+                // products keep their size: the reference goes down by as much as the
+                // unit goes up, as far as the weights' sum has room for, the sums for the rest
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-            int ex;
-            (void)frexpf(top, &ex);
-            const float to = ldexpf(1.f, ex);                // top < to
-            const float f = most == 0.f ? 0.f : unit / to;   // before the first scale there is nothing to keep
+                for (int b = 0; b < NB; ++b) {
+                    int ex;
+                    (void)frexpf(rows_max(st[b].l), &ex);
+                    const int by = min(max(90 - ex, 0), kUnitHigh - kUnitLow);
+                    st[b].m -= (float)by;
+                    st[b].l = ldexpf(st[b].l, by);
+                    st[b].scale_acc(ldexpf(1.f, by - (kUnitHigh - kUnitLow)));
+                }
+                inv = ldexpf(1.f, -kUnitHigh);
+            }
+            most = 1.125f * top;                             // (so that few tiles come here)
+            cap = fmaxf(__builtin_amdgcn_logf(most * inv), kFloor);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) st[b].scale_acc(f);
-            unit = to;
-            most = 2.f * to;
+            for (int b = 0; b < NB; ++b) st[b].limit = st[b].unset() ? -INFINITY : kLazy - cap;
         }
-        return vs * (1.f / unit);
+        return vs * inv;
     }
 };
 
 // Scores, weights and sum of one tile and block.  k_op(u): K operand u = 2 kb + h
 // (dims 64 h .. of key block kb), q_op(d, h): the query's; ks and vs: the K scale of
-// the lane's key and its V scale in units; key0: first key of the lane's page.  The
-// weights come out in two fp16 terms, so that V's codes can follow as they are.
+// the lane's key and its V scale in units, none above 2^cap; key0: first key of the
+// lane's page.  The weights come out in two fp16 terms, so that V's codes can follow as they are.
 template <bool kMask, class K, class Q>
-__device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float ks, float vs, int key0, int seen, State& st,
+__device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float ks, float vs, float cap, int key0, int seen, State& st,
                                       h8 (&hi)[2], h8 (&lo)[2]) {
     // The lowest digit's sum starts at the bits of 1.5 * 2^23, so that it is that
     // float plus the sum without a conversion; the middle one starts 1.5 * 2^23 / 256
@@ -523,18 +564,27 @@ __device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float k
         });
     });
     if (__builtin_amdgcn_ballot_w64(top > st.limit)) {
-        // rare: a column's first keys, and a score more than kLazy above the
-        // reference, put it to kTop below the largest score
-        const float col_top = rows_max(top);
-        const bool moves = col_top > st.limit;
+        // rare: a column's first keys, and a product that may be above 2^kLazy (it is
+        // where its key has the largest scale so far), which puts the reference to where
+        // the largest product is 2^kTop
+        const float r = fmaxf(__builtin_amdgcn_logf(vs), kFloor);
+        float t = -INFINITY;
+        each<16>([&](auto j) { t = fmaxf(t, x[j] + row_lane<j>(r)); });
+        const float col_top = rows_max(t);
+        const bool first = st.unset(), moves = first ? col_top > -INFINITY : rows_max(top) > st.limit && col_top > kTop;
         const float by = moves ? col_top - kTop : 0.f;
-        const float corr = st.limit == kLazy ? __builtin_amdgcn_exp2f(-by) : 0.f;
+        const Factor corr(first ? -INFINITY : -by);
         st.m += by;
-        st.limit = moves ? kLazy : st.limit;
-        st.l *= corr;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] -= by;
-        st.scale_acc(corr);
+        st.limit = moves ? kLazy - cap : st.limit;
+        st.l = corr.of_weights(st.l);
+        each<16>([&](auto j) {
+            // scores of 2^23 and more leave no room for log2 vs beside them: the product stays below
+            // its bound all the same (and a NaN is left as it is)
+            const float most = kLazy - row_lane<j>(r);
+            x[j] -= by;
+            x[j] = x[j] > most ? most : x[j];
+        });
+        st.scale_acc(corr.all);
     }
     float e[2][8];
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -623,8 +673,8 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q8_few_kernel(Q8Args
         h8 hi[NB][2], lo[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            weigh<kMask>([&](int u) { return kr[u]; }, [&](int d, int h) { return q[b].d[d][h]; }, q[b].scale, ks, sv, key0, seen[b], st[b], hi[b],
-                         lo[b]);
+            weigh<kMask>([&](int u) { return kr[u]; }, [&](int d, int h) { return q[b].d[d][h]; }, q[b].scale, ks, sv, unit.cap, key0, seen[b], st[b],
+                         hi[b], lo[b]);
         const bool more = t + 1 < t1;
         if (more) load_k(t + 1);
 #pragma unroll
@@ -648,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q8_few_kernel(Q8Args
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const float l = rows_sum(st[b].l);
-        st[b].scale_acc(unit.unit);
+        st[b].scale_acc(unit.unit());
         if (g == 0) {
             s_m[wave][16 * b + c] = st[b].reference();
             s_l[wave][16 * b + c] = l;
@@ -672,9 +722,9 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q8_few_kernel(Q8Args
             float l = 0.f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(s_m[w][col] - m);
-                sum += *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]) * f;
-                l += s_l[w][col] * f;
+                const Factor f(s_m[w][col] - m);
+                sum += *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]) * f.all;
+                l += f.of_weights(s_l[w][col]);
             }
             if (p.parts == 1) {
                 const int r = col / G, hh = col - r * G;
@@ -728,9 +778,9 @@ __global__ void __launch_bounds__(THREADS) q8_few_join_kernel(Q8Args a, int cols
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float to = fmaxf(m, x[k][0]);
-                    const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[k][0] - to);
-                    ll = ll * f0 + x[k][1] * f1;
-                    o = o * f0 + v[k] * f1;
+                    const Factor f0(m - to), f1(x[k][0] - to);
+                    ll = f0.of_weights(ll) + f1.of_weights(x[k][1]);
+                    o = o * f0.all + v[k] * f1.all;
                     m = to;
                 }
             }
@@ -749,9 +799,9 @@ __global__ void __launch_bounds__(THREADS) q8_few_join_kernel(Q8Args a, int cols
             ll = 0.f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(s_m[w] - m);
-                o += s_o[w][lane] * f;
-                ll += s_l[w] * f;
+                const Factor f(s_m[w] - m);
+                o += s_o[w][lane] * f.all;
+                ll += f.of_weights(s_l[w]);
             }
             const int r = col / G, hh = col - r * G;
             *reinterpret_cast<f2*>(a.o + ((int64_t)(row0 + r) * NH + kvh * G + hh) * HD + 2 * lane) = o * (1.0f / ll);
@@ -890,7 +940,7 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
             const float ks = s_scale[t & 1][0][lane], vs = unit.take(s_scale[t & 1][1][lane], st);
             h8 hi[2], lo[2];
             weigh<kMask>([&](int u) { return *reinterpret_cast<const i4*>(k_at + 256 * u); },
-                         [&](int d, int h) { return q.d[d][h]; }, q.scale, ks, vs, key0, seen, st[0], hi, lo);
+                         [&](int d, int h) { return q.d[d][h]; }, q.scale, ks, vs, unit.cap, key0, seen, st[0], hi, lo);
 #pragma unroll
             for (int e = 0; e < 2 * DB / 4; ++e) {           // two 16-dim blocks, two halves of their tokens
                 h8 v[2][2];
@@ -930,7 +980,7 @@ __global__ void __launch_bounds__(THREADS, 2) q8_many_kernel(Q8Args a) {
         unsigned char* mine = s_mem + wave * kOut;
         if (col0 < n_cols) {
             const float l = rows_sum(st[0].l), m = st[0].reference();
-            st[0].scale_acc(unit.unit);
+            st[0].scale_acc(unit.unit());
 #pragma unroll
             for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(mine + (c * kAccRow + 16 * d + 4 * g) * 4) = st[0].acc[d];
             wave_lds_sync();
@@ -1028,9 +1078,9 @@ __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
         }
         auto add = [&](const f2 x, const f4 p) {
             const float to = fmaxf(m, x[0]);
-            const float f0 = __builtin_amdgcn_exp2f(m - to), f1 = __builtin_amdgcn_exp2f(x[0] - to);
-            l = l * f0 + x[1] * f1;
-            o = o * f0 + p * f1;
+            const Factor f0(m - to), f1(x[0] - to);
+            l = f0.of_weights(l) + f1.of_weights(x[1]);
+            o = o * f0.all + p * f1.all;
             m = to;
         };
         for (int base = w + 1; base < a.gw; base += 64) {

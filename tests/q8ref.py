@@ -145,3 +145,30 @@ def assert_within(got, ref, tol, what):
     worst = (err / np.maximum(tol, 1e-30)).max(initial=0)
     assert (err <= tol).all(), f"{what}: {worst:.2f} of the bound, max abs {err.max():.3e}"
     return worst
+
+
+def attention_by_row(q, k, v, v_scale, first, group):
+    """The formula as in `attention`, and a bound that is each row's own: only keys
+    that the row sees enter it, with their weights.
+
+    e is the relative error of a weight as derived there.  An output element is
+    sum p_j v_j, so weights off by e move it by at most 2 e sum p_j |v_j|, taken per
+    element.  A weight times its value's scale is also rounded to a fixed step: two fp16
+    terms, cut below 2^-24, where the row's largest such product stands at 2^6 or
+    more, so each of n keys adds up to 2^-30 of the largest p_j times its value's
+    largest component (127 scales).  v_scale: the scales [T][NKV]."""
+    n, nh, _ = q.shape
+    out, tol = np.zeros((n, nh, HD)), np.zeros((n, nh, HD))
+    for h in range(nh):
+        kh, vh, sh = k[:, h // group], v[:, h // group], v_scale[:, h // group].astype(np.float64)
+        for r in range(n):
+            m = min(first + r, len(kh))
+            x = q[r, h].astype(np.float64)
+            s = kh[:m] @ x / np.sqrt(HD)
+            size = (np.abs(kh[:m]) @ np.abs(x) + np.abs(x).max() * np.abs(kh[:m]).sum(-1)) / np.sqrt(HD)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            e = 2.0 ** -20 * size.max() + 2.0 ** -20 + (m / 32 + 64) * 2.0 ** -24
+            out[r, h] = p @ vh[:m]
+            tol[r, h] = 2 * e * (p @ np.abs(vh[:m])) + m * 2.0 ** -30 * 127 * (p * sh[:m]).max()
+    return out, tol

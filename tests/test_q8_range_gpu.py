@@ -1,0 +1,115 @@
+"""Attention over 8-bit pages whose rows have far apart scales: a row's result depends
+on the keys it sees, each by its weight, whatever stands beside them."""
+import numpy as np
+import pytest
+
+from q8ref import HD, KB, Q8Pool, attention_by_row, pack, unpack, values
+
+pytestmark = pytest.mark.gpu
+LAYER = 2
+MODEL = "qwen25_1p5b"
+
+
+class Call:
+    """A chunk of `count` rows per session behind `past` keys (decode: the last key's
+    query), over pages whose codes and scales a test has changed."""
+
+    def __init__(self, past, count, seed, scale=0.5, decode=False):
+        import nova_amd
+        self.nova = nova = nova_amd.load(MODEL)
+        self.decode = decode
+        self.past, self.count = np.asarray(past, np.int32), np.asarray(count)
+        self.keys = self.past + self.count
+        self.off = np.concatenate([[0], np.cumsum(self.count)]).astype(np.int32)
+        self.n = int(self.off[-1])
+        pages = (self.keys + KB - 1) // KB
+        self.pool = Q8Pool(nova, int(pages.sum()) + 1, LAYER, seed)
+        self.table = self.pool.tables(pages)
+        self.parts = [np.array(x) for x in unpack(self.pool.rec)]     # K codes, K scales, V codes, V scales
+        self.q = (self.pool.rng.standard_normal((self.n, nova.nh, HD)) * scale).astype(np.float32)
+
+    def at(self, sess, key):
+        """index of a key's scales and codes: [page, all heads, token]"""
+        return self.table[sess, key // KB], slice(None), key % KB
+
+    def towards(self, sess, key, score):
+        """all of the session's queries share a direction u, and this key is a multiple
+        of it, so that its score is about `score` for each of them"""
+        u = np.where(np.arange(HD) % 3 == 0, 1.0, -1.0)
+        a, b = self.off[sess], self.off[sess + 1]
+        self.q[a:b] += np.float32(2) * u.astype(np.float32) - (self.q[a:b] @ u.astype(np.float32))[..., None] * u.astype(np.float32) / HD
+        self.parts[0][self.at(sess, key)] = np.where(score < 0, -127, 127) * u
+        self.parts[1][self.at(sess, key)] = abs(score) * np.sqrt(HD) / (2 * HD * 127)
+
+    def run(self):
+        n, p = self.nova, self.pool
+        p.rec = pack(*self.parts)
+        p.push()
+        lens = self.keys if self.decode else self.past
+        dt, dn, doff, dq = (n.upload(np.ascontiguousarray(x)) for x in (self.table, lens.astype(np.int32), self.off, self.q))
+        o = n.upload(np.full(self.q.shape, 3, np.float32))
+        if self.decode:
+            ws = n.alloc(n.attn_decode_q8_workspace_bytes(len(lens)))
+            n.launch_attn_decode_q8_batch(dq.ptr, p.dev.ptr, dt.ptr, self.table.shape[1], dn.ptr, len(lens), LAYER, p.nb, o.ptr,
+                                          ws.ptr, None)
+        else:
+            most = int(self.count.max())
+            ws = n.alloc(n.attn_chunk_q8_workspace_bytes(len(lens), self.n, most))
+            n.launch_attn_chunk_q8_batch(dq.ptr, p.dev.ptr, dt.ptr, self.table.shape[1], dn.ptr, doff.ptr, len(lens), self.n,
+                                         most, LAYER, p.nb, o.ptr, ws.ptr, None)
+        n.dev_sync()
+        return o.numpy(self.q.shape, np.float32)
+
+    def check(self):
+        got = self.run()
+        assert np.isfinite(got).all()
+        worst = 0.0
+        for i in range(len(self.past)):
+            a, b = self.off[i], self.off[i + 1]
+            m = int(self.keys[i])
+            k, v = values(self.pool.rec, self.table[i], m)
+            pos = np.arange(m)
+            vs = self.parts[3][self.table[i][pos >> 4], :, pos & 15]
+            ref, tol = attention_by_row(self.q[a:b], k, v, vs, int(self.past[i]) + 1, self.nova.group)
+            ratio = np.abs(got[a:b].astype(np.float64) - ref) / np.maximum(tol, 1e-300)
+            worst = max(worst, ratio.max())
+            r = np.unravel_index(ratio.argmax(), ratio.shape)
+            assert ratio.max() <= 1, f"session {i}, row, head, dim {r}: {got[a:b][r]} instead of {ref[r]}, {ratio.max():.3g} of the bound"
+        print(f"  {worst:.3f} of the bound")
+
+
+# rows of a session: 1 and 4 take the kernels of few columns, 70 that of many
+FORMS = [(1, True), (1, False), (4, False), (70, False)]
+
+
+@pytest.mark.parametrize("power", [14, 20, 26, 34, 40, 100])
+@pytest.mark.parametrize("rows", [4, 70])
+def test_later_tokens_do_not_touch_earlier_rows(rows, power):
+    """a token whose value scale is 2^power times the others', hidden from the rows before it"""
+    c = Call([30, 200], [rows, rows], seed=1)
+    for sess in (0, 1):
+        c.parts[3][c.at(sess, int(c.past[sess]) + rows // 2)] *= np.float32(2.0 ** power)
+    c.check()
+
+
+@pytest.mark.parametrize("power", [10, 20, 40, 100])
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_large_value_of_small_weight(rows, decode, power):
+    """a key that all rows see, its value 2^power times the others', its weight 2^-144"""
+    c = Call([900 - rows, 130], [rows, rows], seed=2, decode=decode)
+    for sess, key in ((0, 333), (1, 3)):
+        c.towards(sess, key, -100.0)
+        c.parts[3][c.at(sess, key)] *= np.float32(2.0 ** power)
+    c.check()
+
+
+@pytest.mark.parametrize("score", [8.0, 40.0])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -60, 2.0 ** -20])
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_small_value_of_large_weight(rows, decode, size, score):
+    """a key that takes nearly all of the weight, its value zero or small: the others' count"""
+    c = Call([900 - rows, 130], [rows, rows], seed=3, decode=decode)
+    for sess, key in ((0, 333), (1, 3)):
+        c.towards(sess, key, score)
+        c.parts[3][c.at(sess, key)] *= np.float32(size)
+    c.check()
