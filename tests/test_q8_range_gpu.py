@@ -113,3 +113,22 @@ def test_small_value_of_large_weight(rows, decode, size, score):
         c.towards(sess, key, score)
         c.parts[3][c.at(sess, key)] *= np.float32(size)
     c.check()
+
+
+@pytest.mark.parametrize("keys", [40, 3000])
+@pytest.mark.parametrize("rows,decode", FORMS)
+@pytest.mark.parametrize("top", [1e-34, 1e20, 1e33, 1e37])
+def test_values_near_the_ends_of_fp32(rows, decode, keys, top):
+    """all values of a size, under weights that are nearly equal"""
+    c = Call([max(keys - rows, 0)], [rows], seed=4, scale=0.01, decode=decode)
+    c.parts[3] *= np.float32(top / c.parts[3].max() / 127)
+    c.check()
+
+
+@pytest.mark.parametrize("key", [7, 2000])
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_one_value_near_the_end_of_fp32(rows, decode, key):
+    """one row of 1e37 among ordinary ones, in the first tile or later"""
+    c = Call([3000], [rows], seed=4, decode=decode)
+    c.parts[3][c.at(0, key)] *= np.float32(1e37 / 127 / c.parts[3][c.at(0, key)].max())
+    c.check()
