@@ -557,8 +557,9 @@ __device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float k
         }
         each<4>([&](auto i) {
             constexpr int e = i, j = 4 * kb + i;
-            const float w = fmaf((float)((z[0][e] << 8) + z[1][e]), 256.f, __int_as_float(z[2][e])) * row_lane<j>(ks);
-            x[j] = fmaf(w, q_scale, -st.m);
+            // the two scales first: the sum of codes times K's alone may pass fp32
+            const float w = fmaf((float)((z[0][e] << 8) + z[1][e]), 256.f, __int_as_float(z[2][e]));
+            x[j] = fmaf(w, row_lane<j>(ks) * q_scale, -st.m);
             if (kMask && key0 + j >= seen) x[j] = -INFINITY;
             top = fmaxf(top, x[j]);
         });

@@ -132,3 +132,13 @@ def test_one_value_near_the_end_of_fp32(rows, decode, key):
     c = Call([3000], [rows], seed=4, decode=decode)
     c.parts[3][c.at(0, key)] *= np.float32(1e37 / 127 / c.parts[3][c.at(0, key)].max())
     c.check()
+
+
+@pytest.mark.parametrize("power", [-90, 100])
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_large_keys_and_small_queries(rows, decode, power):
+    """keys 2^power times, queries 2^-power times as large: the same scores"""
+    c = Call([700], [rows], seed=5, decode=decode)
+    c.parts[1] *= np.float32(2.0 ** power)
+    c.q *= np.float32(2.0 ** -power)
+    c.check()
