@@ -68,7 +68,7 @@ constexpr int kMinPiece = 3;
 constexpr int kGroupTiles = 4;
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
-constexpr float kUnset = -1e30f;               // reference of a column without keys, where states are joined
+constexpr float kUnset = -3.40282347e38f;      // reference of a column without keys, where states are joined: below every other
 constexpr float kTop = 6.f, kLazy = 15.9f;      // log2 of a column's largest weight times value scale: where it is put, where it may drift
 constexpr int kUnitLow = -44, kUnitHigh = 35;  // log2 of the units of value scales
 constexpr float kHighFrom = 0x1p42f;           // the scale from which the high one is needed

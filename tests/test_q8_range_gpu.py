@@ -142,3 +142,24 @@ def test_large_keys_and_small_queries(rows, decode, power):
     c.parts[1] *= np.float32(2.0 ** power)
     c.q *= np.float32(2.0 ** -power)
     c.check()
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("keys", [1, 90, 2000])
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_scores_of_any_size(rows, decode, keys, sign):
+    """Scores of 1e33 and more, all of one sign, key j's (1 + j / 64) times the first
+    one's: the largest takes everything, and a row's result is its value."""
+    c = Call([keys - 1], [rows], seed=6, decode=decode)
+    n = c.past[0] + rows
+    u = np.where(np.arange(HD) % 3 == 0, 1, -1)
+    for j in range(n):
+        c.parts[0][c.at(0, j)] = 100 * u
+        c.parts[1][c.at(0, j)] = 1e14 * (1 + j / 64)
+    c.q[:] = sign * 1e15 * u
+    got = c.run()
+    _, v = values(c.pool.rec, c.table[0], int(n))
+    for r in range(rows):
+        want = np.repeat(v[0 if sign < 0 else c.past[0] + r], c.nova.group, 0)
+        # weight times scale: two fp16 terms, 2^-21, and three fp32 operations
+        assert (np.abs(got[r] - want) <= 2.0 ** -20 * np.abs(want)).all(), (r, got[r][0][:4], want[0][:4])
