@@ -223,14 +223,26 @@ __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
         total += __builtin_amdgcn_readlane(scan_incl(tiles), 63);
     }
     // Whole tiles for each wave (nine tiles last as long as twelve), and no more parts
-    // than workgroups that run at once: one that has to wait doubles the time.
-    int share = (max((total + a.gw - 1) / a.gw, a.min_share) + WAVES - 1) / WAVES * WAVES;
-    if (a.n_sess <= 64)
-        while (__builtin_amdgcn_readlane(scan_incl((tiles + share - 1) / share), 63) > a.gw && share < total) share += WAVES;
+    // than workgroups that run at once, as one that has to wait may double the time, but
+    // for that no more than half a share on top: where the sessions alone fill the chip,
+    // parts of the first size that wait cost less than sessions that are not cut.
+    const int least = (max((total + a.gw - 1) / a.gw, a.min_share) + WAVES - 1) / WAVES * WAVES;
+    int share = least;
+    auto parts_of = [&] { return s.rows > 0 ? max((tiles + share - 1) / share, 1) : 0; };
+    if (a.n_sess <= 64) {
+        const int step = max(least / 16 / WAVES, 1) * WAVES;
+        while (__builtin_amdgcn_readlane(scan_incl(parts_of()), 63) > a.gw) {
+            share += step;
+            if (share > least + least / 2) {
+                share = least;
+                break;
+            }
+        }
+    }
     int before = 0;
     for (int base = 0; base < a.n_sess; base += 64) {
         if (a.n_sess > 64) load(base);
-        const int parts = s.rows > 0 ? max((tiles + share - 1) / share, 1) : 0;
+        const int parts = parts_of();
         const int incl = before + scan_incl(parts);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > slot);
         if (hit) {
