@@ -203,12 +203,16 @@ void launch_kv_cow_apply(uint16_t* pool_k, uint16_t* pool_v, int nb, int32_t* ta
 
 void launch_kv_zero_pages(uint16_t* pool_k, uint16_t* pool_v, int nb, const int32_t* pages, int n_pages,
                           nova_stream_t s) {
-    NOVA_REQUIRE(pool_k && pool_v && nb > 0 && n_pages >= 0 && n_pages <= 65535);
+    NOVA_REQUIRE(pool_k && pool_v && nb > 0 && n_pages >= 0);
     if (n_pages == 0) return;
     NOVA_REQUIRE(pages);
-    hipLaunchKernelGGL(zero_pages_kernel, dim3(copy_chunks(), n_pages), dim3(256), 0,
-                       reinterpret_cast<hipStream_t>(s), pool_k, pool_v, nb, pages);
-    NOVA_LAUNCHED();
+    constexpr int kPagesPerLaunch = 65535;         // a launch's grid
+    for (int base = 0; base < n_pages; base += kPagesPerLaunch) {
+        const int n = n_pages - base < kPagesPerLaunch ? n_pages - base : kPagesPerLaunch;
+        hipLaunchKernelGGL(zero_pages_kernel, dim3(copy_chunks(), n), dim3(256), 0,
+                           reinterpret_cast<hipStream_t>(s), pool_k, pool_v, nb, pages + base);
+        NOVA_LAUNCHED();
+    }
 }
 
 void launch_table_patch(int32_t* table_dev, const int32_t* idx, const int32_t* val, int n, nova_stream_t s) {

@@ -327,6 +327,8 @@ q8_zero_kernel(uint8_t* __restrict__ pool, int nb, const int32_t* __restrict__ p
 // workgroups per page over all layers: 8 vectors per thread
 constexpr int kCopyChunks = (int)((Model::L * kPageVecs + 256 * 8 - 1) / (256 * 8));
 
+constexpr int kPagesPerLaunch = 65535;         // of clears: a launch's grid
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Host checks and the grid of the row kernels.  A run of n rows touches at most
@@ -446,12 +448,14 @@ void launch_kv_q8_cow_apply(uint8_t* pool, int nb, int32_t* tables_dev, const no
 }
 
 void launch_kv_q8_zero_pages(uint8_t* pool, int nb, const int32_t* pages, int n_pages, nova_stream_t s) {
-    NOVA_REQUIRE(pool && aligned16(pool) && nb > 0 && n_pages >= 0 && n_pages <= 65535);
+    NOVA_REQUIRE(pool && aligned16(pool) && nb > 0 && n_pages >= 0);
     if (n_pages == 0) return;
     NOVA_REQUIRE(pages);
-    hipLaunchKernelGGL(q8_zero_kernel, dim3(kCopyChunks, n_pages), dim3(256), 0, reinterpret_cast<hipStream_t>(s), pool,
-                       nb, pages);
-    NOVA_LAUNCHED();
+    for (int base = 0; base < n_pages; base += kPagesPerLaunch) {
+        hipLaunchKernelGGL(q8_zero_kernel, dim3(kCopyChunks, std::min(n_pages - base, kPagesPerLaunch)), dim3(256), 0,
+                           reinterpret_cast<hipStream_t>(s), pool, nb, pages + base);
+        NOVA_LAUNCHED();
+    }
 }
 
 }  // extern "C"
