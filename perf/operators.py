@@ -221,10 +221,13 @@ _WORKSPACE = {}
 
 
 def _workspace(nbytes):
-    """One workspace for all calls of the program, as long as it is large enough."""
-    if "buf" not in _WORKSPACE or _WORKSPACE["buf"].numel() < nbytes:
-        _WORKSPACE["buf"] = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-    return _WORKSPACE["buf"].data_ptr()
+    """One workspace for the calls of each stream, as long as it is large enough: calls on two streams may overlap.
+    A larger one takes its place in the stream's own order (it is allocated on that stream)."""
+    stream = torch.cuda.current_stream()
+    key = stream.device_index, stream.cuda_stream
+    if key not in _WORKSPACE or _WORKSPACE[key].numel() < nbytes:
+        _WORKSPACE[key] = torch.empty(nbytes, dtype=torch.uint8, device=stream.device)
+    return _WORKSPACE[key].data_ptr()
 
 
 _LIBRARY = {}
