@@ -70,9 +70,8 @@ constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -3.40282347e38f;      // reference of a column without keys, where states are joined: below every other
 constexpr float kTop = 6.f, kLazy = 15.9f;      // log2 of a column's largest weight times value scale: where it is put, where it may drift
-constexpr int kUnitLow = -44, kUnitHigh = 35;  // log2 of the units of value scales
-constexpr float kHighFrom = 0x1p42f;           // the scale from which the high one is needed
-constexpr float kFloor = -82.f;                // log2 of the smallest scale, in units, that the reference follows
+constexpr int kUnitMost = 36;                  // log2 of the largest unit of value scales
+constexpr float kFloor = -82.f, kUnitRoom = 0x1p86f;   // log2 of the smallest scale in units that the reference follows; the largest scale
 constexpr int kAccRow = HD + 4;                // floats per column in LDS: rows on different banks
 static_assert(HD == 128 && kTilePages == 4 && G <= 16, "tile layout");
 
@@ -467,15 +466,33 @@ struct Pages {
     }
 };
 
-// 2^d, d <= 0, for a state moved to a reference -d higher: in halves for the sum of
-// weights, as these are 2^98 at most and the largest of a column 2^-80 at least, so
-// that a factor below fp32 may leave a sum that counts.  The sums of products
-// stand at one size and need no such care.
+// 2^d, d <= 0, for a state moved to a reference -d higher.  In halves where it may be
+// below fp32 and leave something that counts: for sums of weights, which are 2^98 at
+// most and may count at 2^-100, and for sums of products between waves, whose units differ.
 struct Factor {
-    float half, all;
-    __device__ __forceinline__ explicit Factor(float d) : half(__builtin_amdgcn_exp2f(0.5f * d)), all(half * half) {}
-    __device__ __forceinline__ float of_weights(float l) const { return l * half * half; }
+    float half;
+    __device__ __forceinline__ explicit Factor(float d) : half(__builtin_amdgcn_exp2f(0.5f * d)) {}
+    template <class T>
+    __device__ __forceinline__ T operator*(T v) const { return v * half * half; }
 };
+
+// joins pieces {reference, sum of weights}, v into the state m, l, o
+template <int N, class V>
+__device__ __forceinline__ void join(float& m, float& l, V& o, const f2 (&x)[N], const V (&v)[N]) {
+    float to = m;
+#pragma unroll
+    for (int k = 0; k < N; ++k) to = fmaxf(to, x[k][0]);
+    const Factor f(m - to);
+    l = f * l;
+    o = f * o;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const Factor f(x[k][0] - to);
+        l += f * x[k][1];
+        o += f * v[k];
+    }
+    m = to;
+}
 
 // A block's state over the keys seen so far: lane (g, c) holds the reference, its
 // share of the sum and dims 16 d + 4 g .. + 3 of column c.  Weights are 2^(s - m).
@@ -501,18 +518,20 @@ struct State {
     }
 };
 
-// V's scales in units, so that weights (from 2^(kTop - log2 vs) for the largest
-// product) stay inside fp32 with their tails: a unit serves scales of 2^-82 to 2^86 of
-// its own size.  The low one's are 2^-126 (the quantiser's smallest) to 2^42; a larger scale takes the
-// wave to the high one, 2^-47 to 2^121 (the largest).  There, beside values of
-// 2^49 and more, a column whose values are all below 2^-40 loses bits.
+// V's scales in units, so that weights (2^(kTop - log2 vs) for the largest product)
+// stay near 1, where a score less its reference is exact to 2^-22, and inside fp32 with
+// their tails.  The unit is a power of two: the size of the first tile's largest scale, 2^36 at
+// most.  It serves scales of 2^-82 to 2^86 of its own size; a larger one moves it (to
+// 2^36 at most).  So a column loses bits only where the products that count have scales
+// 2^82 times smaller than others of the session, hidden ones included, and below 2^-46.
 struct ValueUnit {
+    int ex;                    // log2 of the unit
     float inv;                 // 1 / unit
     float most, cap;           // no scale so far is larger; its log2 in units, or kFloor
-    __device__ __forceinline__ bool low() const { return inv > 1.f; }
-    __device__ __forceinline__ float unit() const { return low() ? ldexpf(1.f, kUnitLow) : ldexpf(1.f, kUnitHigh); }
+    __device__ __forceinline__ float unit() const { return ldexpf(1.f, ex); }
     __device__ __forceinline__ void clear() {
-        inv = ldexpf(1.f, -kUnitLow);
+        ex = 0;
+        inv = 1.f;
         most = 0.f;
         cap = kFloor;
     }
@@ -521,19 +540,24 @@ struct ValueUnit {
     __device__ __forceinline__ float take(float vs, State (&st)[NB]) {
         if (__builtin_amdgcn_ballot_w64(vs > most)) {        // rare
             const float top = wave_max(vs);                  // (a NaN does not count)
-            if (low() && top >= kHighFrom) {
+            if (most == 0.f || top * inv > kUnitRoom) {
+                int to;
+                (void)frexpf(top, &to);
+                to = min(to, kUnitMost);
                 // products keep their size: the reference goes down by as much as the
                 // unit goes up, as far as the weights' sum has room for, the sums for the rest
+                if (most > 0.f)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    int ex;
-                    (void)frexpf(rows_max(st[b].l), &ex);
-                    const int by = min(max(90 - ex, 0), kUnitHigh - kUnitLow);
-                    st[b].m -= (float)by;
-                    st[b].l = ldexpf(st[b].l, by);
-                    st[b].scale_acc(ldexpf(1.f, by - (kUnitHigh - kUnitLow)));
-                }
-                inv = ldexpf(1.f, -kUnitHigh);
+                    for (int b = 0; b < NB; ++b) {
+                        int e;
+                        (void)frexpf(rows_max(st[b].l), &e);
+                        const int by = min(max(90 - e, 0), to - ex);
+                        st[b].m -= (float)by;
+                        st[b].l = ldexpf(st[b].l, by);
+                        st[b].scale_acc(ldexpf(1.f, by - (to - ex)));
+                    }
+                ex = to;
+                inv = ldexpf(1.f, -to);
             }
             most = 1.125f * top;                             // (so that few tiles come here)
             cap = fmaxf(__builtin_amdgcn_logf(most * inv), kFloor);
@@ -589,7 +613,7 @@ __device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float k
         const Factor corr(first ? -INFINITY : -by);
         st.m += by;
         st.limit = moves ? kLazy - cap : st.limit;
-        st.l = corr.of_weights(st.l);
+        st.l = corr * st.l;
         each<16>([&](auto j) {
             // scores of 2^23 and more leave no room for log2 vs beside them: the product stays below
             // its bound all the same (and a NaN is left as it is)
@@ -597,7 +621,7 @@ __device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float k
             x[j] -= by;
             x[j] = x[j] > most ? most : x[j];
         });
-        st.scale_acc(corr.all);
+        st.scale_acc(corr.half * corr.half);                 // (in one unit: what this loses weighs nothing)
     }
     float e[2][8];
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -736,8 +760,8 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q8_few_kernel(Q8Args
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 const Factor f(s_m[w][col] - m);
-                sum += *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]) * f.all;
-                l += f.of_weights(s_l[w][col]);
+                sum += f * *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]);
+                l += f * s_l[w][col];
             }
             if (p.parts == 1) {
                 const int r = col / G, hh = col - r * G;
@@ -788,14 +812,7 @@ __global__ void __launch_bounds__(THREADS) q8_few_join_kernel(Q8Args a, int cols
                         v[k] = *reinterpret_cast<const f2*>(a.acc + at * HD + 2 * lane);
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float to = fmaxf(m, x[k][0]);
-                    const Factor f0(m - to), f1(x[k][0] - to);
-                    ll = f0.of_weights(ll) + f1.of_weights(x[k][1]);
-                    o = o * f0.all + v[k] * f1.all;
-                    m = to;
-                }
+                join(m, ll, o, x, v);
             }
             __syncthreads();                                 // the last column has been read
             s_o[wave][lane] = o;
@@ -813,8 +830,8 @@ __global__ void __launch_bounds__(THREADS) q8_few_join_kernel(Q8Args a, int cols
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 const Factor f(s_m[w] - m);
-                o += s_o[w][lane] * f.all;
-                ll += f.of_weights(s_l[w]);
+                o += f * s_o[w][lane];
+                ll += f * s_l[w];
             }
             const int r = col / G, hh = col - r * G;
             *reinterpret_cast<f2*>(a.o + ((int64_t)(row0 + r) * NH + kvh * G + hh) * HD + 2 * lane) = o * (1.0f / ll);
@@ -1089,13 +1106,6 @@ __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
             m = x[0];
             l = x[1];
         }
-        auto add = [&](const f2 x, const f4 p) {
-            const float to = fmaxf(m, x[0]);
-            const Factor f0(m - to), f1(x[0] - to);
-            l = f0.of_weights(l) + f1.of_weights(x[1]);
-            o = o * f0.all + p * f1.all;
-            m = to;
-        };
         for (int base = w + 1; base < a.gw; base += 64) {
             i4 next = i4{-1, 0, 0, 0};
             if (base + lane < a.gw) next = a.info[2 * (base + lane)];
@@ -1122,8 +1132,7 @@ __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
                         todo &= todo - 1;
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < kAtOnce; ++k) add(x[k], p[k]);
+                join(m, l, o, x, p);
             }
             if (__builtin_amdgcn_ballot_w64(ours && next[2])) break;         // the group's end
         }
@@ -1133,7 +1142,11 @@ __global__ void __launch_bounds__(THREADS) q8_many_join_kernel(Q8Args a) {
             if (d == 0) s_ml[row] = f2{m, l};
             __syncthreads();
             if (team) continue;
-            for (int t = 1; t < teams; ++t) add(s_ml[row + t], s_o[row + t][d]);
+            for (int t = 1; t < teams; ++t) {
+                const f2 x[1] = {s_ml[row + t]};
+                const f4 p[1] = {s_o[row + t][d]};
+                join(m, l, o, x, p);
+            }
         }
         const int col = group * COLS + cc;
         if (cc >= cols || col >= s.rows * G) continue;

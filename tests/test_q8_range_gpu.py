@@ -134,6 +134,24 @@ def test_one_value_near_the_end_of_fp32(rows, decode, key):
     c.check()
 
 
+@pytest.mark.parametrize("power", [-100, -60, 60])
+@pytest.mark.parametrize("past,rows,decode", [(899, 1, True), (896, 4, False), (830, 70, False)])
+def test_value_sizes_change_between_tiles(past, rows, decode, power):
+    """the first two tiles' values 2^power times the others'"""
+    c = Call([past], [rows], seed=8, decode=decode)
+    c.parts[3][c.table[0, :8]] *= np.float32(2.0 ** power)
+    c.check()
+
+
+@pytest.mark.parametrize("rows", [4, 70])
+def test_rows_that_see_small_values_only(rows):
+    """beside rows that see others 2^60 times as large in the same tile"""
+    c = Call([0], [rows], seed=9)
+    for key in range(rows // 2):
+        c.parts[3][c.at(0, key)] *= np.float32(2.0 ** -60)
+    c.check()
+
+
 @pytest.mark.parametrize("power", [-90, 100])
 @pytest.mark.parametrize("rows,decode", FORMS)
 def test_large_keys_and_small_queries(rows, decode, power):
