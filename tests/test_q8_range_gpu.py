@@ -181,3 +181,14 @@ def test_scores_of_any_size(rows, decode, keys, sign):
         want = np.repeat(v[0 if sign < 0 else c.past[0] + r], c.nova.group, 0)
         # weight times scale: two fp16 terms, 2^-21, and three fp32 operations
         assert (np.abs(got[r] - want) <= 2.0 ** -20 * np.abs(want)).all(), (r, got[r][0][:4], want[0][:4])
+
+
+@pytest.mark.parametrize("times", [30.0, 1e3, 1e6])
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_query_with_a_loud_channel(rows, decode, times):
+    """The query is held to 2^-24 of its largest component, also where K has only zeros
+    beside that one: the bound's term of max|q| sum|k|."""
+    c = Call([700], [rows], seed=7, decode=decode)
+    c.q[..., 77] *= np.float32(times)
+    c.parts[0][..., 77] = 0
+    c.check()
