@@ -614,13 +614,15 @@ __device__ __forceinline__ void weigh(K&& k_op, Q&& q_op, float q_scale, float k
         st.m += by;
         st.limit = moves ? kLazy - cap : st.limit;
         st.l = corr * st.l;
-        each<16>([&](auto j) {
-            // scores of 2^23 and more leave no room for log2 vs beside them: the product stays below
-            // its bound all the same (and a NaN is left as it is)
-            const float most = kLazy - row_lane<j>(r);
-            x[j] -= by;
-            x[j] = x[j] > most ? most : x[j];
-        });
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] -= by;
+        // scores of 2^23 and more leave no room for log2 vs beside them: the product stays
+        // below its bound all the same (and a NaN is left as it is)
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(by) < 0x1p20f)))
+            each<16>([&](auto j) {
+                const float most = kLazy - row_lane<j>(r);
+                x[j] = x[j] > most ? most : x[j];
+            });
         st.scale_acc(corr.half * corr.half);                 // (in one unit: what this loses weighs nothing)
     }
     float e[2][8];
