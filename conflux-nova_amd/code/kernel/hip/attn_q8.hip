@@ -7,21 +7,28 @@
 // Numbers.  The codes are exact operands: the query goes into three signed digits of
 // base 256 against K's int8 codes (products and sums are exact integers), and a
 // weight times V's scale into two fp16 terms against V's codes, which fp16 holds
-// exactly; sums are fp32.  So the result has fp32's accuracy: 1e-7 (a handful of
-// keys) to 6e-7 (tens of thousands) relative to 64 bits, where fp32 operations on
-// the decoded values have 2e-8 to 2e-6.  That
-// costs one and a half fp16 products for the scores and two for the output.
+// exactly; sums are fp32.  That costs one and a half fp16 products for the scores and
+// two for the output, and rounds in two places where fp32 operations would not:
+//   * the query to 2^-24 of its largest component.  A component far below that one
+//     loses bits which count only where K is exactly 0 beside the large one (a
+//     channel 1000 times the others: 3e-5); elsewhere the quantiser's half step, 2^-8
+//     of the row's largest |k|, under the large component outweighs them by far;
+//   * a weight times scale to 2^-30 of the row's largest one, so n keys that share a sum
+//     with one that outweighs each of them by far lose at most n 2^-30 of it.
+// With rows as projections give them the result is 7e-8 (a handful of keys) to 6.3e-7
+// (tens of thousands) from 64 bits, where fp32 operations on the decoded values are
+// 1e-7 to 2e-6.
 //
 // One pass over the keys with a running reference and sum of the softmax.  The
 // reference m of the weights 2^(s - m) follows the largest weight times V scale, lazily:
 // that product may drift from 2^kTop to 2^kLazy, which the two fp16 terms have room
-// for, so that almost no tile rescales its sums (kTop 2: 268 instead of 275 us for the
-// 8 x 512 tokens below, and 4 bits less for the small products).
+// for, so that almost no tile rescales its sums (kTop 2 instead of 6: 3% off the
+// 8 x 512 tokens below, and 4 bits off the small products).
 //
 // Two kernels, by the columns (query rows x heads of a kv head) that a session may
 // have.  Up to 32: the waves of a workgroup share them and split the keys; K and V
 // go from the pages to registers once and HBM bounds it.  8 x 32768 keys of the 14B
-// model, 554 MB: 90 us, 6.2 TB/s; 16 sessions of 512 to 8192 keys (7B), 66 MB: 21.7 us
+// model, 554 MB: 90 us, 6.2 TB/s; 16 sessions of 512 to 8192 keys (7B), 66 MB: 21.8 us
 // in two launches.  Above: 64 columns a workgroup, K and V through LDS, the
 // matrix instructions and the softmax's vector instructions bound it, of which a SIMD
 // overlaps a part only (a 16x16x32 product and 4 vector instructions take 16 and 16
@@ -58,7 +65,9 @@ constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
-constexpr int kAimWgs = 512;                   // workgroups aimed at: two per CU
+// Workgroups aimed at: two per CU.  (Of the form with two blocks of columns one runs per
+// CU, as it takes the registers of both, so its parts go through in two rounds.)
+constexpr int kAimWgs = 512;
 // Many columns, 12 prompts of up to 300 tokens (1.5B) / 8 x 512 tokens behind up to
 // 4096 (7B), us.  Fewest tiles of a piece of a group: 2 37.3 / 266, 3 36.0 / 266, 4 39.0 / 272.
 constexpr int kMinPiece = 3;
@@ -203,8 +212,8 @@ struct Part {
 
 // Few columns: the session and part of a slot.  With T tiles in the batch and gw
 // workgroups aimed at, a session of t tiles is cut into ceil(t / share) parts,
-// share = max(ceil(T / gw), min_share), so that no workgroup has more than a share
-// whatever the lengths, and at most gw + n_sess slots are used.  Every wave works it
+// share = max(ceil(T / gw), min_share) or up to half more, so that no workgroup has more
+// than that whatever the lengths, and at most gw + n_sess slots are used.  Every wave works it
 // out for itself, 64 sessions at a time.
 template <bool kCausal>
 __device__ __forceinline__ Part find_part(const Q8Args& a, int slot) {
@@ -414,7 +423,7 @@ __device__ __forceinline__ h8 codes_f16(uint32_t w0, uint32_t w1) {
     return __builtin_bit_cast(h8, r) + (_Float16)-1152.0f;
 }
 
-// weights e in fp16 terms hi + lo (hi cut off, lo the rest: 21 bits or more)
+// weights e in fp16 terms hi + lo (hi cut off, lo the rest: 21 bits, fewer below 2^-3, as lo ends at 2^-24)
 __device__ __forceinline__ void split_f16(const float (&e)[8], h8& hi, h8& lo) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
@@ -1163,7 +1172,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // Columns per session up to which a workgroup's waves share them.  At 17 to 32 columns
 // the other kernel is faster behind many long sessions (9 x 4400 keys, 4 rows, 7B: 29.5
-// instead of 35.3 us; 24 x 3000: 38.1, 44.5) and slower for few or short ones (1 x 30000: 57.3,
+// instead of 34.2 us; 24 x 3000: 38.1, 44.5) and slower for few or short ones (1 x 30000: 57.3,
 // 37.3; 16 x 600: 19.8, 17.5; 32 x 100: 14.0, 11.5); the host knows the columns, not the keys.
 constexpr int kFewCols = 32;
 // Tiles of a workgroup that shares a session: one per wave.  Many columns, 12 prompts

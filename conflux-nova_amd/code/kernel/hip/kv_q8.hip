@@ -21,9 +21,11 @@
 // the page stay as they are.
 //
 // All of it is movement, bound by HBM once the call is large and by the launch
-// before that.  8 x 512 tokens of the 7B model (33.6 MB read, 8.7 MB written) take
-// 13.5 us, 3.1 TB/s, where a large copy moves 5.2 TB/s; a decode step's 16 tokens 10 us, which
-// is the call and its launch.  64 page copies of the 7B model over all layers, 30 MB written
+// before that.  8 x 512 tokens of the 7B model, appended and read back (21.1 MB each),
+// take 13.5 us in two launches, 3.1 TB/s, where a large copy moves 5.2 TB/s; RoPE and
+// append of the same tokens (138 MB, the rotated queries most of it) 28 us, 4.9 TB/s.
+// A decode step's 16 tokens, appended and read back, take 10 us, which is the calls
+// and their launches.  64 page copies of the 7B model over all layers, 30 MB written
 // from 4 donors, take 8.6 us, 3.7 TB/s, with the launch; one of the 1.5B model 8.3.
 #include <hip/hip_runtime.h>
 #include <algorithm>

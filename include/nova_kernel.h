@@ -296,7 +296,8 @@ void launch_gemv_q4k_f32(const uint8_t* const* blocks, const int64_t* rows, floa
  * not decreasing, from 0 to at most n_rows), or n_rows / n_sess rows each where
  * row_off is NULL.  A session may have no rows.  Rows behind the last session's
  * are neither read nor written.  tables must hold n_sess rows of table_stride
- * entries; positions past table_stride * 16 are left out, a table entry outside
+ * entries; positions past table_stride * 16 are left out (of the RoPE append with
+ * their q), a session that starts below 0 is left out, a table entry outside
  * [0, nb) is not written through and reads page 0.  fp32 arrays and pools are
  * read 16 bytes at a time and must be 16-byte aligned. */
 size_t kv_q8_page_bytes(void);
@@ -322,7 +323,13 @@ void launch_kv_q8_load_batch(const uint8_t* pool, const int32_t* tables, int tab
                              nova_stream_t s);
 /* Decode attention: one query row per session over keys [0, n_keys[i]) (device
  * int32[n_sess]; the new token already appended).  q, o: [n_sess][NH][HD] fp32.
- * n_keys[i] == 0 gives a row of zeros.  workspace: from
+ * n_keys[i] == 0 gives a row of zeros.  Precision, here and in the chunk attention:
+ * fp32 over the values code * scale, but for two roundings.  A query is held to
+ * 2^-24 of its largest component, and the product of a key's weight and V
+ * scale to 2^-30 of the row's largest such product.  Scores have to be finite in
+ * fp32.  Keys that a row does not see do not enter it, whatever they hold, but for
+ * this: where a session's V scales differ by more than 2^82, rows that only see the
+ * small ones may lose bits.  workspace: from
  * attn_decode_q8_workspace_bytes(n_sess), 16-byte aligned, no initial contents;
  * calls that may overlap need one each. */
 size_t attn_decode_q8_workspace_bytes(int n_sess);
@@ -339,8 +346,8 @@ size_t attn_chunk_q8_workspace_bytes(int n_sess, int n_rows, int max_q);
 void launch_attn_chunk_q8_batch(const float* q, const uint8_t* pool, const int32_t* tables, int table_stride,
                                 const int32_t* n_past, const int32_t* row_off, int n_sess, int n_rows, int max_q,
                                 int layer, int nb, float* o, void* workspace, nova_stream_t s);
-/* launch_kv_cow_apply and launch_kv_zero_pages for 8-bit pages.  The copies of
- * one call run side by side: an op whose dst is another op's dst, or any op's
+/* launch_kv_cow_apply and launch_kv_zero_pages for 8-bit pages (page ids outside
+ * [0, nb) are not cleared).  The copies of one call run side by side: an op whose dst is another op's dst, or any op's
  * src, aborts the call. */
 void launch_kv_q8_cow_apply(uint8_t* pool, int nb, int32_t* tables_dev, const nova_cow_op* ops, int n_ops,
                             nova_stream_t s);
