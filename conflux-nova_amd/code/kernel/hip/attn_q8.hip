@@ -79,7 +79,7 @@ constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -3.40282347e38f;      // reference of a column without keys, where states are joined: below every other
 constexpr float kTop = 6.f, kLazy = 15.9f;      // log2 of a column's largest weight times value scale: where it is put, where it may drift
-constexpr int kUnitMost = 36;                  // log2 of the largest unit of value scales
+constexpr int kUnitLeast = -125, kUnitMost = 36;   // log2 of the units of value scales; 1 / unit is finite
 constexpr float kFloor = -82.f, kUnitRoom = 0x1p86f;   // log2 of the smallest scale in units that the reference follows; the largest scale
 constexpr int kAccRow = HD + 4;                // floats per column in LDS: rows on different banks
 static_assert(HD == 128 && kTilePages == 4 && G <= 16, "tile layout");
@@ -554,7 +554,7 @@ struct ValueUnit {
             if (most == 0.f || top * inv > kUnitRoom) {
                 int to;
                 (void)frexpf(top, &to);
-                to = min(to, kUnitMost);
+                to = min(max(to, kUnitLeast), kUnitMost);
                 // products keep their size: the reference goes down by as much as the
                 // unit goes up, as far as the weights' sum has room for, the sums for the rest
                 if (most > 0.f)

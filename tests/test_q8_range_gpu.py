@@ -134,6 +134,14 @@ def test_one_value_near_the_end_of_fp32(rows, decode, key):
     c.check()
 
 
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_subnormal_scales(rows, decode):
+    """the quantiser makes none, but a page may hold them"""
+    c = Call([700], [rows], seed=10, scale=0.01, decode=decode)
+    c.parts[3] *= np.float32(1e-38 / c.parts[3].max() / 127)
+    c.check()
+
+
 @pytest.mark.parametrize("power", [-100, -60, 60])
 @pytest.mark.parametrize("past,rows,decode", [(899, 1, True), (896, 4, False), (830, 70, False)])
 def test_value_sizes_change_between_tiles(past, rows, decode, power):
