@@ -1,0 +1,614 @@
+"""The operators of a serving step over 4-bit pages: inputs, plain forms, calls and exact results.
+
+Five kinds of case, in the order in which a step comes to them:
+
+* ``plan``    lengths of the step's sessions -> pages given back and handed out, block
+  tables, row offsets, positions and cache slots of every new row, all on the GPU.
+* ``rope``    the rows' angles from their positions (any base, scaled for long contexts),
+  then q and k turned: pairs half a head apart or side by side, the whole head or its
+  first dims.
+* ``store``   q turned; k turned and v, quantised as they are written into each session's
+  pages; the same rows read back (the values that the codes stand for).
+* ``decode``  one query token per session over all of its keys.
+* ``chunk``   a ragged chunk of new tokens per session (already in the cache) over its
+  prefix and itself, causally.
+
+The cache holds K and V in 4-bit floating point (0, .5, 1, 1.5, 2, 3, 4, 6 and their
+negatives; code 0..7, sign in bit 3) with a power of two per token, kv head and 32 dims,
+held as its exponent plus 127 in a byte.  A page (16 tokens of one layer) is a record of
+2176 bytes per kv head:
+
+    K of token t, dim d        byte t * 64 + (d >> 1), the low half for even d
+    V of token t, dim d        byte 1024 + (t >> 3) * 512 + (d & 15) * 32 + (d >> 5) * 8 + (t & 7),
+                               the low half where bit 4 of d is clear
+    K exponent of t, dims 32j..  byte 2048 + t * 4 + j
+    V exponent of t, dims 32j..  byte 2112 + t * 4 + j
+
+and the pool is [layer][page][kv head][2176].  The exponent is the smallest with which no
+value of the 32 passes 7 (so none is off by more than half its step), at most 2^125; values are
+rounded to the nearest, ties to the even code.
+
+Lengths are drawn with the case's own ``mix``, so every seed does the same amount
+of work; pages are scattered over the pool by a seeded shuffle.
+"""
+import math
+import sys
+from pathlib import Path
+
+import numpy as np
+import torch
+
+own = False
+
+KB = 16                      # tokens per page
+HD = 128
+REC = 2176                   # bytes per page and kv head
+K_EXP, V_CODE, V_EXP = 2048, 1024, 2112
+# query heads, kv heads
+MODELS = {"qwen25_1p5b": (12, 2), "qwen25_7b": (28, 4), "qwen25_14b": (40, 8)}
+LAYER, LAYERS = 1, 2         # the cases run on the second layer of two
+STEP = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def listed():
+    return [
+        # a decode step's bookkeeping: 16 sessions grow by one token each
+        dict(name="plan_step", kind="plan", sessions=16, have_lo=511, have_hi=8191, new_lo=1, new_hi=1, ended=0.0,
+             stride=520, mix=2024),
+        # a busy server: sessions end or are cut back while others bring prompts of unequal lengths
+        dict(name="plan_busy", kind="plan", sessions=700, have_lo=0, have_hi=4000, new_lo=0, new_hi=250, ended=0.3,
+             stride=300, mix=11),
+        # a decode step behind long documents, base scaled by parts
+        dict(name="rope_7b_step", kind="rope", model="qwen25_7b", rows=16, pos_hi=131071, rot=128, beside=False,
+             scaling="parts"),
+        # the rows of 8 chunks of 512, pairs side by side, the first half of the head
+        dict(name="rope_7b_chunk_partial", kind="rope", model="qwen25_7b", rows=4096, pos_hi=32767, rot=64, beside=True,
+             scaling="linear"),
+        # a decode step's appends: one token of each of 16 sessions
+        dict(name="store_7b_step", kind="store", model="qwen25_7b", sessions=16, q_lo=1, q_hi=1, past_lo=511,
+             past_hi=8191, rot=128, beside=False, mix=2024),
+        # the appends of the chunked prefill benchmark: 8 sessions x 512 tokens
+        dict(name="store_7b_chunk", kind="store", model="qwen25_7b", sessions=8, q_lo=512, q_hi=512, past_lo=0,
+             past_hi=4096, rot=128, beside=False, mix=2024),
+        # one user, the small model, a chat of 1025 tokens: latency and launches
+        dict(name="decode_1p5b_single", kind="decode", model="qwen25_1p5b", sessions=1, ctx_lo=1025, ctx_hi=1025, mix=1),
+        # the benchmark's own step: a ragged batch of 16 sessions
+        dict(name="decode_7b_ragged16", kind="decode", model="qwen25_7b", sessions=16, ctx_lo=512, ctx_hi=8192,
+             mix=2024),
+        # long documents on the large model
+        dict(name="decode_14b_long", kind="decode", model="qwen25_14b", sessions=8, ctx_lo=32768, ctx_hi=32768, mix=1),
+        # drafted tokens to be checked: 1 to 8 rows per session behind the same contexts
+        dict(name="chunk_7b_drafts", kind="chunk", model="qwen25_7b", sessions=16, q_lo=1, q_hi=8, past_lo=512,
+             past_hi=8192, mix=2024),
+        # prompts of unequal lengths on the small model, some of them follow-ups
+        dict(name="chunk_1p5b_mixed", kind="chunk", model="qwen25_1p5b", sessions=12, q_lo=1, q_hi=300, past_lo=0,
+             past_hi=700, mix=5),
+        # the benchmark's chunked prefill: 8 sessions x 512 tokens over ragged prefixes
+        dict(name="chunk_7b_batch", kind="chunk", model="qwen25_7b", sessions=8, q_lo=512, q_hi=512, past_lo=0,
+             past_hi=4096, mix=2024),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """A case of the same ranges: any model, sizes spread over their logarithm."""
+    kind = rng.choice(["plan"] * 2 + ["rope"] * 2 + ["store"] * 2 + ["decode"] * 4 + ["chunk"] * 4)
+    mix = rng.randrange(1 << 20)
+    if kind == "plan":
+        sessions = _log(rng, 1, 1024)
+        stride = _log(rng, 4, 520)
+        have = rng.randint(0, stride * KB - 1)
+        new = _log(rng, 1, 512)
+        while sessions * new > 1 << 17:
+            new //= 2
+        return dict(kind="plan", sessions=sessions, have_lo=rng.randint(0, have), have_hi=have,
+                    new_lo=rng.choice([0, 1, new]), new_hi=new, ended=rng.choice([0.0, 0.1, 0.5]), stride=stride, mix=mix)
+    model = rng.choice(sorted(MODELS))
+    nh, nkv = MODELS[model]
+    rot = rng.choice([128, 128, 64, 96, 2 * rng.randint(1, 64)])
+    beside = rng.random() < 0.5
+    if kind == "rope":
+        rows = _log(rng, 1, 4096 * 28 // nh)
+        return dict(kind="rope", model=model, rows=rows, pos_hi=_log(rng, 16, 1 << 20), rot=rot, beside=beside,
+                    scaling=rng.choice(["none", "linear", "base", "parts"]))
+    sessions = _log(rng, 1, 32)
+    if kind == "decode":
+        hi = _log(rng, 1, 32768)
+        lo = rng.randint(max(1, hi // 16), hi)
+        while sessions > 1 and sessions * hi * nkv > 8 * 32768 * 8:
+            sessions -= 1
+        return dict(kind="decode", model=model, sessions=sessions, ctx_lo=lo, ctx_hi=hi, mix=mix)
+    q_hi = _log(rng, 1, 1024)
+    q_lo = rng.choice([q_hi, rng.randint(1, q_hi), 1])
+    hi = _log(rng, 1, 16384)
+    lo = rng.choice([0, rng.randint(0, hi), hi])
+    if kind == "store":
+        q_hi = min(q_hi, 8 * 512 * 28 // nh)
+        while sessions > 1 and sessions * q_hi * nh > 8 * 512 * 28:
+            sessions -= 1
+        return dict(kind="store", model=model, sessions=sessions, q_lo=min(q_lo, q_hi), q_hi=q_hi, past_lo=lo, past_hi=hi,
+                    rot=rot, beside=beside, mix=mix)
+    while sessions > 1 and sessions * q_hi * nh * (hi + q_hi) > 2.2e8:
+        sessions -= 1
+    while q_hi > 1 and sessions * q_hi * nh * (hi + q_hi) > 2.2e8:
+        q_hi //= 2
+    return dict(kind="chunk", model=model, sessions=sessions, q_lo=min(q_lo, q_hi), q_hi=q_hi, past_lo=lo, past_hi=hi,
+                mix=mix)
+
+
+# ------------------------------------------------------------------ inputs
+
+class _State:
+    """What a serving program holds before the call."""
+
+
+def _lengths(n, lo, hi, mix):
+    return np.random.default_rng(mix).integers(lo, hi + 1, n).astype(np.int64)
+
+
+def _shape(case):
+    """(keys before the call, rows of the call) per session."""
+    n = case["sessions"]
+    if case["kind"] == "decode":
+        return _lengths(n, case["ctx_lo"], case["ctx_hi"], case["mix"]), np.ones(n, np.int64)
+    return (_lengths(n, case["past_lo"], case["past_hi"], case["mix"]),
+            _lengths(n, case["q_lo"], case["q_hi"], case["mix"] + 1))
+
+
+def _plan_shape(case):
+    """(tokens held, tokens kept, tokens to add) per session: a session that is cut back or ends adds none."""
+    n = case["sessions"]
+    have = _lengths(n, case["have_lo"], case["have_hi"], case["mix"])
+    rng = np.random.default_rng(case["mix"] + 2)
+    cut = rng.random(n) < case["ended"]
+    keep = np.where(cut, (have * rng.choice([0.0, 0.0, 0.9], n)).astype(np.int64), have)
+    new = np.where(cut, 0, _lengths(n, case["new_lo"], case["new_hi"], case["mix"] + 1))
+    return have, keep, new
+
+
+def _dev(array):
+    return torch.from_numpy(np.ascontiguousarray(array)).cuda()
+
+
+def _normal(g, shape, scale=1.0):
+    return torch.empty(shape, device="cuda").normal_(0.0, scale, generator=g)
+
+
+def _rows(g, shape):
+    """K rows as they come out of a projection: a few channels are several times the others, and tokens differ."""
+    gain = torch.ones(shape[-1], device="cuda")
+    gain[torch.randperm(shape[-1], generator=g, device="cuda")[:4]] = 5.0
+    tok = torch.exp(_normal(g, shape[:-1] + (1,), 0.25))
+    return _normal(g, shape) * gain * tok
+
+
+def _to_codes(x):
+    """(codes uint8, exponent bytes uint8 [..., 4]) of rows x [..., 128] fp32."""
+    y = x.unflatten(-1, (4, 32))
+    top = y.abs().amax(-1).contiguous()
+    byte = ((top.view(torch.int32) + 0x1fffff) >> 23) - 2
+    byte = torch.where(byte < 1, torch.zeros_like(byte), byte.clamp(max=252))
+    y = torch.ldexp(y.double(), (127 - byte)[..., None])
+    m = y.abs()
+    step = torch.where(m < 2, 0.5, torch.where(m < 4, 1.0, 2.0))
+    m = (torch.round(m / step) * step).clamp(max=6.0)
+    code = torch.where(m <= 2, 2 * m, torch.where(m < 3.5, 5.0, torch.where(m < 5, 6.0, 7.0))).to(torch.uint8)
+    code = torch.where(byte[..., None] > 0, code | (torch.signbit(y).to(torch.uint8) << 3), torch.zeros_like(code))
+    return code.flatten(-2), byte.to(torch.uint8)
+
+
+def _fill(pool, g):
+    """Random pages for one layer's records [nb][NKV][REC], as an append would have left them."""
+    nb, nkv, _ = pool.shape
+    code, byte = _to_codes(_rows(g, (nb, nkv, KB, HD)))
+    pool[..., :V_CODE] = (code[..., 0::2] | (code[..., 1::2] << 4)).reshape(nb, nkv, 1024)
+    pool[..., K_EXP:V_EXP] = byte.reshape(nb, nkv, 64)
+    code, byte = _to_codes(_normal(g, (nb, nkv, KB, HD)) * torch.exp(_normal(g, (nb, nkv, KB, 1), 0.25)))
+    code = code.view(nb, nkv, 2, 8, 4, 2, 16)                              # token halves, tokens, 32s, halves of them, dims
+    code = (code[..., 0, :] | (code[..., 1, :] << 4)).permute(0, 1, 2, 5, 4, 3)
+    pool[..., V_CODE:K_EXP] = code.reshape(nb, nkv, 1024)
+    pool[..., V_EXP:] = byte.reshape(nb, nkv, 64)
+
+
+def _freqs(rot, scaling):
+    """(turning rates of the pairs in fp32, factor on cos and sin), as a program makes them once from its configuration."""
+    base, factor, train = 1.0e6, 4.0, 32768
+    i = np.arange(0, rot, 2, dtype=np.float64)
+    f = base ** (-i / rot)
+    if scaling == "none":
+        return f.astype(np.float32), 1.0
+    if scaling == "linear":
+        return (f / factor).astype(np.float32), 1.0
+    if scaling == "base":
+        return ((base * factor ** (rot / max(rot - 2, 1))) ** (-i / rot)).astype(np.float32), 1.0
+    turns = train * f / (2 * math.pi)                                       # by parts: fast pairs stay, slow ones are stretched
+    keep = np.clip((turns - 1.0) / (32.0 - 1.0), 0, 1)
+    return (f * keep + f / factor * (1 - keep)).astype(np.float32), 0.1 * math.log(factor) + 1.0
+
+
+def prepare(case, seed):
+    s = _State()
+    s.case = case
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    if case["kind"] == "plan":
+        have, keep, new = _plan_shape(case)
+        s.n, s.stride = len(have), case["stride"]
+        s.max_rows = int(new.sum()) + 16                                    # rows of the step's buffers: some stay empty
+        held = (have + KB - 1) // KB
+        room = int(((keep + new + KB - 1) // KB).sum())
+        s.nb = int(held.sum()) + room + 8
+        perm = np.random.default_rng(seed).permutation(s.nb).astype(np.int32)
+        table = np.zeros((s.n, s.stride), np.int32)
+        off = 0
+        for i, p in enumerate(held):
+            table[i, :p] = perm[off:off + p]
+            off += p
+        free = np.zeros(s.nb, np.int32)
+        free[:s.nb - off] = perm[off:]
+        s.table, s.free = _dev(table), _dev(free)
+        s.n_free = _dev(np.array([s.nb - off], np.int32))
+        s.have, s.keep, s.new = (_dev(x.astype(np.int32)) for x in (have, keep, new))
+        s.past, s.keys = torch.empty_like(s.have), torch.empty_like(s.have)
+        s.row_off = torch.empty(s.n + 1, dtype=torch.int32, device="cuda")
+        s.pos = torch.empty(s.max_rows, dtype=torch.int32, device="cuda")
+        s.slots = torch.empty(s.max_rows, dtype=torch.int64, device="cuda")
+        s.free_left = torch.empty_like(s.n_free)
+        return s
+    nh, nkv = MODELS[case["model"]]
+    if case["kind"] == "rope":
+        s.n_rows = case["rows"]
+        freq, s.magnitude = _freqs(case["rot"], case["scaling"])
+        s.freq = _dev(freq)
+        s.pos = _dev(np.random.default_rng(seed).integers(0, case["pos_hi"] + 1, s.n_rows).astype(np.int32))
+        s.q, s.k = _normal(g, (s.n_rows, nh, HD), 1.5), _rows(g, (s.n_rows, nkv, HD))
+        s.q_out, s.k_out = torch.empty_like(s.q), torch.empty_like(s.k)
+        s.cs, s.sn = (torch.empty((s.n_rows, case["rot"] // 2), device="cuda") for _ in range(2))
+        return s
+    past, rows = _shape(case)
+    keys = past if case["kind"] == "decode" else past + rows
+    pages = (keys + KB - 1) // KB
+    s.nb, s.stride = int(pages.sum()) + 8, int(pages.max())
+    perm = np.random.default_rng(seed).permutation(s.nb).astype(np.int32)
+    table = np.zeros((len(pages), s.stride), np.int32)
+    off = 0
+    for i, p in enumerate(pages):
+        table[i, :p] = perm[off:off + p]
+        off += p
+    s.table = _dev(table)
+    s.n = len(pages)
+    s.n_rows, s.max_q = int(rows.sum()), int(rows.max())
+    s.past = _dev(past.astype(np.int32))                    # decode: the keys of each session
+    s.row_off = _dev(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+    s.pool = torch.zeros((LAYERS, s.nb, nkv, REC), dtype=torch.uint8, device="cuda")
+    if case["kind"] == "store":
+        s.q = _normal(g, (s.n_rows, nh, HD), 1.5)
+        s.k, s.v = _rows(g, (s.n_rows, nkv, HD)), _normal(g, (s.n_rows, nkv, HD))
+        s.q_out, s.k_out, s.v_out = torch.empty_like(s.q), torch.empty_like(s.k), torch.empty_like(s.v)
+        # the step's angles are there already: every layer uses the same
+        freq, _ = _freqs(case["rot"], "none")
+        pos = np.concatenate([p + np.arange(r) for p, r in zip(past, rows)])
+        angle = _dev(pos.astype(np.float64))[:, None] * _dev(freq.astype(np.float64))
+        s.cs, s.sn = torch.cos(angle).float(), torch.sin(angle).float()
+    else:
+        _fill(s.pool[LAYER], g)
+        # post-RoPE queries are not unit scale: scores spread over several units
+        s.q = _normal(g, (s.n_rows, nh, HD), 1.5)
+        s.o = torch.empty_like(s.q)
+    return s
+
+
+# ------------------------------------------------------------------ passes
+
+def run(s):
+    if own:
+        return _own(s)
+    return {"plan": _plain_plan, "rope": _plain_rope, "store": _plain_store, "decode": _plain_attention,
+            "chunk": _plain_attention}[s.case["kind"]](s)
+
+
+_WORKSPACE = {}
+
+
+def _workspace(nbytes):
+    """One workspace for the calls of each stream, as long as it is large enough: calls on two streams may overlap.
+    A larger one takes its place in the stream's own order (it is allocated on that stream)."""
+    stream = torch.cuda.current_stream()
+    key = stream.device_index, stream.cuda_stream
+    if key not in _WORKSPACE or _WORKSPACE[key].numel() < nbytes:
+        _WORKSPACE[key] = torch.empty(nbytes, dtype=torch.uint8, device=stream.device)
+    return _WORKSPACE[key].data_ptr()
+
+
+_LIBRARY = {}
+
+
+def _library(model):
+    """A model's library, loaded once per program."""
+    if model not in _LIBRARY:
+        path = str(Path(__file__).resolve().parent.parent / "conflux-nova_amd")
+        if path not in sys.path:
+            sys.path.insert(0, path)
+        import nova_amd
+        _LIBRARY[model] = nova_amd.load(model)
+    return _LIBRARY[model]
+
+
+def _own(s):
+    case, kind = s.case, s.case["kind"]
+    nova = _library(case.get("model", "qwen25_7b"))
+    st = torch.cuda.current_stream().cuda_stream
+    if kind == "plan":
+        ws = _workspace(nova.kv_step_plan_workspace_bytes(s.n))
+        nova.launch_kv_step_plan(s.table.data_ptr(), s.stride, s.have.data_ptr(), s.keep.data_ptr(), s.new.data_ptr(), s.n,
+                                 s.max_rows, s.free.data_ptr(), s.n_free.data_ptr(), s.nb, s.past.data_ptr(),
+                                 s.keys.data_ptr(), s.row_off.data_ptr(), s.pos.data_ptr(), s.slots.data_ptr(),
+                                 s.free_left.data_ptr(), ws, st)
+        return _plan_outputs(s)
+    if kind == "rope":
+        nova.launch_rope_angles(s.pos.data_ptr(), s.n_rows, s.freq.data_ptr(), case["rot"], s.magnitude, s.cs.data_ptr(),
+                                s.sn.data_ptr(), st)
+        nova.launch_rope_rows(s.q.data_ptr(), s.k.data_ptr(), s.pos.data_ptr(), s.cs.data_ptr(), s.sn.data_ptr(), s.n_rows,
+                              case["rot"], int(case["beside"]), s.q_out.data_ptr(), s.k_out.data_ptr(), st)
+        return s.q_out, s.k_out
+    pool, table, past, off = s.pool.data_ptr(), s.table.data_ptr(), s.past.data_ptr(), s.row_off.data_ptr()
+    if kind == "store":
+        nova.launch_rope_rows_kv_q4_store_batch(s.q.data_ptr(), s.k.data_ptr(), s.v.data_ptr(), s.cs.data_ptr(),
+                                                s.sn.data_ptr(), case["rot"], int(case["beside"]), pool, table, s.stride,
+                                                past, off, s.n, s.n_rows, LAYER, s.nb, s.q_out.data_ptr(), st)
+        nova.launch_kv_q4_load_batch(pool, table, s.stride, past, off, s.n, s.n_rows, LAYER, s.nb, s.k_out.data_ptr(),
+                                     s.v_out.data_ptr(), st)
+        return s.q_out, s.k_out, s.v_out
+    if kind == "decode":
+        ws = _workspace(nova.attn_decode_q4_workspace_bytes(s.n))
+        nova.launch_attn_decode_q4_batch(s.q.data_ptr(), pool, table, s.stride, past, s.n, LAYER, s.nb, s.o.data_ptr(),
+                                         ws, st)
+    else:
+        ws = _workspace(nova.attn_chunk_q4_workspace_bytes(s.n, s.n_rows, s.max_q))
+        nova.launch_attn_chunk_q4_batch(s.q.data_ptr(), pool, table, s.stride, past, off, s.n, s.n_rows, s.max_q, LAYER,
+                                        s.nb, s.o.data_ptr(), ws, st)
+    return s.o
+
+
+def _plan_outputs(s):
+    return {"tables": s.table, "free": s.free, "n_free": s.free_left, "n_past": s.past, "n_keys": s.keys,
+            "row_off": s.row_off, "pos": s.pos, "slots": s.slots}
+
+
+def _plain_plan(s):
+    have, keep, new = s.have.long(), s.keep.long(), s.new.long()
+    first, held = (keep + KB - 1) // KB, (have + KB - 1) // KB
+    back = held - first
+    avail = s.n_free.long() + back.sum()
+    add = torch.where(keep + new > s.stride * KB, 0, new)
+    more = (keep + add + KB - 1) // KB - first
+    fits = (add.cumsum(0) <= s.max_rows) & (more.cumsum(0) <= avail)
+    add, more = torch.where(fits, add, 0), torch.where(fits, more, 0)
+    # pages given back lie on top of the free ones, the first on top of all; pages are taken from the top
+    page = torch.arange(s.stride, device="cuda")[None, :]
+    nth = page - first[:, None]
+    spare = s.nb                                                           # (a place that is thrown away)
+    at = avail - 1 - ((back.cumsum(0) - back)[:, None] + nth)
+    at = torch.where((nth >= 0) & (page < held[:, None]), at, spare)
+    free = torch.cat([s.free, s.free.new_zeros(1)]).scatter_(0, at.reshape(-1), s.table.reshape(-1))
+    at = avail - 1 - ((more.cumsum(0) - more)[:, None] + nth)
+    taken = (nth >= 0) & (nth < more[:, None])
+    s.table.copy_(torch.where(taken, free[torch.where(taken, at, spare)], s.table))
+    s.free.copy_(free[:-1])
+    s.free_left.copy_(avail - more.sum())
+    s.past.copy_(keep)
+    s.keys.copy_(keep + add)
+    s.row_off[0] = 0
+    s.row_off[1:] = add.cumsum(0)
+    row = torch.arange(s.max_rows, device="cuda")
+    sess = torch.searchsorted(s.row_off[1:].long(), row, right=True).clamp(max=s.n - 1)
+    pos = keep[sess] + row - s.row_off.long()[sess]
+    real = row < s.row_off[-1]
+    slot = s.table[sess, torch.where(real, pos // KB, 0)].long() * KB + pos % KB
+    s.pos.copy_(torch.where(real, pos, -1))
+    s.slots.copy_(torch.where(real, slot, -1))
+    return _plan_outputs(s)
+
+
+def _turn(x, c, d, rot, beside):
+    """x [rows][heads][128] turned by the rows' cos and sin [rows][rot / 2]; dims from rot on stay."""
+    c, d = c[:, None, :], d[:, None, :]
+    y = x.clone()
+    a, b = (slice(0, rot, 2), slice(1, rot, 2)) if beside else (slice(0, rot // 2), slice(rot // 2, rot))
+    y[..., a] = x[..., a] * c - x[..., b] * d
+    y[..., b] = x[..., a] * d + x[..., b] * c
+    return y
+
+
+def _plain_rope(s):
+    angle = s.pos.double()[:, None] * s.freq.double()
+    c, d = (torch.cos(angle) * s.magnitude).float(), (torch.sin(angle) * s.magnitude).float()
+    return tuple(_turn(x, c, d, s.case["rot"], s.case["beside"]) for x in (s.q, s.k))
+
+
+def _row_places(s):
+    """(page, slot) of every row of the call."""
+    row = torch.arange(s.n_rows, device="cuda")
+    sess = torch.searchsorted(s.row_off[1:].long(), row, right=True)
+    pos = s.past.long()[sess] + row - s.row_off.long()[sess]
+    return s.table[sess, pos // KB].long(), pos % KB
+
+
+def _values(code):
+    """What 4-bit codes stand for, before their power of two."""
+    steps = torch.tensor(STEP + tuple(-v for v in STEP), device="cuda")
+    return steps[code.long()]
+
+
+def _powers(byte):
+    """2^(byte - 127); 0 where there is none."""
+    return torch.where(byte > 0, torch.ldexp(torch.ones((), device="cuda"), byte.int() - 127), 0.0)
+
+
+def _plain_store(s):
+    layer = s.pool[LAYER]
+    page, slot = _row_places(s)
+    nkv = layer.shape[1]
+    q, k = (_turn(x, s.cs, s.sn, s.case["rot"], s.case["beside"]) for x in (s.q, s.k))
+    page, head = page[:, None, None], torch.arange(nkv, device="cuda")[None, :, None]
+    b, j = torch.arange(64, device="cuda"), torch.arange(4, device="cuda")
+    low, high = torch.arange(0, HD, 2, device="cuda"), torch.arange(1, HD, 2, device="cuda")
+    k_at = slot[:, None] * 64 + b
+    # V: byte (32s j, dim r of 16) holds dims 32 j + r and 32 j + 16 + r
+    v_low = (b // 16) * 32 + b % 16
+    v_at = V_CODE + (slot[:, None] >> 3) * 512 + (b % 16) * 32 + (b // 16) * 8 + (slot[:, None] & 7)
+    out = [q]
+    for x, at, exp_at, lo, hi in ((k, k_at, K_EXP, low, high), (s.v, v_at, V_EXP, v_low, v_low + 16)):
+        code, byte = _to_codes(x)
+        layer[page, head, at[:, None, :]] = code[..., lo] | (code[..., hi] << 4)
+        four = exp_at + 4 * slot[:, None] + j
+        layer[page, head, four[:, None, :]] = byte
+        # read back from the pages
+        got = layer[page, head, at[:, None, :]]
+        y = torch.empty_like(x)
+        y[..., lo], y[..., hi] = _values(got & 15), _values(got >> 4)
+        out.append(y * _powers(layer[page, head, four[:, None, :]]).repeat_interleave(32, -1))
+    return tuple(out)
+
+
+def _plain_attention(s):
+    nh, nkv = MODELS[s.case["model"]]
+    group = nh // nkv
+    n, t = s.n, s.stride * KB
+    rec = s.pool[LAYER][s.table.long()].transpose(1, 2)                    # [n][NKV][pages][REC]
+    k = rec[..., :V_CODE]
+    k = torch.stack([_values(k & 15), _values(k >> 4)], -1).reshape(n, nkv, t, HD)
+    k *= _powers(rec[..., K_EXP:V_EXP]).reshape(n, nkv, t, 4).repeat_interleave(32, -1)
+    v = rec[..., V_CODE:K_EXP].unflatten(-1, (2, 16, 4, 8))                # token halves, dims, 32s, tokens
+    v = torch.stack([_values(v & 15), _values(v >> 4)], -1)
+    v = v.permute(0, 1, 2, 3, 6, 5, 7, 4).reshape(n, nkv, t, HD)
+    v = v * _powers(rec[..., V_EXP:]).reshape(n, nkv, t, 4).repeat_interleave(32, -1)
+    # the rows of each session, padded to the longest chunk
+    row = torch.arange(s.n_rows, device="cuda")
+    sess = torch.searchsorted(s.row_off[1:].long(), row, right=True)
+    at = row - s.row_off.long()[sess]
+    q = torch.zeros((n, s.max_q, nh, HD), device="cuda")
+    q[sess, at] = s.q
+    q = q.view(n, s.max_q, nkv, group, HD).transpose(1, 2).reshape(n, nkv, s.max_q * group, HD)
+    score = torch.matmul(q, k.transpose(2, 3).contiguous()) * (1.0 / math.sqrt(HD))
+    seen = s.past.long()[:, None] + (torch.arange(s.max_q, device="cuda") + 1 if s.case["kind"] == "chunk" else 0)
+    seen = seen.expand(n, s.max_q)
+    hidden = torch.arange(t, device="cuda") >= seen[:, :, None]            # [n][max_q][t]
+    score = score.view(n, nkv, s.max_q, group, t).masked_fill_(hidden[:, None, :, None, :], -math.inf)
+    score -= score.amax(-1, keepdim=True)
+    score.exp_()
+    score /= score.sum(-1, keepdim=True)
+    o = torch.matmul(score.view(n, nkv, s.max_q * group, t), v)
+    o = o.view(n, nkv, s.max_q, group, HD).transpose(1, 2).reshape(n, s.max_q, nh, HD)
+    return o[sess, at]
+
+
+# ------------------------------------------------------------------ work and exact results
+
+def work(case):
+    if case["kind"] == "plan":
+        have, keep, new = _plan_shape(case)
+        n, rows = len(have), int(new.sum())
+        back = int(((have + KB - 1) // KB - (keep + KB - 1) // KB).sum())
+        more = int(((keep + new + KB - 1) // KB - (keep + KB - 1) // KB).sum())
+        # lengths in, lengths and offsets out, a page id moved in or out, position and slot of each row
+        return {"bytes": 4 * 3 * n + 4 * 3 * n + 8 * (back + more) + 12 * (rows + 16), "flops": 0}
+    nh, nkv = MODELS[case["model"]]
+    if case["kind"] == "rope":
+        rows, half = case["rows"], case["rot"] // 2
+        return {"bytes": rows * (2 * (nh + nkv) * HD * 4 + 4) + 4 * half, "flops": 6.0 * rows * (nh + nkv) * half}
+    past, rows = _shape(case)
+    n_rows = int(rows.sum())
+    if case["kind"] == "store":
+        # q, k, v and the angles in; q, codes and exponents out, the values out again
+        row = 2 * nh * HD * 4 + 2 * nkv * HD * 4 + 2 * nkv * 2 * (HD // 2 + 4) + 2 * nkv * HD * 4 + case["rot"] * 4
+        return {"bytes": n_rows * row, "flops": 0}
+    if case["kind"] == "decode":
+        keys, pairs = int(past.sum()), int(past.sum())
+    else:
+        keys = int((past + rows).sum())
+        pairs = int((rows * past + rows * (rows + 1) // 2).sum())
+    return {"bytes": keys * nkv * 2 * (HD // 2 + 4) + 2 * n_rows * nh * HD * 4, "flops": 4.0 * HD * nh * pairs}
+
+
+def _exact_turn(x, cos, sin, rot, beside, rounded):
+    """x turned pair by pair in 64 bits; `rounded`: products and sums as the operator's fp32 has them."""
+    fp = (lambda z: z.to(torch.float32).to(torch.float64)) if rounded else (lambda z: z)
+    y = x.to(torch.float64)
+    out = y.clone()
+    for i in range(rot // 2):
+        a, b = (2 * i, 2 * i + 1) if beside else (i, i + rot // 2)
+        c, d = cos[:, i, None], sin[:, i, None]
+        out[:, :, a] = fp(fp(y[:, :, a] * c) - fp(y[:, :, b] * d))
+        out[:, :, b] = fp(fp(y[:, :, a] * d) + fp(y[:, :, b] * c))
+    return out
+
+
+def _exact_codes(x):
+    """The values that rows x (64 bits) are held as: the nearest of the format's own, ties to the even code."""
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device="cuda")
+    middle = (grid[1:] + grid[:-1]) / 2
+    odd = torch.arange(8, device="cuda") % 2
+    out = torch.zeros_like(x)
+    for j in range(0, HD, 32):
+        part = x[:, :, j:j + 32]
+        top = part.abs().max(dim=2, keepdim=True).values
+        unit = torch.exp2(torch.ceil(torch.log2(top.clamp(min=1e-300) / 7)))
+        unit = torch.where(top > 7 * unit, 2 * unit, torch.where(top <= 3.5 * unit, unit / 2, unit))   # (the logarithm's last bit)
+        m = part.abs() / unit
+        up = torch.searchsorted(middle, m.contiguous(), right=True)         # a tie goes up here,
+        down = torch.searchsorted(middle, m.contiguous(), right=False)      # down here
+        code = torch.where(odd[up] == 0, up, down)
+        out[:, :, j:j + 32] = torch.where(unit >= 2.0 ** -126, grid[code] * unit * torch.sign(part), 0.0)
+    return out
+
+
+def exact(case, seed):
+    """From the definitions, in 64 bits, byte by byte through the page format."""
+    if case["kind"] == "plan":
+        return None
+    s = prepare(case, seed)
+    if case["kind"] == "rope":
+        turn = s.pos.to(torch.float64)[:, None] * s.freq.to(torch.float64)[None, :]
+        c, d = torch.cos(turn) * s.magnitude, torch.sin(turn) * s.magnitude
+        return tuple(_exact_turn(x, c, d, case["rot"], case["beside"], False) for x in (s.q, s.k))
+    if case["kind"] == "store":
+        c, d = s.cs.double(), s.sn.double()
+        q = _exact_turn(s.q, c, d, case["rot"], case["beside"], False)
+        k = _exact_turn(s.k, c, d, case["rot"], case["beside"], True)
+        return q, _exact_codes(k), _exact_codes(s.v.double())
+    nh, nkv = MODELS[case["model"]]
+    group = nh // nkv
+    past, rows = _shape(case)
+    d = torch.arange(HD, device="cuda")
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device="cuda")
+    o = torch.zeros((s.n_rows, nh, HD), dtype=torch.float64, device="cuda")
+    flat = s.pool[LAYER].reshape(-1)
+
+    def decoded(byte, high, exponent):
+        code = torch.where(high, byte >> 4, byte & 15).long()
+        value = grid[code & 7] * torch.where(code > 7, -1.0, 1.0)
+        return value * torch.where(exponent > 0, torch.exp2(exponent.double() - 127), 0.0)
+
+    first = 0
+    for i in range(s.n):
+        n_q = int(rows[i])
+        n_keys = int(past[i]) + (n_q if case["kind"] == "chunk" else 0)
+        tok = torch.arange(n_keys, device="cuda")
+        page, slot = s.table[i].long()[tok // KB], (tok % KB)[:, None]
+        for h in range(nkv):
+            base = ((page * nkv + h) * REC)[:, None]
+            k = decoded(flat[base + slot * 64 + d // 2], (d % 2 == 1)[None, :], flat[base + 2048 + 4 * slot + d // 32])
+            v_at = 1024 + (slot // 8) * 512 + (d % 16) * 32 + (d // 32) * 8 + slot % 8
+            v = decoded(flat[base + v_at], (d // 16 % 2 == 1)[None, :], flat[base + 2112 + 4 * slot + d // 32])
+            q = s.q[first:first + n_q, h * group:(h + 1) * group].reshape(n_q * group, HD).double()
+            score = (q @ k.T) / math.sqrt(HD)
+            if case["kind"] == "chunk":
+                limit = past[i] + torch.arange(n_q, device="cuda").repeat_interleave(group)
+                score[tok[None, :] > limit[:, None]] = -math.inf
+            p = torch.softmax(score, dim=1)
+            o[first:first + n_q, h * group:(h + 1) * group] = (p @ v).view(n_q, group, HD)
+        first += n_q
+    return o
