@@ -19,10 +19,9 @@ held as its exponent plus 127 in a byte.  A page (16 tokens of one layer) is a r
 2176 bytes per kv head:
 
     K of token t, dim d        byte t * 64 + (d >> 1), the low half for even d
-    V of token t, dim d        byte 1024 + (t >> 3) * 512 + (d & 15) * 32 + (d >> 5) * 8 + (t & 7),
-                               the low half where bit 4 of d is clear
-    K exponent of t, dims 32j..  byte 2048 + t * 4 + j
-    V exponent of t, dims 32j..  byte 2112 + t * 4 + j
+    V of token t, dim d        byte 1024 + (d >> 5) * 256 + (d & 15) * 16 + t, the low half where bit 4 of d is clear
+    K exponent of t, dims 32j..  byte 2048 + (t & 3) * 16 + j * 4 + (t >> 2)
+    V exponent of t, dims 32j..  byte 2112 + j * 16 + t
 
 and the pool is [layer][page][kv head][2176].  The exponent is the smallest with which no
 value of the 32 passes 7 (so none is off by more than half its step), at most 2^125; values are
@@ -205,12 +204,12 @@ def _fill(pool, g):
     nb, nkv, _ = pool.shape
     code, byte = _to_codes(_rows(g, (nb, nkv, KB, HD)))
     pool[..., :V_CODE] = (code[..., 0::2] | (code[..., 1::2] << 4)).reshape(nb, nkv, 1024)
-    pool[..., K_EXP:V_EXP] = byte.reshape(nb, nkv, 64)
+    pool[..., K_EXP:V_EXP] = byte.view(nb, nkv, 4, 4, 4).permute(0, 1, 3, 4, 2).reshape(nb, nkv, 64)
     code, byte = _to_codes(_normal(g, (nb, nkv, KB, HD)) * torch.exp(_normal(g, (nb, nkv, KB, 1), 0.25)))
-    code = code.view(nb, nkv, 2, 8, 4, 2, 16)                              # token halves, tokens, 32s, halves of them, dims
-    code = (code[..., 0, :] | (code[..., 1, :] << 4)).permute(0, 1, 2, 5, 4, 3)
+    code = code.view(nb, nkv, KB, 4, 2, 16)                                # tokens, 32s, halves of them, dims
+    code = (code[..., 0, :] | (code[..., 1, :] << 4)).permute(0, 1, 3, 4, 2)
     pool[..., V_CODE:K_EXP] = code.reshape(nb, nkv, 1024)
-    pool[..., V_EXP:] = byte.reshape(nb, nkv, 64)
+    pool[..., V_EXP:] = byte.transpose(2, 3).reshape(nb, nkv, 64)
 
 
 def _freqs(rot, scaling):
@@ -456,14 +455,15 @@ def _plain_store(s):
     b, j = torch.arange(64, device="cuda"), torch.arange(4, device="cuda")
     low, high = torch.arange(0, HD, 2, device="cuda"), torch.arange(1, HD, 2, device="cuda")
     k_at = slot[:, None] * 64 + b
-    # V: byte (32s j, dim r of 16) holds dims 32 j + r and 32 j + 16 + r
+    # V: byte 16 j + r of a token holds dims 32 j + r and 32 j + 16 + r
     v_low = (b // 16) * 32 + b % 16
-    v_at = V_CODE + (slot[:, None] >> 3) * 512 + (b % 16) * 32 + (b // 16) * 8 + (slot[:, None] & 7)
+    v_at = V_CODE + b * 16 + slot[:, None]
+    k_exp = K_EXP + (slot[:, None] & 3) * 16 + j * 4 + (slot[:, None] >> 2)
+    v_exp = V_EXP + j * 16 + slot[:, None]
     out = [q]
-    for x, at, exp_at, lo, hi in ((k, k_at, K_EXP, low, high), (s.v, v_at, V_EXP, v_low, v_low + 16)):
+    for x, at, four, lo, hi in ((k, k_at, k_exp, low, high), (s.v, v_at, v_exp, v_low, v_low + 16)):
         code, byte = _to_codes(x)
         layer[page, head, at[:, None, :]] = code[..., lo] | (code[..., hi] << 4)
-        four = exp_at + 4 * slot[:, None] + j
         layer[page, head, four[:, None, :]] = byte
         # read back from the pages
         got = layer[page, head, at[:, None, :]]
@@ -480,11 +480,12 @@ def _plain_attention(s):
     rec = s.pool[LAYER][s.table.long()].transpose(1, 2)                    # [n][NKV][pages][REC]
     k = rec[..., :V_CODE]
     k = torch.stack([_values(k & 15), _values(k >> 4)], -1).reshape(n, nkv, t, HD)
-    k *= _powers(rec[..., K_EXP:V_EXP]).reshape(n, nkv, t, 4).repeat_interleave(32, -1)
-    v = rec[..., V_CODE:K_EXP].unflatten(-1, (2, 16, 4, 8))                # token halves, dims, 32s, tokens
+    k *= _powers(rec[..., K_EXP:V_EXP].unflatten(-1, (4, 4, 4))).permute(0, 1, 2, 5, 3, 4).reshape(
+        n, nkv, t, 4).repeat_interleave(32, -1)
+    v = rec[..., V_CODE:K_EXP].unflatten(-1, (4, 16, KB))                  # 32s, dims, tokens
     v = torch.stack([_values(v & 15), _values(v >> 4)], -1)
-    v = v.permute(0, 1, 2, 3, 6, 5, 7, 4).reshape(n, nkv, t, HD)
-    v = v * _powers(rec[..., V_EXP:]).reshape(n, nkv, t, 4).repeat_interleave(32, -1)
+    v = v.permute(0, 1, 2, 5, 3, 6, 4).reshape(n, nkv, t, HD)
+    v = v * _powers(rec[..., V_EXP:].unflatten(-1, (4, KB))).transpose(-1, -2).reshape(n, nkv, t, 4).repeat_interleave(32, -1)
     # the rows of each session, padded to the longest chunk
     row = torch.arange(s.n_rows, device="cuda")
     sess = torch.searchsorted(s.row_off[1:].long(), row, right=True)
@@ -600,9 +601,10 @@ def exact(case, seed):
         page, slot = s.table[i].long()[tok // KB], (tok % KB)[:, None]
         for h in range(nkv):
             base = ((page * nkv + h) * REC)[:, None]
-            k = decoded(flat[base + slot * 64 + d // 2], (d % 2 == 1)[None, :], flat[base + 2048 + 4 * slot + d // 32])
-            v_at = 1024 + (slot // 8) * 512 + (d % 16) * 32 + (d // 32) * 8 + slot % 8
-            v = decoded(flat[base + v_at], (d // 16 % 2 == 1)[None, :], flat[base + 2112 + 4 * slot + d // 32])
+            k = decoded(flat[base + slot * 64 + d // 2], (d % 2 == 1)[None, :],
+                        flat[base + 2048 + 16 * (slot % 4) + 4 * (d // 32) + slot // 4])
+            v = decoded(flat[base + 1024 + 256 * (d // 32) + 16 * (d % 16) + slot], (d // 16 % 2 == 1)[None, :],
+                        flat[base + 2112 + 16 * (d // 32) + slot])
             q = s.q[first:first + n_q, h * group:(h + 1) * group].reshape(n_q * group, HD).double()
             score = (q @ k.T) / math.sqrt(HD)
             if case["kind"] == "chunk":
