@@ -23,9 +23,9 @@ held as its exponent plus 127 in a byte.  A page (16 tokens of one layer) is a r
     K exponent of t, dims 32j..  byte 2048 + (t & 3) * 16 + j * 4 + (t >> 2)
     V exponent of t, dims 32j..  byte 2112 + j * 16 + t
 
-and the pool is [layer][page][kv head][2176].  The exponent is the smallest with which no
-value of the 32 passes 7 (so none is off by more than half its step), at most 2^125; values are
-rounded to the nearest, ties to the even code.
+and the pool is [layer][page][kv head][2176].  The power is the smallest with which no
+value of the 32 passes 7 (so none is off by more than half its step), at most 2^96, and all 32 are
+zeros where it would be below 2^-100; values are rounded to the nearest, ties to the even code.
 
 Lengths are drawn with the case's own ``mix``, so every seed does the same amount
 of work; pages are scattered over the pool by a seeded shuffle.
@@ -189,7 +189,7 @@ def _to_codes(x):
     y = x.unflatten(-1, (4, 32))
     top = y.abs().amax(-1).contiguous()
     byte = ((top.view(torch.int32) + 0x1fffff) >> 23) - 2
-    byte = torch.where(byte < 1, torch.zeros_like(byte), byte.clamp(max=252))
+    byte = torch.where(byte < 27, torch.zeros_like(byte), byte.clamp(max=223))
     y = torch.ldexp(y.double(), (127 - byte)[..., None])
     m = y.abs()
     step = torch.where(m < 2, 0.5, torch.where(m < 4, 1.0, 2.0))
@@ -562,7 +562,7 @@ def _exact_codes(x):
         up = torch.searchsorted(middle, m.contiguous(), right=True)         # a tie goes up here,
         down = torch.searchsorted(middle, m.contiguous(), right=False)      # down here
         code = torch.where(odd[up] == 0, up, down)
-        out[:, :, j:j + 32] = torch.where(unit >= 2.0 ** -126, grid[code] * unit * torch.sign(part), 0.0)
+        out[:, :, j:j + 32] = torch.where(unit >= 2.0 ** -100, grid[code] * unit * torch.sign(part), 0.0)
     return out
 
 
