@@ -21,6 +21,7 @@
 #pragma once
 #include <cstdint>
 
+#include "kv_ragged.h"
 #include "model.h"
 
 namespace nova {
@@ -32,28 +33,5 @@ constexpr int kQ8VsOff = kQ8KsOff + 4 * kKvBlock;
 constexpr int kQ8Rec = kQ8VsOff + 4 * kKvBlock;              // 4224
 constexpr int64_t kQ8Page = (int64_t)Model::NKV * kQ8Rec;    // one page of one layer
 static_assert(kQ8Rec == 4224, "documented record size");
-
-// Rows of a ragged call: session i owns rows [off[i], off[i+1]) of the flat
-// arrays, or n rows each where there are no offsets.  Offsets come from device
-// memory, so they are held inside [0, n_rows].
-struct Q8Rows {
-    const int32_t* off;        // device [n_sess + 1] or null
-    int uniform;               // rows per session without offsets
-    int n_rows;
-};
-
-__device__ __forceinline__ int q8_row0(const Q8Rows& r, int i) {
-    return r.off ? min(max(r.off[i], 0), r.n_rows) : i * r.uniform;
-}
-__device__ __forceinline__ int q8_count(const Q8Rows& r, int i) {
-    return r.off ? max(q8_row0(r, i + 1) - q8_row0(r, i), 0) : r.uniform;
-}
-
-// record of logical page pg: table entries outside the pool read page 0, so
-// that no address leaves it
-__device__ __forceinline__ int q8_phys(const int32_t* table, int pg, int nb) {
-    const int p = table[pg];
-    return (unsigned)p < (unsigned)nb ? p : 0;
-}
 
 }  // namespace nova
