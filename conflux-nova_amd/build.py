@@ -37,6 +37,9 @@ HIP_SOURCES = [
     "code/kernel/hip/kv_pages.hip",
     "code/kernel/hip/kv_q8.hip",
     "code/kernel/hip/attn_q8.hip",
+    "code/kernel/hip/kv_q4.hip",
+    "code/kernel/hip/attn_q4.hip",
+    "code/kernel/hip/kv_plan.hip",
     "code/kernel/hip/rope.hip",
     "code/kernel/hip/q4k.hip",
 ]

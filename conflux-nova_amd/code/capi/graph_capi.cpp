@@ -127,6 +127,11 @@ nova_paged_t nova_paged_new_q8(int n_slices, int64_t ctx) {
     h->init(n_slices, ctx, true);
     return h;
 }
+nova_paged_t nova_paged_new_q4(int n_slices, int64_t ctx) {
+    PagedKv* h = new PagedKv;
+    h->init(n_slices, ctx, nova::KvPages::q4);
+    return h;
+}
 void nova_paged_delete(nova_paged_t h) {
     H(h)->destroy();
     delete H(h);
@@ -135,6 +140,7 @@ nova_kvpool_t nova_paged_pool(nova_paged_t h) { return &H(h)->pool(); }
 uint16_t* nova_paged_pool_k(nova_paged_t h) { return H(h)->k_base(); }
 uint16_t* nova_paged_pool_v(nova_paged_t h) { return H(h)->v_base(); }
 void* nova_paged_pool_q8(nova_paged_t h) { return H(h)->q8_base(); }
+void* nova_paged_pool_q4(nova_paged_t h) { return H(h)->q4_base(); }
 int32_t* nova_paged_tables(nova_paged_t h) { return H(h)->tables(); }
 int nova_paged_nb(nova_paged_t h) { return H(h)->nb(); }
 nova_stream_t nova_paged_stream(nova_paged_t h) { return H(h)->stream(); }

@@ -1,0 +1,276 @@
+// kv_plan.hip -- a step's bookkeeping on the GPU: from the lengths of the sessions to
+// pages given back and handed out, block tables, row offsets, positions and cache slots.
+//
+// Session i holds have tokens, keeps the first `keep` of them and adds `new`.  With
+// pages(n) = ceil(n / 16) it gives back its pages [pages(keep), pages(have)) and takes
+// pages(keep + new) - pages(keep).  The pages that are free are a stack; those given back go
+// on top of it, in (session, page) order with the first on top, and pages are taken from the
+// top in the same order, so a step that adds what the one before gave back gets the
+// same pages.  Everything is prefix sums over the sessions, so there are no atomics and
+// the result is the same every time.
+//
+// One workgroup does the sums (two passes over the sessions: what comes back, then what
+// fits) and, for a small step, all the rest.  Larger ones leave pages and rows to two
+// more launches over the whole chip, as the stack must be whole before pages are taken
+// from it.  Latency bounds all of it.
+#include <hip/hip_runtime.h>
+#include <algorithm>
+#include <cstdint>
+
+#include "check.h"
+#include "model.h"
+#include "nova_kernel.h"
+
+namespace nova {
+namespace {
+
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+constexpr int PT = 1024;                       // threads of the workgroup that sums
+constexpr int FT = 256;                        // threads of the others
+constexpr int kOffsets = 4096;                 // sessions whose row offsets fit a workgroup's LDS
+
+struct PlanArgs {
+    int32_t* tables;
+    int64_t stride;
+    const int32_t *have, *keep, *add;          // keep: or null
+    int n_sess, max_rows, nb;
+    int32_t* free_pages;
+    const int32_t* n_free;
+    int32_t *past, *keys, *row_off, *pos;
+    int64_t* slots;
+    int32_t* free_left;
+    i4* info;                                  // workspace: [n_sess] {first, held, pages back before, pages taken before}
+    int64_t* stack;                            // workspace: {free pages with those back, free pages before}
+};
+
+__device__ __forceinline__ int64_t pages_of(int64_t tokens) { return (tokens + kKvBlock - 1) >> kKvBlockShift; }
+
+struct Wish {
+    int64_t have, keep, add;
+};
+__device__ __forceinline__ Wish wish(const PlanArgs& a, int i) {
+    const int64_t most = a.stride * kKvBlock;
+    Wish w;
+    w.have = min(max((int64_t)a.have[i], (int64_t)0), most);
+    w.keep = a.keep ? min(max((int64_t)a.keep[i], (int64_t)0), w.have) : w.have;
+    w.add = max((int64_t)a.add[i], (int64_t)0);
+    if (w.keep + w.add > most) w.add = 0;                    // more than its table holds: nothing
+    return w;
+}
+
+// inclusive sums over the workgroup, in thread order; `total` for all threads
+struct Pair {
+    int64_t a, b;
+};
+__device__ __forceinline__ Pair block_scan(Pair v, Pair* s_wave, Pair& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t a = __shfl_up((long long)v.a, o, 64), b = __shfl_up((long long)v.b, o, 64);
+        if (lane >= o) {
+            v.a += a;
+            v.b += b;
+        }
+    }
+    __syncthreads();                                         // the last call's sums have been read
+    if (lane == 63) s_wave[wave] = v;
+    __syncthreads();
+    total = Pair{0, 0};
+#pragma unroll
+    for (int w = 0; w < PT / 64; ++w) {
+        const Pair p = s_wave[w];
+        if (w < wave) {
+            v.a += p.a;
+            v.b += p.b;
+        }
+        total.a += p.a;
+        total.b += p.b;
+    }
+    return v;
+}
+
+// the pages that sessions from..n_sess step by `step` give back, onto the stack; one wave
+__device__ __forceinline__ void give_back(const PlanArgs& a, int from, int step, int64_t avail, int64_t n_free) {
+    for (int i = from; i < a.n_sess; i += step) {
+        const i4 in = a.info[i];
+        for (int p = in[0] + (int)(threadIdx.x & 63); p < in[1]; p += 64) {
+            const int64_t at = avail - 1 - ((int64_t)in[2] + p - in[0]);
+            if (at >= n_free) a.free_pages[at] = a.tables[i * a.stride + p];
+        }
+    }
+}
+// the page that session i's nth new page is
+__device__ __forceinline__ int taken(const PlanArgs& a, const i4& in, int64_t nth, int64_t avail) {
+    return a.free_pages[avail - 1 - ((int64_t)in[3] + nth)];
+}
+__device__ __forceinline__ void hand_out(const PlanArgs& a, int from, int step, int64_t avail) {
+    for (int i = from; i < a.n_sess; i += step) {
+        const i4 in = a.info[i];
+        const int last = (int)pages_of(a.keys[i]);
+        for (int p = in[0] + (int)(threadIdx.x & 63); p < last; p += 64) a.tables[i * a.stride + p] = taken(a, in, p - in[0], avail);
+    }
+}
+// position and slot of row r; off: the rows' offsets
+__device__ __forceinline__ void place_row(const PlanArgs& a, const int32_t* off, int r, int64_t avail) {
+    int pos = -1;
+    int64_t slot = -1;
+    if (r < off[a.n_sess]) {
+        int lo = 0, hi = a.n_sess - 1;                       // the last session that starts at r or before and has rows
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (off[mid] <= r) lo = mid;
+            else hi = mid - 1;
+        }
+        pos = a.past[lo] + r - off[lo];
+        const int p = pos >> kKvBlockShift;
+        const i4 in = a.info[lo];
+        const int page = p < in[0] ? a.tables[lo * a.stride + p] : taken(a, in, p - in[0], avail);
+        if ((unsigned)page < (unsigned)a.nb) slot = (int64_t)page * kKvBlock + (pos & kKvBlockMask);
+    }
+    a.pos[r] = pos;
+    a.slots[r] = slot;
+}
+
+template <bool kAll>
+__global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
+    __shared__ Pair s_wave[PT / 64];
+    __shared__ int32_t s_off[kAll ? kOffsets + 1 : 1];
+    const int tid = threadIdx.x;
+    const int64_t n_free = min(max((int64_t)*a.n_free, (int64_t)0), (int64_t)a.nb);
+    // what comes back
+    int64_t back = 0;
+    for (int base = 0; base < a.n_sess; base += PT) {
+        const int i = base + tid;
+        i4 in = i4{0, 0, 0, 0};
+        if (i < a.n_sess) {
+            const Wish w = wish(a, i);
+            in[0] = (int)pages_of(w.keep);
+            in[1] = (int)pages_of(w.have);
+        }
+        Pair total;
+        const Pair sum = block_scan(Pair{in[1] - in[0], 0}, s_wave, total);
+        // (more than the stack holds is nowhere)
+        in[2] = (int)min(back + sum.a - (in[1] - in[0]), (int64_t)a.nb);
+        if (i < a.n_sess) a.info[i] = in;
+        back += total.a;
+    }
+    const int64_t avail = min(n_free + back, (int64_t)a.nb);
+    // what fits
+    Pair before{0, 0}, given{0, 0};                          // rows, pages: wished for; granted
+    for (int base = 0; base < a.n_sess; base += PT) {
+        const int i = base + tid;
+        Wish w{0, 0, 0};
+        int64_t more = 0;
+        if (i < a.n_sess) {
+            w = wish(a, i);
+            more = pages_of(w.keep + w.add) - pages_of(w.keep);
+        }
+        Pair total;
+        const Pair sum = block_scan(Pair{w.add, more}, s_wave, total);
+        const bool fits = before.a + sum.a <= a.max_rows && before.b + sum.b <= avail;
+        if (i < a.n_sess) {
+            // sessions behind the first that does not fit get nothing, so the sums up to
+            // a session that fits are those of what was granted
+            const int64_t add = fits ? w.add : 0;
+            a.info[i][3] = fits ? (int)(before.b + sum.b - more) : 0;
+            a.past[i] = (int)w.keep;
+            a.keys[i] = (int)(w.keep + add);
+        }
+        Pair all;
+        const Pair ok = block_scan(Pair{fits ? w.add : 0, fits ? more : 0}, s_wave, all);
+        if (i < a.n_sess) {
+            a.row_off[i + 1] = (int)(given.a + ok.a);
+            if (kAll) s_off[i + 1] = (int)(given.a + ok.a);
+        }
+        before.a += total.a;
+        before.b += total.b;
+        given.a += all.a;
+        given.b += all.b;
+    }
+    if (tid == 0) {
+        a.row_off[0] = 0;
+        if (kAll) s_off[0] = 0;
+        *a.free_left = (int)(avail - given.b);
+        a.stack[0] = avail;
+        a.stack[1] = n_free;
+    }
+    if constexpr (kAll) {
+        __syncthreads();
+        give_back(a, tid >> 6, PT / 64, avail, n_free);
+        __syncthreads();
+        hand_out(a, tid >> 6, PT / 64, avail);
+        for (int r = tid; r < a.max_rows; r += PT) place_row(a, s_off, r, avail);
+    }
+}
+
+__global__ void __launch_bounds__(FT) plan_back_kernel(PlanArgs a) {
+    give_back(a, (int)(blockIdx.x * (FT / 64) + (threadIdx.x >> 6)), (int)gridDim.x * (FT / 64), a.stack[0], a.stack[1]);
+}
+
+// workgroups below row_wgs: rows; the others: tables
+__global__ void __launch_bounds__(FT) plan_rows_kernel(PlanArgs a, int row_wgs) {
+    __shared__ int32_t s_off[kOffsets + 1];
+    const int64_t avail = a.stack[0];
+    if ((int)blockIdx.x >= row_wgs) {
+        const int wgs = (int)gridDim.x - row_wgs;
+        hand_out(a, ((int)blockIdx.x - row_wgs) * (FT / 64) + (int)(threadIdx.x >> 6), wgs * (FT / 64), avail);
+        return;
+    }
+    const bool here = a.n_sess <= kOffsets;
+    if (here)
+        for (int i = threadIdx.x; i <= a.n_sess; i += FT) s_off[i] = a.row_off[i];
+    __syncthreads();
+    for (int r = blockIdx.x * FT + threadIdx.x; r < a.max_rows; r += row_wgs * FT) place_row(a, here ? s_off : a.row_off, r, avail);
+}
+
+// One launch up to this many rows and sessions.
+constexpr int kSmallRows = 2048, kSmallSessions = 256;
+static_assert(kSmallSessions <= kOffsets, "offsets in LDS");
+constexpr int kWgs = 1024;                     // of the larger launches
+
+size_t info_at() { return 256; }
+
+}  // namespace
+}  // namespace nova
+
+using namespace nova;
+
+extern "C" {
+
+size_t kv_step_plan_workspace_bytes(int n_sess) {
+    NOVA_REQUIRE(n_sess >= 1 && n_sess <= 65535);
+    return info_at() + (size_t)n_sess * sizeof(i4);
+}
+
+void launch_kv_step_plan(int32_t* tables, int table_stride, const int32_t* n_have, const int32_t* n_keep,
+                         const int32_t* n_new, int n_sess, int max_rows, int32_t* free_pages, const int32_t* n_free, int nb,
+                         int32_t* n_past, int32_t* n_keys, int32_t* row_off, int32_t* pos, int64_t* slots,
+                         int32_t* n_free_left, void* workspace, nova_stream_t s) {
+    NOVA_REQUIRE(tables && n_have && n_new && free_pages && n_free && n_past && n_keys && row_off && n_free_left);
+    NOVA_REQUIRE(n_sess >= 1 && n_sess <= 65535 && table_stride > 0 && table_stride <= (1 << 26));
+    NOVA_REQUIRE((int64_t)n_sess * table_stride <= (int64_t)1 << 32);
+    NOVA_REQUIRE(max_rows >= 0 && max_rows <= (1 << 24) && nb > 0 && nb <= (1 << 27));
+    NOVA_REQUIRE((pos && slots) || max_rows == 0);
+    NOVA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
+    char* ws = static_cast<char*>(workspace);
+    const PlanArgs a{tables,  table_stride, n_have, n_keep,  n_new, n_sess, max_rows,    nb,
+                     free_pages, n_free,       n_past, n_keys, row_off, pos,   slots,  n_free_left,
+                     reinterpret_cast<i4*>(ws + info_at()), reinterpret_cast<int64_t*>(ws)};
+    const hipStream_t st = reinterpret_cast<hipStream_t>(s);
+    if (max_rows <= kSmallRows && n_sess <= kSmallSessions) {
+        hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(PT), 0, st, a);
+        NOVA_LAUNCHED();
+        return;
+    }
+    hipLaunchKernelGGL(plan_kernel<false>, dim3(1), dim3(PT), 0, st, a);
+    NOVA_LAUNCHED();
+    const int sess_wgs = std::min((n_sess + FT / 64 - 1) / (FT / 64), kWgs);
+    hipLaunchKernelGGL(plan_back_kernel, dim3(sess_wgs), dim3(FT), 0, st, a);
+    NOVA_LAUNCHED();
+    const int row_wgs = std::min((max_rows + FT - 1) / FT, kWgs);
+    hipLaunchKernelGGL(plan_rows_kernel, dim3(row_wgs + sess_wgs), dim3(FT), 0, st, a, row_wgs);
+    NOVA_LAUNCHED();
+}
+
+}  // extern "C"

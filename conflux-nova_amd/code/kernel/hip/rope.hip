@@ -21,6 +21,7 @@
 // head (float4 loads, 16 lanes per head); the fused kernel adds (kv head,
 // octet) units that convert 8 values of v.  HBM-bound elementwise work.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -28,6 +29,7 @@
 #include "model.h"
 #include "nova_kernel.h"
 #include "rope_math.h"
+#include "rope_rows.h"
 
 namespace nova {
 namespace {
@@ -153,6 +155,42 @@ void launch(const RopeArgs& a, int n_sess, hipStream_t s) {
     NOVA_LAUNCHED();
 }
 
+// ---- rows at positions of their own ----
+//
+// A row's angles are pos * freq[i], in double: the product of a 31-bit and a 24-bit number,
+// exact for positions below 2^29, so that a far position's angle is as good as a near one's
+// (in fp32 a position of 10^6 has its first pair's angle to 1/16).  cos and sin are
+// rounded to fp32 once, after the magnitude.  The angles of a step's rows serve all layers
+// and every head, so they are a launch of their own and not part of the rotation.
+__global__ void __launch_bounds__(RT) rope_angles_kernel(const int32_t* __restrict__ pos, int64_t n, const float* __restrict__ freq,
+                                                         int half, double magnitude, float* __restrict__ cs, float* __restrict__ sn) {
+    const int64_t e = (int64_t)blockIdx.x * RT + threadIdx.x;
+    if (e >= n) return;
+    const int64_t row = e / half;
+    const double a = (double)pos[row] * (double)freq[e - row * half];
+    double s, c;
+    sincos(a, &s, &c);
+    cs[e] = (float)(c * magnitude);
+    sn[e] = (float)(s * magnitude);
+}
+
+// A workgroup per row, all heads of q and k.  HBM-bound elementwise work.
+template <RopeForm kForm>
+__global__ void __launch_bounds__(RT) rope_rows_kernel(const float* q, const float* k, const int32_t* pos, const float* cs,
+                                                       const float* sn, int rot, float* q_out, float* k_out) {
+    const int64_t row = blockIdx.x;
+    if (pos && pos[row] < 0) return;
+    const int units = rope_units<kForm>(rot);
+    const float *c = cs + row * (rot / 2), *s = sn + row * (rot / 2);
+    for (int u = threadIdx.x; u < (NH + NKV) * units; u += RT) {
+        const int h = u / units;
+        const int64_t at = h < NH ? (row * NH + h) * HD : (row * NKV + h - NH) * HD;
+        rope_unit<kForm>((h < NH ? q : k) + at, (h < NH ? q_out : k_out) + at, c, s, rot, u - h * units);
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 }  // namespace
 }  // namespace nova
 
@@ -228,6 +266,55 @@ void launch_rope_kv_store_paged_batch(float* q, const float* k, const float* v, 
     a.layer = layer;
     a.nb = nb;
     launch(a, n_sess, reinterpret_cast<hipStream_t>(s));
+}
+
+int nova_rope_freqs(const nova_rope_cfg* cfg, float* freq, double* magnitude) {
+    NOVA_REQUIRE(cfg && freq && magnitude);
+    const int rot = cfg->rot_dim;
+    NOVA_REQUIRE(rot >= 2 && rot <= HD && rot % 2 == 0);
+    NOVA_REQUIRE(cfg->scaling >= NOVA_ROPE_PLAIN && cfg->scaling <= NOVA_ROPE_BY_PARTS);
+    NOVA_REQUIRE(std::isfinite(cfg->base) && cfg->base > 0);
+    const bool scaled = cfg->scaling != NOVA_ROPE_PLAIN, parts = cfg->scaling == NOVA_ROPE_BY_PARTS;
+    NOVA_REQUIRE(!scaled || (std::isfinite(cfg->factor) && cfg->factor >= 1));
+    NOVA_REQUIRE(!parts || (cfg->train_len > 0 && cfg->slow_turns >= 0 && cfg->fast_turns > cfg->slow_turns));
+    const double base = cfg->scaling == NOVA_ROPE_BASE ? cfg->base * std::pow(cfg->factor, (double)rot / std::max(rot - 2, 1)) : cfg->base;
+    for (int i = 0; i < rot / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / rot);
+        if (cfg->scaling == NOVA_ROPE_LINEAR) f /= cfg->factor;
+        if (parts) {
+            const double turns = cfg->train_len * f / (2 * M_PI);
+            const double keep = std::min(std::max((turns - cfg->slow_turns) / (cfg->fast_turns - cfg->slow_turns), 0.0), 1.0);
+            f = f * keep + f / cfg->factor * (1 - keep);
+        }
+        freq[i] = (float)f;
+    }
+    *magnitude = parts ? 0.1 * std::log(cfg->factor) + 1 : 1;
+    return rot / 2;
+}
+
+void launch_rope_angles(const int32_t* pos, int n_rows, const float* freq, int rot_dim, double magnitude, float* cs, float* sn,
+                        nova_stream_t s) {
+    NOVA_REQUIRE(pos && freq && cs && sn && n_rows >= 0 && n_rows <= (1 << 24));
+    NOVA_REQUIRE(rot_dim >= 2 && rot_dim <= HD && rot_dim % 2 == 0);
+    NOVA_REQUIRE(std::isfinite(magnitude));
+    if (n_rows == 0) return;
+    const int64_t n = (int64_t)n_rows * (rot_dim / 2);
+    hipLaunchKernelGGL(rope_angles_kernel, dim3((unsigned)((n + RT - 1) / RT)), dim3(RT), 0, reinterpret_cast<hipStream_t>(s), pos,
+                       n, freq, rot_dim / 2, magnitude, cs, sn);
+    NOVA_LAUNCHED();
+}
+
+void launch_rope_rows(const float* q, const float* k, const int32_t* pos, const float* cs, const float* sn, int n_rows,
+                      int rot_dim, int beside, float* q_out, float* k_out, nova_stream_t s) {
+    NOVA_REQUIRE(q && k && cs && sn && q_out && k_out && n_rows >= 0 && n_rows <= (1 << 24));
+    NOVA_REQUIRE(rot_dim >= 2 && rot_dim <= HD && rot_dim % 2 == 0);
+    NOVA_REQUIRE(aligned16(q) && aligned16(k) && aligned16(cs) && aligned16(sn) && aligned16(q_out) && aligned16(k_out));
+    if (n_rows == 0) return;
+    rope_forms(rot_dim, beside != 0, [&](auto form) {
+        hipLaunchKernelGGL(rope_rows_kernel<decltype(form)::value>, dim3((unsigned)n_rows), dim3(RT), 0,
+                           reinterpret_cast<hipStream_t>(s), q, k, pos, cs, sn, rot_dim, q_out, k_out);
+        NOVA_LAUNCHED();
+    });
 }
 
 }  // extern "C"

@@ -12,7 +12,7 @@
 // Differences, all MI355X-motivated:
 //   * pools are fp16 and sized by (n_slices, ctx) at run time, from one
 //     dev_alloc per pool; at 288 GB per GPU the pool is the dominant tenant.
-//     The same layer serves one pool of 8-bit pages (init's q8)
+//     The same layer serves one pool of 8-bit or 4-bit pages (init's KvPages)
 //   * page clears and COW copies are single launches (launch_kv_zero_pages,
 //     launch_kv_cow_apply) instead of 2*L memset/memcpy calls per page; the
 //     table patch rides in the same launch
@@ -38,18 +38,23 @@
 
 namespace nova {
 
+// what the pages of a PagedKv hold: fp16 values in two pools, or codes in one
+enum class KvPages { f16, q8, q4 };
+
 class PagedKv {
 public:
     // n_slices sessions of up to ctx tokens share NB = n_slices * ceil(ctx/16) pages.
-    // q8: one pool of 8-bit pages instead of the two fp16 pools; tables, page ids,
-    // refcounts and COW decisions are the same, and KvSlice::k, v stay null.
-    void init(int n_slices, int64_t ctx, bool q8 = false) {
+    // q8, q4: one pool of 8-bit or 4-bit pages instead of the two fp16 pools; tables, page
+    // ids, refcounts and COW decisions are the same, and KvSlice::k, v stay null.
+    void init(int n_slices, int64_t ctx, bool q8 = false) { init(n_slices, ctx, q8 ? KvPages::q8 : KvPages::f16); }
+    void init(int n_slices, int64_t ctx, KvPages pages) {
         geo_ = nova_model_geometry();
         pool_.init(n_slices, ctx);
         nb_ = pool_.nb_total();
-        if (q8) {
-            pool_bytes_ = (uint64_t)geo_.n_layers * (uint64_t)nb_ * (uint64_t)kv_q8_page_bytes();
-            q8_ = static_cast<uint8_t*>(dev_alloc(pool_bytes_));
+        if (pages != KvPages::f16) {
+            const uint64_t page = pages == KvPages::q8 ? kv_q8_page_bytes() : kv_q4_page_bytes();
+            pool_bytes_ = (uint64_t)geo_.n_layers * (uint64_t)nb_ * page;
+            (pages == KvPages::q8 ? q8_ : q4_) = static_cast<uint8_t*>(dev_alloc(pool_bytes_));
         } else {
             const uint64_t per_pool = (uint64_t)geo_.n_layers * (uint64_t)nb_ * (uint64_t)geo_.kv_block *
                                       (uint64_t)geo_.nkv * (uint64_t)geo_.hd * 2ull;
@@ -67,10 +72,11 @@ public:
         dev_free(k_);
         dev_free(v_);
         dev_free(q8_);
+        dev_free(q4_);
         dev_free(tables_);
         if (stream_) dev_stream_destroy(stream_);
         k_ = v_ = nullptr;
-        q8_ = nullptr;
+        q8_ = q4_ = nullptr;
         tables_ = nullptr;
         stream_ = nullptr;
     }
@@ -215,6 +221,7 @@ public:
     uint16_t* k_base() const { return k_; }
     uint16_t* v_base() const { return v_; }
     uint8_t* q8_base() const { return q8_; }           // null unless the pool holds 8-bit pages
+    uint8_t* q4_base() const { return q4_; }           // null unless it holds 4-bit pages
     int32_t* tables() const { return tables_; }
     int nb() const { return nb_; }
     uint64_t pool_bytes() const { return pool_bytes_; }
@@ -223,11 +230,13 @@ public:
 private:
     void zero_pages(const int32_t* pages_dev, int n) {
         if (q8_) launch_kv_q8_zero_pages(q8_, nb_, pages_dev, n, stream_);
+        else if (q4_) launch_kv_q4_zero_pages(q4_, nb_, pages_dev, n, stream_);
         else launch_kv_zero_pages(k_, v_, nb_, pages_dev, n, stream_);
     }
 
     void cow_apply(const nova_cow_op* ops, int n, nova_stream_t st) {
         if (q8_) launch_kv_q8_cow_apply(q8_, nb_, tables_, ops, n, st);
+        else if (q4_) launch_kv_q4_cow_apply(q4_, nb_, tables_, ops, n, st);
         else launch_kv_cow_apply(k_, v_, nb_, tables_, ops, n, st);
     }
 
@@ -252,6 +261,7 @@ private:
     uint16_t* k_ = nullptr;
     uint16_t* v_ = nullptr;
     uint8_t* q8_ = nullptr;
+    uint8_t* q4_ = nullptr;
     int32_t* tables_ = nullptr;
     uint64_t pool_bytes_ = 0;
     nova_stream_t stream_ = nullptr;

@@ -21,7 +21,7 @@ PKG = Path(__file__).resolve().parent.parent
 LIB_DIR = Path(os.environ.get("NOVA_LIB_DIR", str(PKG / "lib")))
 MODELS = ("qwen25_1p5b", "qwen25_7b", "qwen25_14b")
 
-vp, i32, i64, u64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_size_t
+vp, i32, i64, u64, f32, f64, sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_double, C.c_size_t
 P_i32 = C.POINTER(C.c_int32)
 P_i64 = C.POINTER(C.c_int64)
 P_int = C.POINTER(C.c_int)
@@ -35,6 +35,15 @@ class Geometry(C.Structure):
 
 class CowOp(C.Structure):
     _fields_ = [("src", C.c_int32), ("dst", C.c_int32), ("table_index", C.c_int64)]
+
+
+class RopeCfg(C.Structure):
+    _fields_ = [("rot_dim", C.c_int), ("scaling", C.c_int), ("base", C.c_double), ("factor", C.c_double),
+                ("train_len", C.c_int), ("slow_turns", C.c_double), ("fast_turns", C.c_double)]
+
+
+# nova_rope_cfg.scaling
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BY_PARTS = range(4)
 
 
 # name -> (restype, argtypes)
@@ -105,6 +114,22 @@ _SIGS = {
     "launch_attn_chunk_q8_batch": (None, [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp]),
     "launch_kv_q8_cow_apply": (None, [vp, i32, vp, C.POINTER(CowOp), i32, vp]),
     "launch_kv_q8_zero_pages": (None, [vp, i32, vp, i32, vp]),
+    "nova_rope_freqs": (i32, [C.POINTER(RopeCfg), C.POINTER(f32), C.POINTER(f64)]),
+    "launch_rope_angles": (None, [vp, i32, vp, i32, f64, vp, vp, vp]),
+    "launch_rope_rows": (None, [vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp]),
+    "kv_q4_page_bytes": (sz, []),
+    "launch_kv_q4_store_batch": (None, [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]),
+    "launch_rope_rows_kv_q4_store_batch": (None, [vp, vp, vp, vp, vp, i32, i32, vp, vp, i32, vp, vp, i32, i32, i32, i32,
+                                                  vp, vp]),
+    "launch_kv_q4_load_batch": (None, [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp]),
+    "attn_decode_q4_workspace_bytes": (sz, [i32]),
+    "launch_attn_decode_q4_batch": (None, [vp, vp, vp, i32, vp, i32, i32, i32, vp, vp, vp]),
+    "attn_chunk_q4_workspace_bytes": (sz, [i32, i32, i32]),
+    "launch_attn_chunk_q4_batch": (None, [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "launch_kv_q4_cow_apply": (None, [vp, i32, vp, C.POINTER(CowOp), i32, vp]),
+    "launch_kv_q4_zero_pages": (None, [vp, i32, vp, i32, vp]),
+    "kv_step_plan_workspace_bytes": (sz, [i32]),
+    "launch_kv_step_plan": (None, [vp, i32, vp, vp, vp, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     # nova_graph.h
     "nova_kvpool_new": (vp, [i32, i64]),
     "nova_kvpool_delete": (None, [vp]),
@@ -143,6 +168,8 @@ _SIGS = {
     "nova_paged_new": (vp, [i32, i64]),
     "nova_paged_new_q8": (vp, [i32, i64]),
     "nova_paged_pool_q8": (vp, [vp]),
+    "nova_paged_new_q4": (vp, [i32, i64]),
+    "nova_paged_pool_q4": (vp, [vp]),
     "nova_paged_delete": (None, [vp]),
     "nova_paged_pool": (vp, [vp]),
     "nova_paged_pool_k": (vp, [vp]),

@@ -73,6 +73,9 @@ nova_paged_t  nova_paged_new(int n_slices, int64_t ctx);
  * clears 8-bit pages and the COW calls copy them. */
 nova_paged_t  nova_paged_new_q8(int n_slices, int64_t ctx);
 void*         nova_paged_pool_q8(nova_paged_t h);
+/* ... and over one pool of 4-bit pages. */
+nova_paged_t  nova_paged_new_q4(int n_slices, int64_t ctx);
+void*         nova_paged_pool_q4(nova_paged_t h);
 void          nova_paged_delete(nova_paged_t h);
 nova_kvpool_t nova_paged_pool(nova_paged_t h);          /* its KvPool, for the getters above */
 uint16_t*     nova_paged_pool_k(nova_paged_t h);

@@ -353,6 +353,124 @@ void launch_kv_q8_cow_apply(uint8_t* pool, int nb, int32_t* tables_dev, const no
                             nova_stream_t s);
 void launch_kv_q8_zero_pages(uint8_t* pool, int nb, const int32_t* pages, int n_pages, nova_stream_t s);
 
+/* ---- rows at positions of their own (no reference counterpart) ----
+ *
+ * The rotation of launch_rope_batch for any configuration: the first rot_dim dims of a
+ * head (even, 2..HD) turn in pairs, half of them apart (dims i and i + rot_dim/2; beside = 0)
+ * or side by side (2i and 2i + 1; beside = 1), dims from rot_dim on stay; pair i of a
+ * row at position p turns by the angle p * freq[i].  y0 = x0*c - x1*s, y1 = x0*s + x1*c,
+ * every product rounded (the bits of launch_rope_batch for the same cos and sin). */
+enum { NOVA_ROPE_PLAIN = 0, NOVA_ROPE_LINEAR = 1, NOVA_ROPE_BASE = 2, NOVA_ROPE_BY_PARTS = 3 };
+typedef struct {
+    int rot_dim;           /* turning dims of a head */
+    int scaling;           /* NOVA_ROPE_*, for contexts `factor` times as long as the model's */
+    double base;           /* freq[i] = base^(-2i/rot_dim) */
+    double factor;         /* >= 1; not read by NOVA_ROPE_PLAIN */
+    int train_len;         /* BY_PARTS: the model's own context */
+    double slow_turns;     /* BY_PARTS: pairs that turn fewer times over train_len are stretched ... */
+    double fast_turns;     /* ... and those that turn more often stay; between, by degrees */
+} nova_rope_cfg;
+/* The pairs' rates in fp32 (host array of rot_dim/2; made in 64 bits) and the factor on
+ * cos and sin, once per model.  LINEAR: freq / factor.  BASE: base * factor^(rot_dim /
+ * (rot_dim - 2)).  BY_PARTS: freq of the fast pairs, freq / factor of the slow ones, and
+ * a magnitude of 0.1 ln(factor) + 1 (else 1).  Returns rot_dim / 2. */
+int nova_rope_freqs(const nova_rope_cfg* cfg, float* freq, double* magnitude);
+/* The angles of a step's rows, for all layers: cs, sn [n_rows][rot_dim/2] =
+ * fp32(cos(pos[r] * freq[i]) * magnitude), and sin, in 64 bits before the one rounding; the angle
+ * is exact for |pos| < 2^29.  pos: device int32[n_rows]; freq: device. */
+void launch_rope_angles(const int32_t* pos, int n_rows, const float* freq, int rot_dim, double magnitude, float* cs,
+                        float* sn, nova_stream_t s);
+/* Turn q [n_rows][NH][HD] into q_out and k [n_rows][NKV][HD] into k_out (each may be its own
+ * input).  Rows whose pos is negative (launch_kv_step_plan's empty rows) are left as they are; pos
+ * may be NULL: all rows.  All fp32 arrays 16-byte aligned. */
+void launch_rope_rows(const float* q, const float* k, const int32_t* pos, const float* cs, const float* sn, int n_rows,
+                      int rot_dim, int beside, float* q_out, float* k_out, nova_stream_t s);
+
+/* ---- 4-bit pages (no reference counterpart) ----
+ *
+ * A cache at 68 instead of 256 bytes per row of 128 values: 4-bit floating point codes
+ * (0, .5, 1, 1.5, 2, 3, 4, 6 for codes 0..7, the sign in bit 3) with a power of two per 32
+ * dims, held as its exponent plus 127 in a byte: the block-scaled fp4 operand of the
+ * matrix instructions.  One pool
+ *     pool[layer][NB][NKV][2176]  (bytes; kv_q4_page_bytes() = NKV * 2176),
+ * 16-byte aligned, with the block tables, positions and page ids of the other pools.  The
+ * record of a page and kv head holds, for token t of the page and dim d:
+ *     K code       at t*64 + (d>>1), the low half of the byte for even d
+ *     V code       at 1024 + (d>>5)*256 + (d&15)*16 + t, the low half where bit 4 of d is clear
+ *     K exponent   at 2048 + (t&3)*16 + (d>>5)*4 + (t>>2)
+ *     V exponent   at 2112 + (d>>5)*16 + t
+ * An exponent byte b stands for 2^(b - 127), 255 for NaN.  All-zero memory is a page of zeros.
+ *
+ * Quantiser, per 32 values with largest |x| = a: the power is the smallest 2^e with
+ * a <= 7 * 2^e, the codes the values nearest to x / 2^e, ties to the even code, so that no
+ * value is off by more than half its step.  e is at most 96 (values past 7 * 2^96 are held as
+ * 6 * 2^96); where it would be below -100 the 32 are stored as zeros.  A row of 128 that holds an infinity or a NaN gets the exponent byte 255
+ * in all its blocks and reads back as NaN.
+ *
+ * Ragged calls, tables, positions outside them and alignment are those of the 8-bit calls above. */
+size_t kv_q4_page_bytes(void);
+/* Append: the 4-bit form of launch_kv_q8_store_batch. */
+void launch_kv_q4_store_batch(uint8_t* pool, const int32_t* tables, int table_stride, const int32_t* pos0,
+                              const int32_t* row_off, int n_sess, int n_rows, int layer, int nb, const float* k,
+                              const float* v, nova_stream_t s);
+/* Rotation and append in one launch: q's rows turn into q_out (which may be q), k's rows turn and
+ * are quantised with v's (k's buffer is left as passed).  cs, sn: the rows' angles from
+ * launch_rope_angles; rot_dim and beside as in launch_rope_rows, whose bits the turned
+ * rows have. */
+void launch_rope_rows_kv_q4_store_batch(const float* q, const float* k, const float* v, const float* cs, const float* sn,
+                                        int rot_dim, int beside, uint8_t* pool, const int32_t* tables, int table_stride,
+                                        const int32_t* n_past, const int32_t* row_off, int n_sess, int n_rows, int layer,
+                                        int nb, float* q_out, nova_stream_t s);
+/* Read back as fp32 [n_rows][NKV][HD]; every value is exact. */
+void launch_kv_q4_load_batch(const uint8_t* pool, const int32_t* tables, int table_stride, const int32_t* pos0,
+                             const int32_t* row_off, int n_sess, int n_rows, int layer, int nb, float* k, float* v,
+                             nova_stream_t s);
+/* Decode and chunk attention: the calls of the 8-bit pages, with the same arguments.
+ * Precision: fp32 over the values of the codes, but for one rounding: a query (times
+ * 1/sqrt(HD) log2 e) is held to 2^-24 of the largest of each 32 of its dims, or to 2^-124.  Scores
+ * have to be finite in fp32.  Keys that a row does not see do not enter it, whatever they hold. */
+size_t attn_decode_q4_workspace_bytes(int n_sess);
+void launch_attn_decode_q4_batch(const float* q, const uint8_t* pool, const int32_t* tables, int table_stride,
+                                 const int32_t* n_keys, int n_sess, int layer, int nb, float* o, void* workspace,
+                                 nova_stream_t s);
+size_t attn_chunk_q4_workspace_bytes(int n_sess, int n_rows, int max_q);
+void launch_attn_chunk_q4_batch(const float* q, const uint8_t* pool, const int32_t* tables, int table_stride,
+                                const int32_t* n_past, const int32_t* row_off, int n_sess, int n_rows, int max_q,
+                                int layer, int nb, float* o, void* workspace, nova_stream_t s);
+/* launch_kv_q8_cow_apply and launch_kv_q8_zero_pages for 4-bit pages. */
+void launch_kv_q4_cow_apply(uint8_t* pool, int nb, int32_t* tables_dev, const nova_cow_op* ops, int n_ops,
+                            nova_stream_t s);
+void launch_kv_q4_zero_pages(uint8_t* pool, int nb, const int32_t* pages, int n_pages, nova_stream_t s);
+
+/* ---- a step's bookkeeping on the GPU (no reference counterpart) ----
+ *
+ * For servers that give sessions their pages as they grow: the pages of a pool that no
+ * session holds are a stack on the device (free_pages[0 .. *n_free), room for nb), and one call per
+ * step turns the sessions' lengths into everything that the step's calls take.  Any page
+ * format; a page belongs to one session (sessions that share pages stay with the session
+ * manager of nova_graph.h).
+ *
+ * Session i holds n_have[i] tokens, keeps the first n_keep[i] of them (n_keep NULL: all; 0: it
+ * ends) and adds n_new[i].  With pages(n) = ceil(n / 16):
+ *   - its pages [pages(keep), pages(have)) go back: on top of the stack, in (session, page)
+ *     order, the first of all on top;
+ *   - it takes pages(keep + new) - pages(keep) pages from the top, sessions in order, into its
+ *     row of `tables`.  The first session with which the step's rows would pass max_rows
+ *     or its pages would pass the free ones gets no rows, nor does any after it; one whose
+ *     table is too short for keep + new gets none and the others are served.
+ * Lengths below 0 count as 0, n_have past the table as full, n_keep past n_have as n_have.
+ * Out (device): n_past[i] = keep, n_keys[i] = keep + rows granted, row_off [n_sess+1] their sums, and
+ * for each row r of max_rows its position pos[r] and its place in the cache slots[r] =
+ * page * 16 + pos % 16 (-1 where the page is outside [0, nb)); rows behind the last have -1 in both.
+ * *n_free_left: pages free afterwards.  n_keys or n_past may be n_have, n_free_left may be n_free; else
+ * no output overlaps another array.  pos and slots may be NULL if max_rows is 0.  workspace: 16-byte aligned, no
+ * initial contents; calls that may overlap need one each. */
+size_t kv_step_plan_workspace_bytes(int n_sess);
+void launch_kv_step_plan(int32_t* tables, int table_stride, const int32_t* n_have, const int32_t* n_keep,
+                         const int32_t* n_new, int n_sess, int max_rows, int32_t* free_pages, const int32_t* n_free, int nb,
+                         int32_t* n_past, int32_t* n_keys, int32_t* row_off, int32_t* pos, int64_t* slots,
+                         int32_t* n_free_left, void* workspace, nova_stream_t s);
+
 #ifdef __cplusplus
 }
 #endif
