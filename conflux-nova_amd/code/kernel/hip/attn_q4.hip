@@ -8,16 +8,29 @@
 // Numbers.  K goes into the block-scaled matrix instructions as the page holds it.  The
 // query goes in as five 6-bit terms (steps of 1/8 up to 2, each 2^-5 of the one before,
 // with a power of two per 32 dims): it is held to 2^-24 of the largest of its 32 dims, and
-// sums are fp32.  V becomes bf16 with its power of two, which is exact, and a weight is
-// the exact sum of three bf16 terms (8 bits each), so the products lose nothing and their
-// sums are fp32.
+// sums are fp32.  V's values have one bit of mantissa, so a tile of 64 keys whose powers of two
+// lie close together (a window of eight, kSpread) is exact in fp16, and a weight goes in as
+// two fp16 terms: 2^-22 of itself, or 2^-24 - the end of fp16 - where the tile's largest weight in
+// that row stands at 2^kLow or more, which makes it 2^-26 of that weight and, with powers no
+// further apart, 2^-18 of the tile's largest product of weight and value at the very worst.  Any other tile (powers far apart, blocks of zeros, NaN, values past fp16) takes
+// V as bf16 with its power of two, exact too, and a weight as the exact sum of three
+// bf16 terms (8 bits each).  Sums are fp32.
 //
 // One pass over the keys with a running reference and sum of the softmax.  The reference
-// of the weights 2^(s - m) follows the largest score lazily: a weight may grow to
-// 2^kLazy before the sums are rescaled, so that almost no tile does it.
+// m of the weights 2^(s - m) follows the largest score of the tiles, both ways and
+// lazily: a tile's largest weight may lie from 2^kLow to 2^kHigh before the sums are rescaled.  It
+// goes down no further than kDrop below its highest, so that the sums stay inside fp32; what
+// lies lower counts with 2^(kLow - 24 - kDrop) of the row's largest weight at worst.
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <type_traits>
+
+namespace nova {
+namespace {
+constexpr int kMinPiece = 3;
+constexpr int kGroupTiles = 4;
+}  // namespace
+}  // namespace nova
 
 #include "attn_ragged.h"
 #include "check.h"
@@ -28,14 +41,19 @@
 namespace nova {
 namespace {
 
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u6 __attribute__((ext_vector_type(6)));
 typedef int i8v __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef float f32v __attribute__((ext_vector_type(32)));
 
-constexpr float kLazy = 8.f;                   // log2 of a weight that may be above 1 so far
+constexpr float kLow = 2.f, kSet = 10.f, kHigh = 15.9f;   // log2 of a tile's largest weight in fp16 terms: at least, where it is put, at most
+constexpr float kLazy = 8.f;                   // and at most in bf16 terms: 2^21 products of the largest values stay inside fp32
+constexpr float kDrop = 80.f;
+constexpr int kSpread = 8;                     // powers of two of a tile in fp16: this many in a row
+constexpr int kLeastHalf = 127 - 23, kMostHalf = 127 + 13;   // exponent bytes whose values fp16 holds exactly
 constexpr int kTerms = 5;                      // of the query
 constexpr int kLeastExp = -100;                // of a query block: its last term's power is a normal number
 
@@ -45,7 +63,7 @@ constexpr int kLeastExp = -100;                // of a query block: its last ter
 // holds dims 32 g .. + 31 of column c, the block that one power of two serves.
 struct QTerms {
     u6 d[kTerms];
-    int ex;                    // exponent byte of the first term; each one after it 5 less
+    int ex[kTerms];            // exponent bytes of the terms, each 5 less than the one before
 };
 
 __device__ __forceinline__ void q_terms(const f4 (&x)[8], QTerms& out) {
@@ -62,7 +80,8 @@ __device__ __forceinline__ void q_terms(const f4 (&x)[8], QTerms& out) {
         }
     const bool finite = top < 0x7f800000u;
     const int ex = max((int)(top >> 23) - 127, kLeastExp);   // largest < 2^(ex + 1)
-    out.ex = finite ? ex + 127 : kQ4Nan;
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t) out.ex[t] = finite ? ex + 127 - 5 * t : kQ4Nan;
 #pragma unroll
     for (int t = 0; t < kTerms; ++t) {
         const float unit = __uint_as_float((uint32_t)(ex + 127 - 5 * t) << 23);
@@ -85,17 +104,15 @@ __device__ __forceinline__ void q_terms(const f4 (&x)[8], QTerms& out) {
 }
 
 // The query rows of a block's column, lane (g, c) its dims 32 g .. + 31.
-__device__ __forceinline__ void load_q(const AttnArgs& a, const Session& s, int kvh, int col, QTerms& out, int& seen) {
+__device__ __forceinline__ void load_q(const AttnArgs& a, const Session& s, int kvh, int col, f4 (&x)[8], int& seen) {
     const bool real = col < s.rows * G;
     const int r = real ? col / G : 0, hh = real ? col - r * G : 0;
     const float* src = a.q + ((int64_t)(s.row0 + r) * NH + kvh * G + hh) * HD + 32 * ((threadIdx.x & 63) >> 4);
-    f4 x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         x[j] = *reinterpret_cast<const f4*>(src + 4 * j);
         if (!real) x[j] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    q_terms(x, out);
     seen = real ? min(s.past + r + 1, s.keys) : 0;
 }
 
@@ -113,122 +130,227 @@ __device__ __forceinline__ float exponent_of(uint32_t w) {
     return __uint_as_float(kByte == 3 ? w >> 1 : w << (23 - 8 * kByte));
 }
 
-// V of 8 tokens and two dims (32 b + r, 32 b + 16 + r): a byte of `w0`, `w1` per token, low
-// half the lower dim; e0, e1: exponents, a byte per token
-__device__ __forceinline__ void values_bf16(uint32_t w0, uint32_t w1, uint32_t e0, uint32_t e1, b8& lower, b8& upper) {
-    uint32_t p[8];
-    each<4>([&](auto t) {
-        constexpr int kByte = t;
-        p[t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w0, exponent_of<kByte>(e0), kByte));
-        p[4 + t] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w1, exponent_of<kByte>(e1), kByte));
-    });
-    u4 lo, hi;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        lo[i] = __builtin_amdgcn_perm(p[2 * i + 1], p[2 * i], 0x05040100u);
-        hi[i] = __builtin_amdgcn_perm(p[2 * i + 1], p[2 * i], 0x07060302u);
-    }
-    lower = __builtin_bit_cast(b8, lo);
-    upper = __builtin_bit_cast(b8, hi);
+template <bool kHalf, int kByte>
+__device__ __forceinline__ uint32_t pair_of(uint32_t w, uint32_t e) {
+    if constexpr (kHalf) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, exponent_of<kByte>(e), kByte));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, exponent_of<kByte>(e), kByte));
 }
 
-// weights as the exact sums of three bf16 terms: their bits from the top, 8 at a time
-__device__ __forceinline__ void split_bf16(const float (&e)[8], b8 (&out)[3]) {
-    u4 w[3];
+// V of 4 tokens and two dims (32 b + r, 32 b + 16 + r) in fp16 or bf16: a byte of `w` per token,
+// low half the lower dim; e: exponents, a byte per token.  Both dims of a token in a word.
+template <bool kHalf>
+__device__ __forceinline__ void pairs_of(uint32_t w, uint32_t e, uint32_t (&p)[4]) {
+    each<4>([&](auto t) { p[t] = pair_of<kHalf, t>(w, e); });
+}
+// 8 tokens of either dim
+__device__ __forceinline__ void by_dim(const uint32_t (&p)[4], const uint32_t (&q)[4], u4& lower, u4& upper) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        lower[i] = __builtin_amdgcn_perm(p[2 * i + 1], p[2 * i], 0x05040100u);
+        upper[i] = __builtin_amdgcn_perm(p[2 * i + 1], p[2 * i], 0x07060302u);
+        lower[2 + i] = __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x05040100u);
+        upper[2 + i] = __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x07060302u);
+    }
+}
+template <bool kHalf>
+__device__ __forceinline__ void values_of(uint32_t w0, uint32_t w1, uint32_t e0, uint32_t e1, u4& lower, u4& upper) {
+    uint32_t p[4], q[4];
+    pairs_of<kHalf>(w0, e0, p);
+    pairs_of<kHalf>(w1, e1, q);
+    by_dim(p, q, lower, upper);
+}
+
+// 8 tokens' values (A) by their weights (B), added to z
+template <bool kHalf>
+__device__ __forceinline__ f4 add_up(u4 v, u4 w, f4 z) {
+    if constexpr (kHalf) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, v), __builtin_bit_cast(h8, w), z, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, v), __builtin_bit_cast(b8, w), z, 0, 0, 0);
+}
+
+// Terms of the weights: two of fp16, cut off (the second ends at 2^-24), or the three of
+// bf16 that are the weight's bits from the top, 8 at a time.
+template <bool kHalf>
+constexpr int kParts = kHalf ? 2 : 3;
+template <bool kHalf>
+__device__ __forceinline__ void split(const float (&e)[8], u4 (&w)[kParts<kHalf>]) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         float a = e[j], b = e[j + 1];
+        if constexpr (kHalf) {
+            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+            // what is left, a - h[0] and b - h[1], exact: one operation on the half as it is
+            // (the compiler converts it first)
+            float ra, rb;
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
+            w[0][j / 2] = h;
+            w[1][j / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ra, rb));
+        } else {
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            w[k][j / 2] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-            if (k < 2) {
-                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            for (int k = 0; k < 3; ++k) {
+                w[k][j / 2] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+                if (k < 2) {
+                    a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                    b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+                }
             }
         }
     }
-#pragma unroll
-    for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(b8, w[k]);
 }
 
-// which of the four bytes are 255, as bits 0, 8, 16, 24 (exact: the lowest of them and
-// everything below it; those above may be wrong only where one below is right, so this asks
-// byte by byte)
-__device__ __forceinline__ uint32_t bytes_255(uint32_t w) {
+// The tokens of four exponent bytes that are NaN, as four bits; their bytes become 0 (the
+// value counts through its weight instead).
+__device__ __forceinline__ uint32_t take_nan(uint32_t& w) {
     uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m |= ((w >> (8 * k)) & 255u) == 255u ? 1u << (8 * k) : 0u;
+    for (int k = 0; k < 4; ++k)
+        if ((w >> (8 * k) & 255u) == (uint32_t)kQ4Nan) {
+            m |= 1u << k;
+            w &= ~(255u << (8 * k));
+        }
     return m;
 }
-// quick: none of the bytes is 255 if this is 0
-__device__ __forceinline__ uint32_t maybe_255(uint32_t w) { return (~w - 0x01010101u) & w & 0x80808080u; }
+
+// The window of exponent bytes that tiles in fp16 lie in: `base` to base + kSpread - 1.
+struct Window {
+    uint32_t add, want, fill;  // per byte: what is added to a byte of the window gives `want` in its upper five bits
+    bool closed;               // a value past fp16 has been seen: no more fp16, so that the reference's drop keeps the sums finite
+    __device__ __forceinline__ void at(int base) {
+        const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane(base), up = -b & (kSpread - 1);
+        add = up * 0x01010101u;
+        want = (b + up) * 0x01010101u;
+        fill = b * 0x01010101u;
+    }
+    __device__ __forceinline__ void clear() {
+        closed = false;
+        at(127 - kSpread / 2);
+    }
+    // 0 where the four bytes lie in it (a byte that carries into the next one is itself outside)
+    __device__ __forceinline__ uint32_t outside(uint32_t w) const { return ((w + add) ^ want) & 0xf8f8f8f8u; }
+    // Moved to what a tile has, smallest and largest byte: true if that fits a window
+    __device__ __forceinline__ bool move(int least, int most) {
+        least = __builtin_amdgcn_readfirstlane(least);       // (the same in all lanes)
+        most = __builtin_amdgcn_readfirstlane(most);
+        if (most > kMostHalf) closed = true;
+        const bool fits = !closed && most - least < kSpread && least >= kLeastHalf;
+        if (fits) at(min(max((least + most + 1 - kSpread) / 2, kLeastHalf), kMostHalf + 1 - kSpread));
+        return fits;
+    }
+};
+static_assert(kSpread == 8, "upper five bits");
+
+// smallest and largest of a lane's bytes, into the running ones
+__device__ __forceinline__ void byte_range(uint32_t w, int& least, int& most) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int b = (int)(w >> (8 * k) & 255u);
+        least = min(least, b);
+        most = max(most, b);
+    }
+}
+__device__ __forceinline__ void wave_range(int& least, int& most) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        least = min(least, __shfl_xor(least, o, 64));
+        most = max(most, __shfl_xor(most, o, 64));
+    }
+}
 
 // A block's state over the keys seen so far: lane (g, c) holds the reference, its share of
-// the sum and dims 16 d + 4 g .. + 3 of column c.  A score above `limit` moves the
-// reference (a column's first one always does).
+// the sum and dims 16 d + 4 g .. + 3 of column c.  `low` and `high`: between these a tile's
+// largest score, less the reference, leaves it where it is (a column's first one moves it); top:
+// the largest score that it was moved for.
 struct State {
-    float m, l, limit;
+    float m, l, low, high, top;
     f4 acc[DB];
     __device__ __forceinline__ void clear() {
         m = l = 0.f;
-        limit = -INFINITY;
+        low = top = high = -INFINITY;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ float reference() const { return limit == -INFINITY ? kUnset : m; }
+    __device__ __forceinline__ bool unset() const { return high == -INFINITY; }
+    __device__ __forceinline__ float reference() const { return unset() ? kUnset : m; }
+    // the reference by `by` up or down for columns that move; z: scores less it
+    __device__ __forceinline__ void move(bool moves, float col_top, float by, f4 (&z)[4]) {
+        const float corr = !moves ? 1.f : unset() ? 0.f : __builtin_amdgcn_exp2f(-by);
+        if (moves) {
+            top = fmaxf(top, m + col_top);
+            m += by;
+            high = kHigh;
+            low = m > top - kDrop ? kLow : -INFINITY;
+        }
+        l *= corr;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] *= corr;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z[u] -= moves ? by : 0.f;
+    }
 };
 
-// Scores, weights and sum of one tile and block.  k_op(u): K operand of key block u (row
-// 4p + i: token 4u + i of page p), ke: the exponents of its four key blocks; key0: first key
-// of the lane's page; nan: tokens of it whose value is NaN (bit per token; 0 in almost all tiles).
-template <bool kMask, class K>
-__device__ __forceinline__ void weigh(K&& k_op, const QTerms& q, int ke, int key0, int seen, uint32_t nan, State& st,
-                                      b8 (&p)[2][3]) {
-    f4 z[4];
-    const i4 k[4] = {k_op(0), k_op(1), k_op(2), k_op(3)};
+// Scores of one tile and block less the reference m.  k[u]: K operand of key block u (row
+// 4p + i: token 4u + i of page p), ke: the exponents of its four key blocks.  Token j of the lane's
+// page in z[j / 4][j % 4].  The sums begin at -m and take the query's largest term first:
+// where the score is near m, and its weight counts, the others are added to a small number.
+__device__ __forceinline__ void scores(const i4 (&k)[4], const QTerms& q, int ke, float m, f4 (&z)[4]) {
+    const f4 from = f4{-m, -m, -m, -m};
 #pragma unroll
-    for (int u = 0; u < 4; ++u) z[u] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int t = kTerms - 1; t >= 0; --t) {                  // the small terms first
-        const int qe = q.ex == kQ4Nan ? kQ4Nan : q.ex - 5 * t;
-        z[0] = product<0>(k[0], q.d[t], z[0], ke, qe);
-        z[1] = product<1>(k[1], q.d[t], z[1], ke, qe);
-        z[2] = product<2>(k[2], q.d[t], z[2], ke, qe);
-        z[3] = product<3>(k[3], q.d[t], z[3], ke, qe);
+    for (int t = 0; t < kTerms; ++t) {
+        z[0] = product<0>(k[0], q.d[t], t ? z[0] : from, ke, q.ex[t]);
+        z[1] = product<1>(k[1], q.d[t], t ? z[1] : from, ke, q.ex[t]);
+        z[2] = product<2>(k[2], q.d[t], t ? z[2] : from, ke, q.ex[t]);
+        z[3] = product<3>(k[3], q.d[t], t ? z[3] : from, ke, q.ex[t]);
     }
-    float x[16];
+}
+
+// scores of keys that the column does not see; key0: first key of the lane's page
+__device__ __forceinline__ void hide(f4 (&z)[4], int key0, int seen) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (key0 + j >= seen) z[j / 4][j % 4] = -INFINITY;
+}
+
+// The reference follows a tile's scores.
+template <bool kHalf>
+__device__ __forceinline__ void follow(f4 (&z)[4], State& st) {
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        x[j] = z[j / 4][j % 4];
-        if (kMask && key0 + j >= seen) x[j] = -INFINITY;
-        top = fmaxf(top, x[j]);
+    for (int j = 0; j < 16; ++j) top = fmaxf(top, z[j / 4][j % 4]);
+    if constexpr (kHalf) {
+        // some lane above, or a column none of whose lanes is high enough
+        uint64_t fine = __builtin_amdgcn_ballot_w64(top >= st.low);
+        fine |= fine >> 32;
+        fine |= fine >> 16;
+        if (__builtin_amdgcn_ballot_w64(top > st.high) | (~fine & 0xffffu)) {
+            const float col_top = rows_max(top);
+            // (down no further than kDrop below the top)
+            const float by = fmaxf(col_top - kSet, fminf(fmaxf(st.top - st.m, col_top) - kDrop, 0.f));
+            st.move(col_top > -INFINITY && (col_top > st.high || (col_top < st.low && by < 0.f)), col_top, by, z);
+        }
+    } else {
+        if (__builtin_amdgcn_ballot_w64(top > st.high - (kHigh - kLazy))) {
+            const float col_top = rows_max(top);
+            st.move(col_top > st.high - (kHigh - kLazy), col_top, col_top, z);
+        }
     }
-    if (__builtin_amdgcn_ballot_w64(top > st.limit)) {       // rare
-        const float col_top = rows_max(top);
-        const bool moves = col_top > st.limit, first = st.limit == -INFINITY;
-        const float to = moves ? col_top : st.m;
-        const float corr = first ? 0.f : __builtin_amdgcn_exp2f(st.m - to);
-        st.m = to;
-        st.limit = moves ? to + kLazy : st.limit;
-        st.l *= corr;
+}
+
+// Weights; nan: tokens of the lane's page whose value is NaN (bit per token; bf16 tiles only).
+template <bool kHalf>
+__device__ __forceinline__ void weights(const f4 (&z)[4], uint32_t nan, float (&e)[2][8]) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d) st.acc[d] *= corr;
-    }
-    float e[2][8];
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        e[j / 8][j % 8] = __builtin_amdgcn_exp2f(x[j] - st.m);
-        sum[j / 4] += e[j / 8][j % 8];
-    }
-    if (__builtin_amdgcn_ballot_w64(nan != 0))               // rare: a seen value that is NaN makes the row NaN
+    for (int j = 0; j < 16; ++j) e[j / 8][j % 8] = __builtin_amdgcn_exp2f(z[j / 4][j % 4]);
+    if (!kHalf && __builtin_amdgcn_ballot_w64(nan != 0))     // a seen value that is NaN makes the row NaN
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            if ((nan >> j & 1) && key0 + j < seen) e[j / 8][j % 8] = __builtin_nanf("");
-    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    split_bf16(e[0], p[0]);
-    split_bf16(e[1], p[1]);
+            if ((nan >> j & 1) && z[j / 4][j % 4] > -INFINITY) e[j / 8][j % 8] = __builtin_nanf("");
+}
+
+__device__ __forceinline__ float sum_of(const float (&e)[2][8]) {
+    float sum[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = (e[0][j] + e[0][4 + j]) + (e[1][j] + e[1][4 + j]);
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // ---- few columns ----
@@ -275,55 +397,81 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
 #pragma unroll
         for (int b = 0; b < 4; ++b) vr[b] = page_load<kOnce>(v_at + kQ4VOff + 256 * b + 16 * c);
     };
+    f4 x[NB][8];               // the queries first: they have come when the first pages are on their way
+    int seen[NB];              // keys that the column sees
+#pragma unroll
+    for (int b = 0; b < NB; ++b) load_q(a, p.s, kvh, 16 * b + c, x[b], seen[b]);
     if (t0 < t1) {
         load_k(t0);
         load_v();
     }
     QTerms q[NB];
-    int seen[NB];              // keys that the column sees
     State st[NB];
+    Window win;
+    win.clear();
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        load_q(a, p.s, kvh, 16 * b + c, q[b], seen[b]);
+        q_terms(x[b], q[b]);
         st[b].clear();
     }
     auto step = [&](auto mask_tag, int t) {
         constexpr bool kMask = decltype(mask_tag)::value;
         const int key0 = t * TILE + 16 * g;
-        uint32_t ex = (uint32_t)ve, nan = 0;                 // the lane's: tokens 4 (c & 3) .. of block c >> 2
+        uint32_t ex = (uint32_t)ve;                          // the lane's: tokens 4 (c & 3) .. of block c >> 2
         if (kMask) {                                         // a slot behind the last key may hold anything
             const int rest = p.s.keys - key0 - 4 * (c & 3);
-            ex = rest >= 4 ? ex : rest <= 0 ? 0u : ex & ((1u << (8 * rest)) - 1u);
+            const uint32_t keep = rest >= 4 ? ~0u : rest <= 0 ? 0u : (1u << (8 * rest)) - 1u;
+            ex = (ex & keep) | (win.fill & ~keep);
         }
-        if (__builtin_amdgcn_ballot_w64(maybe_255(ex) != 0)) {               // rare
-            const uint32_t m = bytes_255(ex);
-            ex &= ~(m * 255u);                               // the value counts through its weight instead
-            nan = ((m & 1u) | (m >> 7 & 2u) | (m >> 14 & 4u) | (m >> 21 & 8u)) << (4 * (c & 3));
+        auto rest = [&](auto half_tag, uint32_t nan) {
+            constexpr bool kHalf = decltype(half_tag)::value;
+            constexpr int kN = kParts<kHalf>;
+            u4 w[NB][2][kN];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                f4 z[4];
+                float e[2][8];
+                scores(kr, q[b], ke, st[b].m, z);
+                if (kMask) hide(z, key0, seen[b]);
+                follow<kHalf>(z, st[b]);
+                weights<kHalf>(z, nan, e);
+                st[b].l += sum_of(e);
+                split<kHalf>(e[0], w[b][0]);
+                split<kHalf>(e[1], w[b][1]);
+            }
+            const bool more = t + 1 < t1;
+            if (more) load_k(t + 1);
+            each<4>([&](auto b) {
+                constexpr int kB = b;
+                uint32_t e[4];
+                each<4>([&](auto i) { e[i] = __float_as_uint(row_lane<4 * kB + i>(__uint_as_float(ex))); });
+                each<2>([&](auto h) {
+                    u4 lower, upper;
+                    values_of<kHalf>((uint32_t)vr[b][2 * h], (uint32_t)vr[b][2 * h + 1], e[2 * h], e[2 * h + 1], lower, upper);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int k = kN - 1; k >= 0; --k) {
+                            st[n].acc[2 * b] = add_up<kHalf>(lower, w[n][h][k], st[n].acc[2 * b]);
+                            st[n].acc[2 * b + 1] = add_up<kHalf>(upper, w[n][h][k], st[n].acc[2 * b + 1]);
+                        }
+                });
+            });
+            if (more) load_v();
+        };
+        bool half = !win.closed && __builtin_amdgcn_ballot_w64(win.outside(ex) != 0) == 0;
+        uint32_t nan = 0;
+        if (!half) {                                         // rare: another window, or none
+            nan = take_nan(ex) << (4 * (c & 3));
+            int least = 255, most = 0;
+            byte_range(ex, least, most);
+            wave_range(least, most);
+            half = win.move(least, most);                    // (not with NaN in it, whose bytes are 0 now)
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) nan |= (uint32_t)__shfl_xor((int)nan, o, 64);
         }
-        b8 w[NB][2][3];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) weigh<kMask>([&](int u) { return kr[u]; }, q[b], ke, key0, seen[b], nan, st[b], w[b]);
-        const bool more = t + 1 < t1;
-        if (more) load_k(t + 1);
-        each<4>([&](auto b) {
-            constexpr int kB = b;
-            uint32_t e[4];
-            each<4>([&](auto i) { e[i] = __float_as_uint(row_lane<4 * kB + i>(__uint_as_float(ex))); });
-            each<2>([&](auto h) {
-                b8 lower, upper;
-                values_bf16((uint32_t)vr[b][2 * h], (uint32_t)vr[b][2 * h + 1], e[2 * h], e[2 * h + 1], lower, upper);
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int k = 2; k >= 0; --k) {
-                        st[n].acc[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lower, w[n][h][k], st[n].acc[2 * b], 0, 0, 0);
-                        st[n].acc[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(upper, w[n][h][k], st[n].acc[2 * b + 1], 0, 0, 0);
-                    }
-            });
-        });
-        if (more) load_v();
+        if (half) rest(std::true_type{}, 0u);
+        else rest(std::false_type{}, nan);
     };
     const int t_clear = max(min(t1, clear_keys / TILE), t0);
     for (int t = t0; t < t_clear; ++t) step(std::false_type{}, t);
@@ -375,29 +523,28 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
 
 // ---- many columns ----
 
-// Each wave has its own 16 columns of a group, and all go over the same keys: V's
-// conversion to bf16 is done once for 64 columns, and a tile's loads once.  Wave w brings
-// page w of a tile through its registers to LDS: K's codes and exponents as they are (pages
-// 64 B further apart than they are long, so that the operand reads are free of bank
-// conflicts), V as bf16 in operand order, two tiles of everything.  A tile's loads go out
-// at the start of the tile before it; one barrier per tile.
+// Each wave has its own 16 columns of a group, and all go over the same keys.  A wave takes K
+// from the pages to its registers (the four of a workgroup find it in the caches), so its scores and
+// weights wait for nobody; V's conversion is done once for 64 columns: wave w turns page w of a
+// tile into fp16 (or bf16) in operand order in LDS, two tiles of it.  A tile's loads go out
+// while the one before it is worked on; one barrier per tile, between the weights and the products
+// that they go into.  All waves see the exponents of the whole tile, so they agree on
+// its type without a word.
 __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
     constexpr int COLS = kManyCols;
-    constexpr int kPageLds = kQ4KBytes + 64, kStage = kTilePages * kPageLds;
     constexpr int kOut = 16 * kAccRow * 4;                   // a block's results, per wave
     constexpr int kVTile = 2 * DB * 1024;
     static_assert(kTilePages == WAVES, "a page per wave");
-    static_assert(WAVES * kOut <= 2 * kStage + 2 * kVTile, "the results overwrite the tiles");
-    __shared__ __attribute__((aligned(16))) unsigned char s_mem[2 * kStage + 2 * kVTile];
-    __shared__ int s_ke[2][kTilePages][16];                  // K exponents
-    __shared__ uint32_t s_nan[2][kTilePages];                // tokens whose value is NaN
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int g = lane >> 4, c = lane & 15;
+    constexpr int kMem = WAVES * kOut > 2 * kVTile ? WAVES * kOut : 2 * kVTile;      // the results overwrite the tiles
+    __shared__ __attribute__((aligned(16))) unsigned char s_mem[kMem];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x, w = blockIdx.y;
 
     Place at, to;
     find_stretch(a, w, at, to);
     i4 piece[2] = {i4{-1, 0, 0, 0}, i4{-1, 0, 0, 0}};        // the group begun before this stretch; the one it leaves open
+    Window win;
+    win.clear();
     for (;;) {
         if (at.sess >= a.n_sess || at.sess > to.sess ||
             (at.sess == to.sess && (at.group > to.group || (at.group == to.group && at.tile >= to.tile))))
@@ -409,6 +556,11 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
             at = Place{at.sess + 1, 0, 0};
             continue;
         }
+        // (a lane number that is new for each group: what is made of it is made again, and not kept
+        // in registers that the tiles need, or behind them in memory)
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));
+        const int g = lane >> 4, c = lane & 15;
         const int sess = at.sess, group = at.group;
         const int tiles = __builtin_amdgcn_readfirstlane(group_tiles(s, group));
         const int t_lo = __builtin_amdgcn_readfirstlane(at.tile);
@@ -421,103 +573,169 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
         const int t1 = __builtin_amdgcn_readfirstlane(min(t_hi, (wave_keys + TILE - 1) / TILE));   // this wave's last tile
         const int t_clear = __builtin_amdgcn_readfirstlane(min(s.past + col0 / G + 1, s.keys) / TILE);   // tiles below: seen by all its columns
 
-        // ---- a tile's way into LDS ----
-        const int32_t* table = a.tables + sess * a.table_stride;
-        const int last_page = (s.keys - 1) >> kKvBlockShift;
-        int win = -64, held = 0;                             // 64 table entries from `win` on
-        i4 kr, vr, ve;
+        // ---- a tile's way to the wave ----
+        Pages pages(a, sess, s.keys);
+        const uint8_t* const head = a.pool + kvh * kQ4Rec;
+        i4 kr[4], vr, ve;                                    // K of the tile; V of page `wave` and its exponents of block g
         int ke = 0;
-        auto load = [&](int t) {                             // page `wave` of tile t
+        uint32_t vx = 0;                                     // V's exponents of the tile: page c >> 2, block g, tokens 4 (c & 3) ..
+        struct Where {
+            int lane, wave;                                  // pages of the pool: c >> 2 of a tile, and `wave`
+        };
+        auto where = [&](int t) {
             const int pg = t * kTilePages;
-            if (pg + kTilePages > win + 64) {
-                win = pg;
-                held = table[min(pg + lane, last_page)];
-            }
-            const int e = __builtin_amdgcn_readlane(held, min(pg + wave, last_page) - win);
-            const int phys = (unsigned)e < (unsigned)a.nb ? e : 0;           // an entry outside the pool reads page 0
-            const uint8_t* rec = a.pool + phys * kQ4Page + kvh * kQ4Rec;
-            kr = *reinterpret_cast<const i4*>(rec + 16 * lane);
+            pages.reach(pg);
+            const int own = __builtin_amdgcn_readlane(pages.held, min(pg + wave, pages.last) - pages.win);
+            return Where{pages[pg + (c >> 2)], (unsigned)own < (unsigned)a.nb ? own : 0};
+        };
+        auto load_v = [&](const Where& at) {
+            const uint8_t* rec = head + at.wave * kQ4Page;
             vr = *reinterpret_cast<const i4*>(rec + kQ4VOff + 16 * lane);
-            ve = *reinterpret_cast<const i4*>(rec + kQ4VeOff + 16 * g);      // block g's exponents of the page's tokens
-            ke = *reinterpret_cast<const int*>(rec + kQ4KeOff + 4 * c);
+            ve = *reinterpret_cast<const i4*>(rec + kQ4VeOff + 16 * g);
+            vx = *reinterpret_cast<const uint32_t*>(head + at.lane * kQ4Page + kQ4VeOff + g * 16 + (c & 3) * 4);
         };
-        auto put = [&](int t) {                              // lane (g, c): dims 32 g + c and 32 g + 16 + c
-            *reinterpret_cast<i4*>(s_mem + (t & 1) * kStage + wave * kPageLds + 16 * lane) = kr;
-            if (lane < 16) s_ke[t & 1][wave][c] = ke;
-            const int rest = s.keys - t * TILE - 16 * wave;  // a slot behind the last key may hold anything
-            uint32_t nan = 0;
+        auto load_k = [&](const Where& at) {
+            const uint8_t* rec = head + at.lane * kQ4Page;
+            const uint8_t* k_at = rec + (c & 3) * 64 + g * 16;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t x = (uint32_t)ve[i];
-                if (rest < 16) x = rest >= 4 * i + 4 ? x : rest <= 4 * i ? 0u : x & ((1u << (8 * (rest - 4 * i))) - 1u);
-                nan |= maybe_255(x);
-                ve[i] = (int)x;
-            }
-            if (__builtin_amdgcn_ballot_w64(nan != 0)) {     // rare
-                nan = 0;
+            for (int u = 0; u < 4; ++u) kr[u] = *reinterpret_cast<const i4*>(k_at + 256 * u);
+            ke = *reinterpret_cast<const int*>(rec + kQ4KeOff + (c & 3) * 16 + g * 4);
+        };
+        // the exponents of tokens from..from + 3 with those of slots behind the last key, which
+        // may hold anything, replaced
+        auto cut = [&](uint32_t x, int from) {
+            const int rest = s.keys - from;
+            const uint32_t keep = rest >= 4 ? ~0u : rest <= 0 ? 0u : (1u << (8 * rest)) - 1u;
+            return (x & keep) | (win.fill & ~keep);
+        };
+        // V of a tile in operand order, lane (g, c) dims 32 g + c and 32 g + 16 + c of page `wave`; to LDS
+        auto turn = [&](auto half_tag, u4 (&v)[2][2]) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t m = bytes_255((uint32_t)ve[i]);
-                    ve[i] &= (int)~(m * 255u);               // the value counts through its weight instead
-                    nan |= ((m & 1u) | (m >> 7 & 2u) | (m >> 14 & 4u) | (m >> 21 & 8u)) << (4 * i);
+            for (int h = 0; h < 2; ++h)
+                values_of<decltype(half_tag)::value>((uint32_t)vr[2 * h], (uint32_t)vr[2 * h + 1], (uint32_t)ve[2 * h],
+                                                     (uint32_t)ve[2 * h + 1], v[0][h], v[1][h]);
+        };
+        auto write_v = [&](const u4 (&v)[2][2], int t) {
+            unsigned char* dst = s_mem + (t & 1) * kVTile + g * 4096 + (16 * wave + c) * 16;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) *reinterpret_cast<u4*>(dst + x * 2048 + h * 1024) = v[x][h];
+        };
+        uint32_t nan = 0;                                    // tokens of page g whose value is NaN
+        // the same for any tile; true: in fp16
+        auto put = [&](int t) {
+            uint32_t x = cut(vx, t * TILE + 16 * (c >> 2) + 4 * (c & 3));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ve[i] = (int)cut((uint32_t)ve[i], t * TILE + 16 * wave + 4 * i);
+            bool half = !win.closed && __builtin_amdgcn_ballot_w64(win.outside(x) != 0) == 0;
+            nan = 0;
+            if (!half) {                                     // another window, or none
+                const uint32_t m = take_nan(x) << (4 * (c & 3));
+                int least = 255, most = 0;
+                byte_range(x, least, most);
+                wave_range(least, most);
+                half = win.move(least, most);                // (not with NaN in it, whose bytes are 0 now)
+                if (__builtin_amdgcn_ballot_w64(m != 0)) {
+                    nan = m;
+                    nan |= (uint32_t)__shfl_xor((int)nan, 1, 64);
+                    nan |= (uint32_t)__shfl_xor((int)nan, 2, 64);
+                    nan |= (uint32_t)__shfl_xor((int)nan, 16, 64);
+                    nan |= (uint32_t)__shfl_xor((int)nan, 32, 64);
+                    nan = (uint32_t)__shfl((int)nan, 4 * g, 64);             // page c >> 2 -> page g
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t y = (uint32_t)ve[i];
+                        (void)take_nan(y);
+                        ve[i] = (int)y;
+                    }
                 }
-                nan |= (uint32_t)__shfl_xor((int)nan, 16, 64);
-                nan |= (uint32_t)__shfl_xor((int)nan, 32, 64);
             }
-            if (lane == 0) s_nan[t & 1][wave] = nan;
-            unsigned char* dst = s_mem + 2 * kStage + (t & 1) * kVTile + g * 4096 + (16 * wave + c) * 16;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                b8 lower, upper;
-                values_bf16((uint32_t)vr[2 * h], (uint32_t)vr[2 * h + 1], (uint32_t)ve[2 * h], (uint32_t)ve[2 * h + 1], lower, upper);
-                *reinterpret_cast<b8*>(dst + h * 1024) = lower;
-                *reinterpret_cast<b8*>(dst + 2048 + h * 1024) = upper;
-            }
+            u4 v[2][2];
+            if (half) turn(std::true_type{}, v);
+            else turn(std::false_type{}, v);
+            write_v(v, t);
+            return half;
         };
-        load(t_lo);
+        // the wave's LDS accesses are done; loads in flight stay there
+        auto barrier = [&] {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
         QTerms q;
         int seen;
         State st;
-        load_q(a, s, kvh, col0 + c, q, seen);
-        st.clear();
-        put(t_lo);
-        __syncthreads();
-        const uint32_t k_off = (uint32_t)((c >> 2) * kPageLds + (c & 3) * 64 + g * 16);
-        auto tile = [&](auto mask_tag, int t) {
-            constexpr bool kMask = decltype(mask_tag)::value;
-            const unsigned char* k_at = s_mem + (t & 1) * kStage + k_off;
-            const unsigned char* v_at = s_mem + 2 * kStage + (t & 1) * kVTile + 16 * lane;
-            b8 p[2][3];
-            weigh<kMask>([&](int u) { return *reinterpret_cast<const i4*>(k_at + 256 * u); }, q, s_ke[t & 1][c >> 2][4 * (c & 3) + g],
-                         t * TILE + 16 * g, seen, s_nan[t & 1][g], st, p);
+        const Where start = where(t_lo);
+        {
+            f4 x[8];
+            load_q(a, s, kvh, col0 + c, x, seen);
+            load_v(start);
+            load_k(start);
+            q_terms(x, q);
+            st.clear();
+        }
+        // One tile: its scores and weights, then the barrier that V waits for, then its
+        // products.  True: V of the next tile is in LDS as well, in fp16 (what almost all are).
+        // (Behind the last tile the same once more: no branch, so that the registers stay where
+        // they are.)
+        auto tile = [&](auto half_tag, int t) {
+            constexpr bool kHalf = decltype(half_tag)::value;
+            constexpr int kN = kParts<kHalf>;
+            const Where next = where(min(t + 1, t_hi - 1));
+            load_v(next);
+            f4 z[4];
+            float e[2][8];
+            scores(kr, q, ke, st.m, z);
+            __builtin_amdgcn_sched_barrier(0);               // K's registers are free now
+            __builtin_amdgcn_s_setprio(1);                   // vector work goes first: the other workgroup's products run beside it
+            load_k(next);
+            if (t >= t_clear) hide(z, t * TILE + 16 * g, seen);
+            follow<kHalf>(z, st);
+            weights<kHalf>(z, nan, e);
+            st.l += sum_of(e);
+            __builtin_amdgcn_s_setprio(0);
+            barrier();
+            const unsigned char* v_at = s_mem + (t & 1) * kVTile + 16 * lane;
+            u4 p[2][kN];
+            split<kHalf>(e[0], p[0]);
+            split<kHalf>(e[1], p[1]);
 #pragma unroll
             for (int d = 0; d < DB; d += 2) {                // two 16-dim blocks, two halves of their tokens
-                b8 v[2][2];
+                u4 v[2][2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) v[x][h] = *reinterpret_cast<const b8*>(v_at + 1024 * (2 * (d + x) + h));
+                    for (int h = 0; h < 2; ++h) v[x][h] = *reinterpret_cast<const u4*>(v_at + 1024 * (2 * (d + x) + h));
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int k = 2; k >= 0; --k)
+                    for (int k = kN - 1; k >= 0; --k)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            st.acc[d + x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[x][h], p[h][k], st.acc[d + x], 0, 0, 0);
+                        for (int x = 0; x < 2; ++x) st.acc[d + x] = add_up<kHalf>(v[x][h], p[h][k], st.acc[d + x]);
             }
+            // (the last tile, whose page may end behind the last key, goes the other way)
+            if (!kHalf || t + 1 >= t1 || (t + 2) * TILE > s.keys || __builtin_amdgcn_ballot_w64(win.outside(vx) != 0) != 0)
+                return false;
+            u4 w[2][2];
+            turn(std::true_type{}, w);
+            write_v(w, t + 1);
+            return true;
         };
-        // every wave goes through all tiles of the stretch, for its page of them and the
-        // barrier; its own columns need the first ones, up to t_clear without a mask
-        auto round = [&](int t, auto&& compute) {
-            if (t + 1 < t_hi) load(t + 1);
-            compute();
-            if (t + 1 < t_hi) put(t + 1);
-            __syncthreads();
-        };
-        int t = t_lo;
-        for (; t < min(t1, t_clear); ++t) round(t, [&] { tile(std::false_type{}, t); });
-        for (; t < t1; ++t) round(t, [&] { tile(std::true_type{}, t); });
-        for (; t < t_hi; ++t) round(t, [] {});
+        // Every wave goes through all tiles of the stretch, for its page of them and the
+        // barrier; its own columns need the first ones, up to t_clear without a mask.
+        for (int t = t_lo; t < t_hi; ++t) {
+            const bool half = put(t);
+            if (t < t1 && half) {
+                while (tile(std::true_type{}, t)) ++t;
+            } else if (t < t1) {
+                tile(std::false_type{}, t);
+            } else {
+                load_v(where(min(t + 1, t_hi - 1)));
+                barrier();
+            }
+        }
+        barrier();                                           // all waves are past their products
 
         // results through LDS (every wave is past its tiles), rows in address order:
         // the output, or a piece of a group that others have the rest of
@@ -525,10 +743,11 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
         const int slot = 2 * w + (t_lo > 0 ? 0 : 1);
         if (!whole) piece[t_lo > 0 ? 0 : 1] = i4{sess, group, t_hi == tiles, min(n_cols - group * COLS, COLS)};
         unsigned char* mine = s_mem + wave * kOut;
+        asm volatile("" : "+v"(lane));
         if (col0 < n_cols) {
             const float l = rows_sum(st.l), m = st.reference();
 #pragma unroll
-            for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(mine + (c * kAccRow + 16 * d + 4 * g) * 4) = st.acc[d];
+            for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(mine + ((lane & 15) * kAccRow + 16 * d + 4 * (lane >> 4)) * 4) = st.acc[d];
             wave_lds_sync();
 #pragma unroll
             for (int e = 0; e < 16 * (HD / 4) / 64; ++e) {
@@ -546,7 +765,7 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
                 }
             }
         }
-        __syncthreads();                                     // the next group's tiles come where the results were
+        barrier();                                           // the next group's tiles come where the results were
     }
     if (kvh == 0 && tid < 2) a.info[2 * w + tid] = tid ? piece[1] : piece[0];
 }

@@ -42,6 +42,18 @@
 #include <cstdint>
 #include <type_traits>
 
+namespace nova {
+namespace {
+// Many columns, 12 prompts of up to 300 tokens (1.5B) / 8 x 512 tokens behind up to
+// 4096 (7B), us.  Fewest tiles of a piece of a group: 2 37.3 / 266, 3 36.0 / 266, 4 39.0 / 272.
+constexpr int kMinPiece = 3;
+// What a group costs beside its tiles, in tiles: 0 43.2 / 277, 2 36.6 / 276, 4 39.0 / 272,
+// 8 35.7 / 279 with pieces of 4; short sessions need it most (8 of 19 rows, 7B: 0 135, 2 17.6,
+// 4 11.8, 8 12.0), as a workgroup is given several of them.
+constexpr int kGroupTiles = 4;
+}  // namespace
+}  // namespace nova
+
 #include "attn_ragged.h"
 #include "check.h"
 #include "kv_q8.h"

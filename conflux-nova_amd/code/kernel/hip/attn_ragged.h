@@ -8,7 +8,9 @@
 // work leaves {reference m, sum of 2^(s - m)} and the weighted sum of values per column in
 // the workspace.
 //
-// Everything here has internal linkage: each format's source compiles its own.
+// Everything here has internal linkage: each format's source compiles its own, with its own
+// kMinPiece (many columns: fewest tiles of a piece of a group) and kGroupTiles (what a group
+// costs beside its tiles, in tiles), defined before this header.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <algorithm>
@@ -37,13 +39,6 @@ constexpr int kTilePages = TILE / kKvBlock;
 // Workgroups aimed at: two per CU.  (Of the form with two blocks of columns one runs per
 // CU, as it takes the registers of both, so its parts go through in two rounds.)
 constexpr int kAimWgs = 512;
-// Many columns, 12 prompts of up to 300 tokens (1.5B) / 8 x 512 tokens behind up to
-// 4096 (7B), us.  Fewest tiles of a piece of a group: 2 37.3 / 266, 3 36.0 / 266, 4 39.0 / 272.
-constexpr int kMinPiece = 3;
-// What a group costs beside its tiles, in tiles: 0 43.2 / 277, 2 36.6 / 276, 4 39.0 / 272,
-// 8 35.7 / 279 with pieces of 4; short sessions need it most (8 of 19 rows, 7B: 0 135, 2 17.6,
-// 4 11.8, 8 12.0), as a workgroup is given several of them.
-constexpr int kGroupTiles = 4;
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
 constexpr float kUnset = -3.40282347e38f;      // reference of a column without keys, where states are joined: below every other

@@ -140,7 +140,10 @@ def attention(q, k, v, first, group):
     row sees.  Weights are fp32 numbers relative to a reference that is at most the row's
     largest score, so one below 2^-126 of the largest is no normal number and may count as 0
     (as its product with a value may, and once more where pieces are joined): each of
-    n keys then adds up to 2^-125 of the largest |v|."""
+    n keys then adds up to 2^-125 of the largest |v|.  A weight in fp16 terms is cut below 2^-24
+    where the largest of its tile (64 keys from a multiple of 64) stands at 2^2 or more, so it
+    loses up to 2^-26 of that one, or, where the reference has come down by its 80 octaves,
+    2^-102 of the row's largest."""
     n, nh, _ = q.shape
     out, tol = np.zeros((n, nh, HD)), np.zeros((n, nh, HD))
     if len(k) == 0:
@@ -159,7 +162,10 @@ def attention(q, k, v, first, group):
         out[:, h] = p @ vz
         e = 2.0 ** -20 * np.where(seen, size, 0).max(-1) + 2.0 ** -20 + (3 * len(kh) / 32 + 64) * 2.0 ** -24
         most = np.where(seen, np.abs(vz).max(-1), 0).max(-1)
-        tol[:, h] = 2 * e[:, None] * (p @ np.abs(vz)) + (seen.sum(-1) * 2.0 ** -125 * most)[:, None]
+        tiles = np.arange(len(kh)) // 64
+        tops = np.stack([p[:, tiles == t].max(-1) for t in range(tiles[-1] + 1)], -1)[:, tiles] * seen
+        tol[:, h] = (2 * e[:, None] * (p @ np.abs(vz)) + 2.0 ** -26 * (tops @ np.abs(vz)) +
+                     (seen.sum(-1) * (2.0 ** -125 + 2.0 ** -102) * most)[:, None])
     return out, tol
 
 

@@ -271,7 +271,7 @@ def test_large_keys_and_small_queries(rows, decode, power):
 @pytest.mark.parametrize("rows,decode", FORMS)
 def test_scores_of_any_size(rows, decode, keys, sign):
     """Scores of 2^90 to 2^113, key j's 1, 1.5, 1, 1.5 .. and twice that every eighth key: the largest
-    (or the first) take everything, and a row's result is the mean of their values."""
+    (or the first) take everything, and a row's result lies between their values."""
     keys = max(keys, rows)
     c = _call([keys], rows, decode, seed=6)
     p = c.parts()
@@ -289,10 +289,13 @@ def test_scores_of_any_size(rows, decode, keys, sign):
         m = keys if decode else int(c.past[0]) + r + 1
         s = c.q[r, 0].astype(np.float64) @ k[:m, 0].T
         best = np.flatnonzero(s == s.max())                  # alike: the same codes and powers
-        want = np.repeat(v[best].mean(0), c.nova.group, 0)
-        size = np.repeat(np.abs(v[best]).mean(0), c.nova.group, 0)
-        # equal weights, their sum and its reciprocal
-        assert (np.abs(got[r] - want) <= (len(best) / 32 * 3 + 64) * 2.0 ** -23 * size).all(), r
+        # A score of 2^113 in fp32, added up in five steps of 2^-23 of it, is off by up to 2^93, and less
+        # the reference it is a number of that size: of keys that are alike by their codes, in tiles
+        # with another reference, any may take any part of the whole.  The others' scores are a
+        # sixteenth and more below, 2^104: they take nothing.
+        lo, hi = (np.repeat(f(v[best], axis=0), c.nova.group, 0) for f in (np.min, np.max))
+        slack = 2.0 ** -20 * np.repeat(np.abs(v[best]).max(0), c.nova.group, 0)
+        assert ((got[r] >= lo - slack) & (got[r] <= hi + slack)).all(), r
 
 
 def test_the_same_every_time():
@@ -384,3 +387,79 @@ def test_beyond_32_bit_offsets():
     assert_within(o.numpy(q.shape, np.float32), ref, tol, "chunk")
     ref, tol = attention(q[:1], kk, vv, n, nova.group)
     assert_within(o1.numpy(q[:1].shape, np.float32), ref, tol, "decode")
+
+
+@pytest.mark.parametrize("rows,decode", FORMS)
+@pytest.mark.parametrize("spread", [7, 8, 30])
+def test_value_powers_within_a_tile(rows, decode, spread):
+    """powers that lie a window apart, one more, and far apart, in some tiles or all"""
+    c = _call([700, 333], rows, decode, seed=11, scale=0.5)
+    p = c.parts()
+    rng = np.random.default_rng(spread)
+    p[3] = (120 + rng.integers(0, spread + 1, p[3].shape)).astype(np.uint8)
+    some = c.table[0, 8:20]
+    p[3][some] = 126
+    c.set_parts(p)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("rows,decode", FORMS)
+@pytest.mark.parametrize("powers", [(-40, 0, 40), (-100, -20, -100, 13, -14, 90), (14, 10, 14, 13, 12, -23, -24)])
+def test_value_powers_change_between_tiles(rows, decode, powers):
+    """every two tiles of another size: in fp16's reach and past it, up and down"""
+    c = _call([64 * 2 * len(powers) * 3 + 5], rows, decode, seed=12, scale=0.02)
+    p = c.parts()
+    n = c.table.shape[1] - 3
+    for i in range(n):
+        p[3][c.table[0, i]] = 127 + powers[i // 8 % len(powers)] - (np.arange(4) % 2)
+    c.set_parts(p)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("rows,decode", FORMS)
+@pytest.mark.parametrize("size", [3.0, 20.0, 80.0, 200.0])
+@pytest.mark.parametrize("first", ["high", "low", "by turns"])
+def test_scores_rise_and_fall_between_tiles(rows, decode, size, first):
+    """tiles whose scores lie `size` apart, so that the reference goes up and down, and values of the
+    tiles with the high scores that are zero in half of the dims: the other tiles' count there"""
+    c = _call([64 * 14 + 9], rows, decode, seed=13, scale=0.3)
+    p = c.parts()
+    u = np.where(np.arange(HD) % 3 == 0, 1.0, -1.0).astype(np.float32)
+    c.q += 2 * u - (c.q @ u)[..., None] * u / HD
+    rng = np.random.default_rng(3)
+    for i in range(c.table.shape[1] - 3):
+        tile = i // 4
+        up = {"high": tile < 3, "low": tile >= 11, "by turns": tile % 3 == 0}[first]
+        x = rng.standard_normal((c.nova.nkv, KB, HD)).astype(np.float32) * 0.1
+        if up:
+            x += u * np.float32(size * np.sqrt(HD) / (2 * HD))
+            p[2][c.table[0, i], :, :, ::2] = 0
+        p[0][c.table[0, i]], p[1][c.table[0, i]] = quantise(x)
+    c.set_parts(p)
+    c.upload()
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("rows,decode", FORMS)
+def test_zero_and_nan_blocks_in_some_tiles(rows, decode):
+    """blocks of zeros among others, a NaN row that is hidden from half of the rows, huge values after it"""
+    c = _call([600 + rows], rows, decode, seed=14, scale=0.5)
+    p = c.parts()
+    p[3][c.table[0, 5], :, 3, 1], p[2][c.table[0, 5], :, 3, 32:64] = 0, 0
+    p[3][c.table[0, 9:11]], p[2][c.table[0, 9:11]] = 0, 0
+    p[3][c.table[0, 20], :, 2] = 200
+    hidden = 600 + rows // 2
+    if rows > 1:
+        p[3][c.table[0, hidden // KB], 1, hidden % KB] = NAN
+    c.set_parts(p)
+    got = c.run()
+    k, v = values(c.pool.rec, c.table[0], 600 + rows)
+    ref, tol = attention(c.q[:rows], k, v, int(c.past[0]) + (0 if decode else 1), c.nova.group)
+    if rows > 1:
+        bad = np.isnan(got).reshape(rows, c.nova.nkv, -1)
+        assert bad[rows // 2:, 1].all() and not bad[:, 0].any() and not bad[:rows // 2].any()
+        got = np.where(np.isnan(got), ref, got)
+    assert_within(got, ref, tol, "zeros")
