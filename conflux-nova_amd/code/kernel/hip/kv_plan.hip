@@ -10,9 +10,11 @@
 // the result is the same every time.
 //
 // One workgroup does the sums (two passes over the sessions: what comes back, then what
-// fits) and, for a small step, all the rest.  Larger ones leave pages and rows to two
-// more launches over the whole chip, as the stack must be whole before pages are taken
-// from it.  Latency bounds all of it.
+// fits) and, for a small step, all the rest, out of registers and LDS.  Larger ones leave pages
+// and rows to two more launches over the whole chip, as the stack must be whole before
+// pages are taken from it.  It moves a few KB (16 sessions of a token each) to a MB, so latency
+// bounds all of it: 3.6 us for those 16, 11 us for 700 sessions and 60000 rows (3.4, 3.3 and 4.4),
+// where a launch that does nothing takes 2.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cstdint>
@@ -27,8 +29,15 @@ namespace {
 typedef int i4 __attribute__((ext_vector_type(4)));
 
 constexpr int PT = 1024;                       // threads of the workgroup that sums
+constexpr int kPlanWaves = PT / 64;
+constexpr uint32_t kNoneFits = ~0u;
+static_assert(kPlanWaves == 16, "a wave's sums in a row of 16 lanes");
 constexpr int FT = 256;                        // threads of the others
 constexpr int kOffsets = 4096;                 // sessions whose row offsets fit a workgroup's LDS
+// One launch up to this many rows and sessions.  One launch against three (us, one after another in a
+// graph, 31 pages held): 16 sessions of 1 row 3.7, 6.6; 64 of 32 6.9, 8.1; 256 of 8 6.6, 7.9; past it 16 of 256
+// 6.3, 7.7, but 256 of 16 15.0, 8.4 and 1000 of 1 10.4, 9.4.
+constexpr int kSmallRows = 2048, kSmallSessions = 256;
 
 struct PlanArgs {
     int32_t* tables;
@@ -59,41 +68,49 @@ __device__ __forceinline__ Wish wish(const PlanArgs& a, int i) {
     return w;
 }
 
-// inclusive sums over the workgroup, in thread order; `total` for all threads
+// Inclusive sums over the workgroup, in thread order; `total` for all threads.  They stop at
+// 2^32 - 1, past every number of rows or pages that there is room for.
 struct Pair {
-    int64_t a, b;
+    uint32_t a, b;
 };
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ void scan_step(uint32_t& v) {
+    v = __builtin_elementwise_add_sat(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, false));
+}
+__device__ __forceinline__ uint32_t scan16(uint32_t v) {     // over each 16 lanes
+    scan_step<0x111>(v);                                     // row_shr 1, 2, 4, 8
+    scan_step<0x112>(v);
+    scan_step<0x114>(v);
+    scan_step<0x118>(v);
+    return v;
+}
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {
+    v = scan16(v);
+    scan_step<0x142, 0xa>(v);                                // row 0 -> 1, 2 -> 3
+    scan_step<0x143, 0xc>(v);                                // rows 0, 1 -> 2, 3
+    return v;
+}
 __device__ __forceinline__ Pair block_scan(Pair v, Pair* s_wave, Pair& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t a = __shfl_up((long long)v.a, o, 64), b = __shfl_up((long long)v.b, o, 64);
-        if (lane >= o) {
-            v.a += a;
-            v.b += b;
-        }
-    }
-    __syncthreads();                                         // the last call's sums have been read
+    v.a = scan64(v.a);
+    v.b = scan64(v.b);
     if (lane == 63) s_wave[wave] = v;
     __syncthreads();
-    total = Pair{0, 0};
-#pragma unroll
-    for (int w = 0; w < PT / 64; ++w) {
-        const Pair p = s_wave[w];
-        if (w < wave) {
-            v.a += p.a;
-            v.b += p.b;
-        }
-        total.a += p.a;
-        total.b += p.b;
+    const Pair p = s_wave[lane & (kPlanWaves - 1)];
+    const uint32_t a = scan16(p.a), b = scan16(p.b);
+    total = Pair{(uint32_t)__builtin_amdgcn_readlane(a, kPlanWaves - 1), (uint32_t)__builtin_amdgcn_readlane(b, kPlanWaves - 1)};
+    if (wave > 0) {                                          // uniform
+        const int up = __builtin_amdgcn_readfirstlane(wave) - 1;
+        v.a = __builtin_elementwise_add_sat(v.a, (uint32_t)__builtin_amdgcn_readlane(a, up));
+        v.b = __builtin_elementwise_add_sat(v.b, (uint32_t)__builtin_amdgcn_readlane(b, up));
     }
     return v;
 }
 
 // the pages that sessions from..n_sess step by `step` give back, onto the stack; one wave
-__device__ __forceinline__ void give_back(const PlanArgs& a, int from, int step, int64_t avail, int64_t n_free) {
+__device__ __forceinline__ void give_back(const PlanArgs& a, const i4* info, int from, int step, int64_t avail, int64_t n_free) {
     for (int i = from; i < a.n_sess; i += step) {
-        const i4 in = a.info[i];
+        const i4 in = info[i];
         for (int p = in[0] + (int)(threadIdx.x & 63); p < in[1]; p += 64) {
             const int64_t at = avail - 1 - ((int64_t)in[2] + p - in[0]);
             if (at >= n_free) a.free_pages[at] = a.tables[i * a.stride + p];
@@ -104,15 +121,16 @@ __device__ __forceinline__ void give_back(const PlanArgs& a, int from, int step,
 __device__ __forceinline__ int taken(const PlanArgs& a, const i4& in, int64_t nth, int64_t avail) {
     return a.free_pages[avail - 1 - ((int64_t)in[3] + nth)];
 }
-__device__ __forceinline__ void hand_out(const PlanArgs& a, int from, int step, int64_t avail) {
+__device__ __forceinline__ void hand_out(const PlanArgs& a, const i4* info, const int32_t* keys, int from, int step, int64_t avail) {
     for (int i = from; i < a.n_sess; i += step) {
-        const i4 in = a.info[i];
-        const int last = (int)pages_of(a.keys[i]);
+        const i4 in = info[i];
+        const int last = (int)pages_of(keys[i]);
         for (int p = in[0] + (int)(threadIdx.x & 63); p < last; p += 64) a.tables[i * a.stride + p] = taken(a, in, p - in[0], avail);
     }
 }
 // position and slot of row r; off: the rows' offsets
-__device__ __forceinline__ void place_row(const PlanArgs& a, const int32_t* off, int r, int64_t avail) {
+__device__ __forceinline__ void place_row(const PlanArgs& a, const i4* info, const int32_t* past, const int32_t* off, int r,
+                                          int64_t avail) {
     int pos = -1;
     int64_t slot = -1;
     if (r < off[a.n_sess]) {
@@ -122,9 +140,9 @@ __device__ __forceinline__ void place_row(const PlanArgs& a, const int32_t* off,
             if (off[mid] <= r) lo = mid;
             else hi = mid - 1;
         }
-        pos = a.past[lo] + r - off[lo];
+        pos = past[lo] + r - off[lo];
         const int p = pos >> kKvBlockShift;
-        const i4 in = a.info[lo];
+        const i4 in = info[lo];
         const int page = p < in[0] ? a.tables[lo * a.stride + p] : taken(a, in, p - in[0], avail);
         if ((unsigned)page < (unsigned)a.nb) slot = (int64_t)page * kKvBlock + (pos & kKvBlockMask);
     }
@@ -132,80 +150,100 @@ __device__ __forceinline__ void place_row(const PlanArgs& a, const int32_t* off,
     a.slots[r] = slot;
 }
 
+// kAll: everything, for up to kSmallSessions sessions, whose numbers stay in registers and LDS
 template <bool kAll>
 __global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
-    __shared__ Pair s_wave[PT / 64];
-    __shared__ int32_t s_off[kAll ? kOffsets + 1 : 1];
+    constexpr int kKept = kAll ? kSmallSessions : 1;
+    __shared__ Pair s_wave[3][kPlanWaves];
+    __shared__ int32_t s_off[kKept + 1], s_past[kKept], s_keys[kKept];
+    __shared__ __attribute__((aligned(16))) i4 s_info[kKept];
     const int tid = threadIdx.x;
     const int64_t n_free = min(max((int64_t)*a.n_free, (int64_t)0), (int64_t)a.nb);
     // what comes back
     int64_t back = 0;
+    Wish w{0, 0, 0};
+    i4 in = i4{0, 0, 0, 0};
     for (int base = 0; base < a.n_sess; base += PT) {
         const int i = base + tid;
-        i4 in = i4{0, 0, 0, 0};
+        in = i4{0, 0, 0, 0};
         if (i < a.n_sess) {
-            const Wish w = wish(a, i);
+            w = wish(a, i);
             in[0] = (int)pages_of(w.keep);
             in[1] = (int)pages_of(w.have);
         }
         Pair total;
-        const Pair sum = block_scan(Pair{in[1] - in[0], 0}, s_wave, total);
+        const int of = base / PT & 1;                        // (the last call's sums may still be read)
+        const Pair sum = block_scan(Pair{(uint32_t)(in[1] - in[0]), 0}, s_wave[of], total);
         // (more than the stack holds is nowhere)
         in[2] = (int)min(back + sum.a - (in[1] - in[0]), (int64_t)a.nb);
-        if (i < a.n_sess) a.info[i] = in;
+        if (!kAll && i < a.n_sess) a.info[i] = in;
         back += total.a;
     }
     const int64_t avail = min(n_free + back, (int64_t)a.nb);
-    // what fits
-    Pair before{0, 0}, given{0, 0};                          // rows, pages: wished for; granted
+    // What fits: the sessions before the first with which the sums of what was wished for pass the room, so
+    // the sums up to a session that fits are those of what was granted.
+    int64_t rows_before = 0, pages_before = 0;               // wished for by the sessions of the passes before
+    Pair given{0, 0};                                        // rows, pages
+    if (!kAll) __syncthreads();                              // s_wave is used again
     for (int base = 0; base < a.n_sess; base += PT) {
         const int i = base + tid;
-        Wish w{0, 0, 0};
-        int64_t more = 0;
-        if (i < a.n_sess) {
-            w = wish(a, i);
-            more = pages_of(w.keep + w.add) - pages_of(w.keep);
-        }
+        const bool real = i < a.n_sess;
+        if (!kAll) w = real ? wish(a, i) : Wish{0, 0, 0};
+        const int64_t rows = min(w.add, (int64_t)a.max_rows + 1);            // one too many is as good as more
+        const int64_t more = pages_of(w.keep + rows) - pages_of(w.keep);
         Pair total;
-        const Pair sum = block_scan(Pair{w.add, more}, s_wave, total);
-        const bool fits = before.a + sum.a <= a.max_rows && before.b + sum.b <= avail;
-        if (i < a.n_sess) {
-            // sessions behind the first that does not fit get nothing, so the sums up to
-            // a session that fits are those of what was granted
-            const int64_t add = fits ? w.add : 0;
-            a.info[i][3] = fits ? (int)(before.b + sum.b - more) : 0;
+        const Pair sum = block_scan(Pair{(uint32_t)rows, (uint32_t)more}, s_wave[kAll ? 1 : 0], total);
+        const int64_t all_rows = rows_before + sum.a, all_pages = pages_before + sum.b;
+        const bool fits = all_rows <= a.max_rows && all_pages <= avail;
+        // what those that fit have together: with the wave's last of them, and the last wave's
+        const uint64_t hits = __builtin_amdgcn_ballot_w64(fits);
+        if (hits ? (tid & 63) == 63 - __builtin_clzll(hits) : (tid & 63) == 0)
+            s_wave[2][tid >> 6] = hits ? Pair{(uint32_t)all_rows, (uint32_t)all_pages} : Pair{kNoneFits, 0};
+        __syncthreads();
+        const Pair fit = s_wave[2][tid & (kPlanWaves - 1)];
+        const int fit_waves = __builtin_popcountll(__builtin_amdgcn_ballot_w64(fit.a != kNoneFits) & ((1u << kPlanWaves) - 1));
+        if (fit_waves > 0)
+            given = Pair{(uint32_t)__builtin_amdgcn_readlane(fit.a, fit_waves - 1),
+                         (uint32_t)__builtin_amdgcn_readlane(fit.b, fit_waves - 1)};
+        if (real) {
+            const int keys = (int)(w.keep + (fits ? rows : 0)), end = (int)(fits ? all_rows : given.a);
+            const int first = fits ? (int)(all_pages - more) : 0;
             a.past[i] = (int)w.keep;
-            a.keys[i] = (int)(w.keep + add);
+            a.keys[i] = keys;
+            a.row_off[i + 1] = end;
+            if constexpr (kAll) {
+                in[3] = first;
+                s_info[i] = in;
+                s_past[i] = (int)w.keep;
+                s_keys[i] = keys;
+                s_off[i + 1] = end;
+            } else a.info[i][3] = first;
         }
-        Pair all;
-        const Pair ok = block_scan(Pair{fits ? w.add : 0, fits ? more : 0}, s_wave, all);
-        if (i < a.n_sess) {
-            a.row_off[i + 1] = (int)(given.a + ok.a);
-            if (kAll) s_off[i + 1] = (int)(given.a + ok.a);
-        }
-        before.a += total.a;
-        before.b += total.b;
-        given.a += all.a;
-        given.b += all.b;
+        rows_before += total.a;
+        pages_before += total.b;
     }
     if (tid == 0) {
         a.row_off[0] = 0;
         if (kAll) s_off[0] = 0;
         *a.free_left = (int)(avail - given.b);
-        a.stack[0] = avail;
-        a.stack[1] = n_free;
+        if (!kAll) {
+            a.stack[0] = avail;
+            a.stack[1] = n_free;
+        }
     }
     if constexpr (kAll) {
         __syncthreads();
-        give_back(a, tid >> 6, PT / 64, avail, n_free);
-        __syncthreads();
-        hand_out(a, tid >> 6, PT / 64, avail);
-        for (int r = tid; r < a.max_rows; r += PT) place_row(a, s_off, r, avail);
+        if (back > 0) {                                      // uniform
+            give_back(a, s_info, tid >> 6, PT / 64, avail, n_free);
+            __syncthreads();
+        }
+        hand_out(a, s_info, s_keys, tid >> 6, PT / 64, avail);
+        for (int r = tid; r < a.max_rows; r += PT) place_row(a, s_info, s_past, s_off, r, avail);
     }
 }
 
 __global__ void __launch_bounds__(FT) plan_back_kernel(PlanArgs a) {
-    give_back(a, (int)(blockIdx.x * (FT / 64) + (threadIdx.x >> 6)), (int)gridDim.x * (FT / 64), a.stack[0], a.stack[1]);
+    give_back(a, a.info, (int)(blockIdx.x * (FT / 64) + (threadIdx.x >> 6)), (int)gridDim.x * (FT / 64), a.stack[0], a.stack[1]);
 }
 
 // workgroups below row_wgs: rows; the others: tables
@@ -214,19 +252,16 @@ __global__ void __launch_bounds__(FT) plan_rows_kernel(PlanArgs a, int row_wgs) 
     const int64_t avail = a.stack[0];
     if ((int)blockIdx.x >= row_wgs) {
         const int wgs = (int)gridDim.x - row_wgs;
-        hand_out(a, ((int)blockIdx.x - row_wgs) * (FT / 64) + (int)(threadIdx.x >> 6), wgs * (FT / 64), avail);
+        hand_out(a, a.info, a.keys, ((int)blockIdx.x - row_wgs) * (FT / 64) + (int)(threadIdx.x >> 6), wgs * (FT / 64), avail);
         return;
     }
     const bool here = a.n_sess <= kOffsets;
     if (here)
         for (int i = threadIdx.x; i <= a.n_sess; i += FT) s_off[i] = a.row_off[i];
     __syncthreads();
-    for (int r = blockIdx.x * FT + threadIdx.x; r < a.max_rows; r += row_wgs * FT) place_row(a, here ? s_off : a.row_off, r, avail);
+    for (int r = blockIdx.x * FT + threadIdx.x; r < a.max_rows; r += row_wgs * FT) place_row(a, a.info, a.past, here ? s_off : a.row_off, r, avail);
 }
 
-// One launch up to this many rows and sessions.
-constexpr int kSmallRows = 2048, kSmallSessions = 256;
-static_assert(kSmallSessions <= kOffsets, "offsets in LDS");
 constexpr int kWgs = 1024;                     // of the larger launches
 
 size_t info_at() { return 256; }

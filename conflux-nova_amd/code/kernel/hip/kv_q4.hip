@@ -33,7 +33,9 @@ namespace {
 constexpr int NH = Model::NH, NKV = Model::NKV, HD = Model::HD;
 constexpr int kLanes = 16;                     // lanes per token
 constexpr int QT = kKvBlock * kLanes;          // threads of a workgroup
+constexpr int kHeads = 4;                      // query heads of a workgroup
 static_assert(QT == 256 && kLanes * 8 == HD, "one page per workgroup, 8 dims per lane");
+static_assert(NH % kHeads == 0, "whole workgroups of query heads");
 
 struct StoreArgs : RowArgs {
     const float* q_in;         // RoPE: [n_rows][NH][HD]
@@ -82,11 +84,21 @@ __device__ __forceinline__ uint32_t v_byte(const uint32_t* token, int b, int r) 
     return ((token[at] >> sh) & 15u) | (((token[at + 2] >> sh) & 15u) << 4);
 }
 
-// grid: x = pages of the call (an upper bound), y = kv heads, then (RoPE) query heads
+// Workgroups of a page: its kv heads, then (RoPE) kHeads query heads each, one after another in the
+// grid, as their rows stand in memory.  Workgroups go round the 8 XCDs in turn, so a number
+// of units that 8 divides would give each XCD the same units of every page, kv heads to some and
+// query heads to others (7B, 4096 rows, one launch: 1, 2, 4, 8 heads: 44.1, 31.6, 32.1, 48.0 us, where 1
+// and 8 are such numbers; 4 heads in an order of all pages of a head first: 33.4).
+template <bool kRope>
+constexpr int kUnits = NKV + (kRope ? NH / kHeads : 0);
+static_assert(kUnits<true> % 8 != 0, "units spread over the XCDs");
+
+// grid: pages of the call (an upper bound) times kUnits
 template <bool kRope, RopeForm kForm>
 __global__ void __launch_bounds__(QT) q4_store_kernel(StoreArgs a) {
-    const PageItem it = page_item(a, blockIdx.x);
+    const PageItem it = page_item(a, blockIdx.x / kUnits<kRope>);
     if (it.sess < 0) return;
+    const int head = blockIdx.x % kUnits<kRope>;
     const int t = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
     const int pos = it.page * kKvBlock + t;
     const int first = max(it.pos0 - it.page * kKvBlock, 0);                   // tokens [first, last) of the page
@@ -94,15 +106,17 @@ __global__ void __launch_bounds__(QT) q4_store_kernel(StoreArgs a) {
     const bool real = t >= first && t < last;
     const int64_t row = it.row0 + pos - it.pos0;
     if constexpr (kRope) {
-        if ((int)blockIdx.y >= NKV) {                                        // a query head
+        if (head >= NKV) {                                        // query heads
             if (!real) return;
-            const int64_t at = (row * NH + blockIdx.y - NKV) * HD, angle = row * (a.rot / 2);
-            for (int u = j; u < rope_units<kForm>(a.rot); u += kLanes)
-                rope_unit<kForm>(a.q_in + at, a.q + at, a.cs + angle, a.sn + angle, a.rot, u);
+            const int64_t at = (row * NH + (head - NKV) * kHeads) * HD, angle = row * (a.rot / 2);
+            const int units = rope_units<kForm>(a.rot);
+            for (int u = j; u < units; u += kLanes)
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h)
+                    rope_unit<kForm>(a.q_in + at + h * HD, a.q + at + h * HD, a.cs + angle, a.sn + angle, a.rot, u);
             return;
         }
     }
-    const int head = blockIdx.y;
     float k[8] = {}, v[8] = {};                                              // the rows, requested beside the table entry
     if (real) {
         const int64_t at = (row * NKV + head) * HD;
@@ -199,7 +213,7 @@ void launch_kv_q4_store_batch(uint8_t* pool, const int32_t* tables, int table_st
     if (n_rows == 0) return;
     a.k = k;
     a.v = v;
-    hipLaunchKernelGGL((q4_store_kernel<false, kRopeApart4>), dim3(page_bound(a), NKV), dim3(QT), 0,
+    hipLaunchKernelGGL((q4_store_kernel<false, kRopeApart4>), dim3(page_bound(a) * kUnits<false>), dim3(QT), 0,
                        reinterpret_cast<hipStream_t>(s), a);
     NOVA_LAUNCHED();
 }
@@ -219,7 +233,7 @@ void launch_rope_rows_kv_q4_store_batch(const float* q, const float* k, const fl
     a.cs = cs;
     a.sn = sn;
     rope_forms(rot_dim, beside != 0, [&](auto form) {
-        hipLaunchKernelGGL((q4_store_kernel<true, decltype(form)::value>), dim3(page_bound(a), NKV + NH), dim3(QT), 0,
+        hipLaunchKernelGGL((q4_store_kernel<true, decltype(form)::value>), dim3(page_bound(a) * kUnits<true>), dim3(QT), 0,
                            reinterpret_cast<hipStream_t>(s), a);
         NOVA_LAUNCHED();
     });

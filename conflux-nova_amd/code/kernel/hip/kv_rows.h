@@ -61,24 +61,19 @@ __device__ __forceinline__ PageItem page_item(const RowArgs& a, int index) {
             n = (int64_t)p0 + n > end ? (int)(end > p0 ? end - p0 : 0) : n;
             if (n > 0) pages = ((p0 + n - 1) >> kKvBlockShift) - (p0 >> kKvBlockShift) + 1;
         }
-        int incl = pages;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int t = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += t;
-        }
+        const int incl = scan_incl(pages);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(before + incl > index);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             PageItem it;
             it.sess = base + l;
-            it.pos0 = __shfl(p0, l, 64);
-            it.row0 = __shfl(r0, l, 64);
-            it.n = __shfl(n, l, 64);
-            it.page = (it.pos0 >> kKvBlockShift) + index - (before + __shfl(incl, l, 64) - __shfl(pages, l, 64));
+            it.pos0 = __builtin_amdgcn_readlane(p0, l);
+            it.row0 = __builtin_amdgcn_readlane(r0, l);
+            it.n = __builtin_amdgcn_readlane(n, l);
+            it.page = (it.pos0 >> kKvBlockShift) + index - (before + __builtin_amdgcn_readlane(incl - pages, l));
             return it;
         }
-        before += __shfl(incl, 63, 64);
+        before += __builtin_amdgcn_readlane(incl, 63);
     }
     return PageItem{-1, 0, 0, 0, 0};
 }
