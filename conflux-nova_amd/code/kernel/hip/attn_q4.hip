@@ -10,24 +10,42 @@
 // with a power of two per 32 dims): it is held to 2^-24 of the largest of its 32 dims, and
 // sums are fp32.  V's values have one bit of mantissa, so a tile of 64 keys whose powers of two
 // lie close together (a window of eight, kSpread) is exact in fp16, and a weight goes in as
-// two fp16 terms: 2^-22 of itself, or 2^-24 - the end of fp16 - where the tile's largest weight in
-// that row stands at 2^kLow or more, which makes it 2^-26 of that weight and, with powers no
-// further apart, 2^-18 of the tile's largest product of weight and value at the very worst.  Any other tile (powers far apart, blocks of zeros, NaN, values past fp16) takes
-// V as bf16 with its power of two, exact too, and a weight as the exact sum of three
-// bf16 terms (8 bits each).  Sums are fp32.
+// two fp16 terms, to 2^-22 of itself or, where fp16 ends first, to 2^-24.  The largest weight
+// of that row in the tile stands at 2^kLow or more, so 2^-24 is 2^-26 of that weight.  Any other
+// tile (powers far apart, blocks of zeros, NaN, values past fp16) takes V as bf16 with its
+// power of two, exact too, and a weight as the exact sum of three bf16 terms (8 bits each).
+// Sums are fp32.
 //
 // One pass over the keys with a running reference and sum of the softmax.  The reference
 // m of the weights 2^(s - m) follows the largest score of the tiles, both ways and
 // lazily: a tile's largest weight may lie from 2^kLow to 2^kHigh before the sums are rescaled.  It
-// goes down no further than kDrop below its highest, so that the sums stay inside fp32; what
-// lies lower counts with 2^(kLow - 24 - kDrop) of the row's largest weight at worst.
+// goes down no further than kDrop below its highest, so that the sums stay inside fp32: a
+// tile further down, whose largest weight may be anything, loses 2^-104 of the row's largest
+// per key (2^-24 of a unit that is 2^-kDrop of it).
+//
+// What bounds it (one MI355X).  Few columns: HBM where the keys are many (8 x 32768 keys, 14B, 285
+// MB: 51 us, 5.6 TB/s, where a large read reaches 6.1; the joining launch takes 4 more), a chain of
+// latencies where they are few (16 ragged sessions of 512 to 8192 keys, 7B, 34 MB: 16 us and 4; of
+// a workgroup's 11: 1.3 until it knows its part, 1.7 until the queries are in terms, 4.7 for 2 or 3
+// tiles a wave, 1.9 for the end).  Many columns: what a wave issues, one instruction after another
+// (8 x 512 rows behind up to 4096 keys, 7B, 122 GFLOP of scores and outputs: 241 us, 506 TFLOP/s;
+// per tile and wave 216 vector and 52 matrix instructions, 110 others, 2.0 us with two waves a
+// SIMD; a wave issues for 42% of that time, waits to issue for 34% and on memory, LDS or the
+// barrier for 24%).  Left out of it one by one, the barrier is worth 4% of the time, three quarters
+// of LDS reads 2%, of K's loads nothing, 16 of the 52 products or the conversion of V 9% each.
+// Three waves a SIMD, both terms of 32 columns a wave, the next tile's scores under the softmax:
+// slower, for want of registers.
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <type_traits>
 
 namespace nova {
 namespace {
+// Batch of 8 x 512 rows (7B), 12 prompts of up to 300 rows (1.5B), 16 sessions of 1 to 8 rows (7B), us.
+// kMinPiece 1: 245, 46.9, 34.3; 2: 243, 39.9, 32.6; 3: 242, 36.8, 32.5; 6: 240, 35.9, 35.8.
 constexpr int kMinPiece = 3;
+// A group's start (table, pages, queries in terms) and end against its tiles of 2 us.  0: 263, 45.2, 34.4;
+// 1: 258, 41.2, 33.3; 2: 252, 38.9, 33.9; 4: 249, 36.6, 32.7.
 constexpr int kGroupTiles = 4;
 }  // namespace
 }  // namespace nova
@@ -688,7 +706,9 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
             float e[2][8];
             scores(kr, q, ke, st.m, z);
             __builtin_amdgcn_sched_barrier(0);               // K's registers are free now
-            __builtin_amdgcn_s_setprio(1);                   // vector work goes first: the other workgroup's products run beside it
+            // vector work goes first: the other workgroup's products run beside it (batch 240 us;
+            // 248 without, 244 the other way round)
+            __builtin_amdgcn_s_setprio(1);
             load_k(next);
             if (t >= t_clear) hide(z, t * TILE + 16 * g, seen);
             follow<kHalf>(z, st);
@@ -791,7 +811,10 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
             return;
         }
     }
-    // Tables this short: a workgroup per session and kv head, nothing to join.
+    // Tables this short: a workgroup per session and kv head, nothing to join.  One launch against two
+    // (us, one after another in a graph): 1 / 16 / 64 sessions of 300 keys (7B) 8.0, 8.1, 8.2 against 9.4, 9.8,
+    // 13.0; of 768 9.2, 9.4, 10.5 against 9.5, 10.1, 15.3; of 1024 10.5, 10.8, 12.4 against 9.6, 10.2, 16.3.  (Past
+    // 48 pages the lengths would decide, which the host does not have.)
     const bool solo = a.table_stride <= kSoloPages;
     if (solo) a.min_share = kSoloPages;
     const dim3 grid(NKV, solo ? a.n_sess : f.slots);
