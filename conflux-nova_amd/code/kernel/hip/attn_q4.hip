@@ -27,14 +27,13 @@
 // MB: 51 us, 5.6 TB/s, where a large read reaches 6.1; the joining launch takes 4 more), a chain of
 // latencies where they are few (16 ragged sessions of 512 to 8192 keys, 7B, 34 MB: 16 us and 4; of
 // a workgroup's 11: 1.3 until it knows its part, 1.7 until the queries are in terms, 4.7 for 2 or 3
-// tiles a wave, 1.9 for the end).  Many columns: what a wave issues, one instruction after another
-// (8 x 512 rows behind up to 4096 keys, 7B, 122 GFLOP of scores and outputs: 241 us, 506 TFLOP/s;
-// per tile and wave 216 vector and 52 matrix instructions, 110 others, 2.0 us with two waves a
-// SIMD; a wave issues for 42% of that time, waits to issue for 34% and on memory, LDS or the
-// barrier for 24%).  Left out of it one by one, the barrier is worth 4% of the time, three quarters
-// of LDS reads 2%, of K's loads nothing, 16 of the 52 products or the conversion of V 9% each.
-// Three waves a SIMD, both terms of 32 columns a wave, the next tile's scores under the softmax:
-// slower, for want of registers.
+// tiles a wave, 1.9 for the end).  Many columns: vector and matrix instructions, which a SIMD
+// hardly overlaps (8 x 512 rows behind up to 4096 keys, 7B, 122 GFLOP of scores and outputs: 241
+// us, 506 TFLOP/s; per tile and wave 216 vector and 52 matrix instructions and 110 others take 960 ns
+// of a SIMD, where the vector and matrix ones alone, on registers, take 678).  Left out one by
+// one, the barrier is worth 4% of the time, three quarters of the LDS reads 2%, of K's loads nothing,
+// 16 of the 52 products or the conversion of V 9% each.  Three waves a SIMD, and the next tile's
+// scores under the softmax, are slower for want of registers.
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <type_traits>
@@ -70,6 +69,7 @@ typedef float f32v __attribute__((ext_vector_type(32)));
 constexpr float kLow = 2.f, kSet = 10.f, kHigh = 15.9f;   // log2 of a tile's largest weight in fp16 terms: at least, where it is put, at most
 constexpr float kLazy = 8.f;                   // and at most in bf16 terms: 2^21 products of the largest values stay inside fp32
 constexpr float kDrop = 80.f;
+constexpr int kSoloPages = 64;                 // tables that take one launch, see launch()
 constexpr int kSpread = 8;                     // powers of two of a tile in fp16: this many in a row
 constexpr int kLeastHalf = 127 - 23, kMostHalf = 127 + 13;   // exponent bytes whose values fp16 holds exactly
 constexpr int kTerms = 5;                      // of the query
@@ -371,6 +371,11 @@ __device__ __forceinline__ float sum_of(const float (&e)[2][8]) {
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+__device__ __forceinline__ Session uniform(const Session& s) {
+    return Session{__builtin_amdgcn_readfirstlane(s.keys), __builtin_amdgcn_readfirstlane(s.past),
+                   __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.row0)};
+}
+
 // ---- few columns ----
 //
 // Up to 16 NB columns (query rows x heads of a kv head) of a session: the workgroup's waves
@@ -379,14 +384,20 @@ __device__ __forceinline__ float sum_of(const float (&e)[2][8]) {
 // that have read their registers.  kOnce: non-temporal loads, for pools that no cache
 // holds until the next step (see launch()).
 template <int NB, bool kCausal, bool kOnce>
-__global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a, bool solo) {
     constexpr int COLS = 16 * NB;
     __shared__ __attribute__((aligned(16))) float s_acc[WAVES][16][kAccRow];
     __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x, slot = blockIdx.y;
-    const Part p = find_part<kCausal>(a, slot);
-    if (p.sess < 0) return;
+    const int kvh = blockIdx.x % NKV, slot = blockIdx.x / NKV;
+    Part p;
+    if (solo) {                                              // a slot per session
+        p = Part{slot, 0, 1, uniform(session_of<kCausal>(a, slot))};
+        if (p.s.rows <= 0) return;
+    } else {
+        p = find_part<kCausal>(a, slot);
+        if (p.sess < 0) return;
+    }
     if (kvh == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
     const int n_cols = p.s.rows * G;
     // the part's tiles, and this wave's of them
@@ -567,9 +578,7 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
         if (at.sess >= a.n_sess || at.sess > to.sess ||
             (at.sess == to.sess && (at.group > to.group || (at.group == to.group && at.tile >= to.tile))))
             break;
-        Session s = session_of<true>(a, at.sess);
-        s = Session{__builtin_amdgcn_readfirstlane(s.keys), __builtin_amdgcn_readfirstlane(s.past),
-                    __builtin_amdgcn_readfirstlane(s.rows), __builtin_amdgcn_readfirstlane(s.row0)};
+        const Session s = uniform(session_of<true>(a, at.sess));
         if (at.group >= n_groups(s)) {
             at = Place{at.sess + 1, 0, 0};
             continue;
@@ -811,21 +820,19 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
             return;
         }
     }
-    // Tables this short: a workgroup per session and kv head, nothing to join.  One launch against two
-    // (us, one after another in a graph): 1 / 16 / 64 sessions of 300 keys (7B) 8.0, 8.1, 8.2 against 9.4, 9.8,
-    // 13.0; of 768 9.2, 9.4, 10.5 against 9.5, 10.1, 15.3; of 1024 10.5, 10.8, 12.4 against 9.6, 10.2, 16.3.  (Past
-    // 48 pages the lengths would decide, which the host does not have.)
+    // Tables this short: a workgroup per session and kv head, nothing to find and nothing to join.  One
+    // launch against two (us, one after another in a graph), 1 / 16 / 64 sessions of 7B: of 300 keys 7.1, 7.2, 7.4
+    // against 9.4, 9.9, 13.0; of 1024 9.4, 9.8, 11.6 against 9.6, 10.3, 16.3; of 1280 10.6, 11.2, 13.4 against 9.6, 12.1, 18.4.
     const bool solo = a.table_stride <= kSoloPages;
-    if (solo) a.min_share = kSoloPages;
-    const dim3 grid(NKV, solo ? a.n_sess : f.slots);
+    const dim3 grid(NKV * (solo ? a.n_sess : f.slots));      // (slots may be past what a second dimension holds)
     // The pages of a pool larger than the 256 MB memory-side cache (all layers of it,
     // as a step walks through them) come from HBM.
     const bool once = (int64_t)Model::L * a.nb * kQ4Page > (int64_t)256 << 20;
     auto run = [&](auto once_tag) {
         constexpr bool kOnce = decltype(once_tag)::value;
-        if (f.cols == 16) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce>), grid, dim3(THREADS), 0, s, a);
+        if (f.cols == 16) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce>), grid, dim3(THREADS), 0, s, a, solo);
         if constexpr (kCausal)
-            if (f.cols == 32) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce>), grid, dim3(THREADS), 0, s, a);
+            if (f.cols == 32) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce>), grid, dim3(THREADS), 0, s, a, solo);
     };
     if (once) run(std::true_type{});
     else run(std::false_type{});

@@ -66,6 +66,7 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
+constexpr int kSoloPages = 48;                  // tables that take one launch, see launch()
 constexpr float kTop = 6.f, kLazy = 15.9f;      // log2 of a column's largest weight times value scale: where it is put, where it may drift
 constexpr int kUnitLeast = -125, kUnitMost = 36;   // log2 of the units of value scales; 1 / unit is finite
 constexpr float kFloor = -82.f, kUnitRoom = 0x1p86f;   // log2 of the smallest scale in units that the reference follows; the largest scale

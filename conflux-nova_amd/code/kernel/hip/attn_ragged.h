@@ -564,7 +564,6 @@ constexpr int kFewCols = 32;
 // Tiles of a workgroup that shares a session: one per wave.  Many columns, 12 prompts
 // of up to 300 tokens (1.5B): 2 42.9 us, 4 43.1, 6 44.3, 8 57.4.
 constexpr int kMinShare = 4;
-constexpr int kSoloPages = 48;            // see launch()
 // A joining launch that fills the chip (4096: 16 sessions of 1 to 8 rows, 7B, 34.8 us instead
 // of 34.4; 12 prompts of up to 300 tokens, 1.5B, 38.5, 37.4).
 constexpr int kJoinWgs = 2048;

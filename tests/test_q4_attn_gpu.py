@@ -105,6 +105,20 @@ def test_short_tables(n_keys):
     d.check("short")
 
 
+@pytest.mark.parametrize("model", MODELS)
+@pytest.mark.parametrize("stride", [64, 65])
+def test_tables_at_the_one_launch_limit(model, stride):
+    """tables of up to 64 pages take one launch, with sessions of no keys and no rows among them"""
+    d = Call(model, [1024, 0, 1023, 1, 700], seed=75)
+    c = Call(model, [1020, 9, 0, 500, 1000], [3, 0, 1, 2, 0], seed=76, behind=2)
+    for x in (d, c):
+        assert x.table.shape[1] >= stride
+        x.table = np.ascontiguousarray(x.table[:, :stride])
+        x.upload()
+        x.run()
+        x.check(f"{stride} pages")
+
+
 def test_keys_behind_the_table_are_left_out():
     d = Call("qwen25_1p5b", [64, 40], seed=65, poison=False)
     d.table = np.ascontiguousarray(d.table[:, :3])           # 48 tokens each
