@@ -9,12 +9,13 @@
 // same pages.  Everything is prefix sums over the sessions, so there are no atomics and
 // the result is the same every time.
 //
-// One workgroup does the sums (two passes over the sessions: what comes back, then what
-// fits) and, for a small step, all the rest, out of registers and LDS.  Larger ones leave pages
-// and rows to two more launches over the whole chip, as the stack must be whole before
-// pages are taken from it.  It moves a few KB (16 sessions of a token each) to a MB, so latency
-// bounds all of it: 3.6 us for those 16, 11 us for 700 sessions and 60000 rows (3.4, 3.3 and 4.4),
-// where a launch that does nothing takes 2.
+// A workgroup does the sums (two passes over the sessions: what comes back, then what fits)
+// and, for a small step, all the rest, out of registers and LDS.  Larger ones take two launches over
+// the chip, as the stack must be whole before pages are taken from it: in the first, workgroups
+// that sum for themselves what comes back put it on the stack, and one works out what fits;
+// the second hands out pages and places rows.  It moves a few KB (16 sessions of a token each) to a
+// MB, so latency bounds all of it: 3.6 us for those 16, 8.0 for 700 sessions and 60000 rows (3.8 and
+// 4.2), where a launch that does nothing takes 2.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cstdint>
@@ -33,11 +34,15 @@ constexpr int kPlanWaves = PT / 64;
 constexpr uint32_t kNoneFits = ~0u;
 static_assert(kPlanWaves == 16, "a wave's sums in a row of 16 lanes");
 constexpr int FT = 256;                        // threads of the others
+constexpr int kBackWgs = 64;                   // workgroups that give pages back, PT / kBackWgs sessions of every PT each
+constexpr int kMine = PT / kBackWgs;
+constexpr int kMostPasses = 64;                // PT sessions at a time
+static_assert(kMostPasses * PT > 65535, "every session");
 constexpr int kOffsets = 4096;                 // sessions whose row offsets fit a workgroup's LDS
-// One launch up to this many rows and sessions.  One launch against three (us, one after another in a
-// graph, 31 pages held): 16 sessions of 1 row 3.7, 6.6; 64 of 32 6.9, 8.1; 256 of 8 6.6, 7.9; past it 16 of 256
-// 6.3, 7.7, but 256 of 16 15.0, 8.4 and 1000 of 1 10.4, 9.4.
-constexpr int kSmallRows = 2048, kSmallSessions = 256;
+// One launch up to this many rows and sessions.  One launch against two (us, one after another in a
+// graph, 31 pages held; a launch more costs the host another 3): 16 sessions of 1 row 3.7, 5.2; of 64 4.6, 5.9;
+// 64 of 16 6.3, 6.0; 256 of 4 5.7, 6.5; past it 64 of 32 7.1, 6.0, 256 of 8 6.6, 6.3, of 16 15.6, 6.5, 1000 of 1 10.4, 7.9.
+constexpr int kSmallRows = 1024, kSmallSessions = 256;
 
 struct PlanArgs {
     int32_t* tables;
@@ -49,8 +54,10 @@ struct PlanArgs {
     int32_t *past, *keys, *row_off, *pos;
     int64_t* slots;
     int32_t* free_left;
-    i4* info;                                  // workspace: [n_sess] {first, held, pages back before, pages taken before}
-    int64_t* stack;                            // workspace: {free pages with those back, free pages before}
+    // workspace, between the two launches of a larger step
+    i4* info;                                  // [n_sess] {first, held, pages back before, pages taken before}
+    int32_t *ws_past, *ws_keys, *ws_off;       // what past, keys and row_off become (have may be one of them)
+    int64_t* stack;                            // {free pages with those back, free pages left}
 };
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens) { return (tokens + kKvBlock - 1) >> kKvBlockShift; }
@@ -107,14 +114,11 @@ __device__ __forceinline__ Pair block_scan(Pair v, Pair* s_wave, Pair& total) {
     return v;
 }
 
-// the pages that sessions from..n_sess step by `step` give back, onto the stack; one wave
-__device__ __forceinline__ void give_back(const PlanArgs& a, const i4* info, int from, int step, int64_t avail, int64_t n_free) {
-    for (int i = from; i < a.n_sess; i += step) {
-        const i4 in = info[i];
-        for (int p = in[0] + (int)(threadIdx.x & 63); p < in[1]; p += 64) {
-            const int64_t at = avail - 1 - ((int64_t)in[2] + p - in[0]);
-            if (at >= n_free) a.free_pages[at] = a.tables[i * a.stride + p];
-        }
+// the pages that session i gives back, onto the stack; one wave
+__device__ __forceinline__ void give_back(const PlanArgs& a, int i, const i4& in, int64_t avail, int64_t n_free) {
+    for (int p = in[0] + (int)(threadIdx.x & 63); p < in[1]; p += 64) {
+        const int64_t at = avail - 1 - ((int64_t)in[2] + p - in[0]);
+        if (at >= n_free) a.free_pages[at] = a.tables[i * a.stride + p];
     }
 }
 // the page that session i's nth new page is
@@ -150,12 +154,13 @@ __device__ __forceinline__ void place_row(const PlanArgs& a, const i4* info, con
     a.slots[r] = slot;
 }
 
-// kAll: everything, for up to kSmallSessions sessions, whose numbers stay in registers and LDS
+// kAll: everything, for up to kSmallSessions sessions, whose numbers stay in registers and LDS.
+// Else workgroup 0 leaves in the workspace what the second launch needs, and the others give pages back.
 template <bool kAll>
 __global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
-    constexpr int kKept = kAll ? kSmallSessions : 1;
+    constexpr int kKept = kAll ? kSmallSessions : kMine * kMostPasses;
     __shared__ Pair s_wave[3][kPlanWaves];
-    __shared__ int32_t s_off[kKept + 1], s_past[kKept], s_keys[kKept];
+    __shared__ int32_t s_off[kAll ? kKept + 1 : 1], s_past[kAll ? kKept : 1], s_keys[kAll ? kKept : 1];
     __shared__ __attribute__((aligned(16))) i4 s_info[kKept];
     const int tid = threadIdx.x;
     const int64_t n_free = min(max((int64_t)*a.n_free, (int64_t)0), (int64_t)a.nb);
@@ -176,10 +181,21 @@ __global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
         const Pair sum = block_scan(Pair{(uint32_t)(in[1] - in[0]), 0}, s_wave[of], total);
         // (more than the stack holds is nowhere)
         in[2] = (int)min(back + sum.a - (in[1] - in[0]), (int64_t)a.nb);
-        if (!kAll && i < a.n_sess) a.info[i] = in;
+        if (!kAll) {
+            if (blockIdx.x == 0) {
+                if (i < a.n_sess) a.info[i] = in;
+            } else if (tid / kMine == (int)blockIdx.x - 1) s_info[base / PT * kMine + tid % kMine] = in;
+        }
         back += total.a;
     }
     const int64_t avail = min(n_free + back, (int64_t)a.nb);
+    if (!kAll && blockIdx.x > 0) {
+        __syncthreads();
+        const int kept = (a.n_sess + PT - 1) / PT * kMine;
+        for (int j = tid >> 6; j < kept; j += kPlanWaves)     // (sessions behind the last hold nothing)
+            give_back(a, j / kMine * PT + ((int)blockIdx.x - 1) * kMine + j % kMine, s_info[j], avail, n_free);
+        return;
+    }
     // What fits: the sessions before the first with which the sums of what was wished for pass the room, so
     // the sums up to a session that fits are those of what was granted.
     int64_t rows_before = 0, pages_before = 0;               // wished for by the sessions of the passes before
@@ -208,9 +224,9 @@ __global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
         if (real) {
             const int keys = (int)(w.keep + (fits ? rows : 0)), end = (int)(fits ? all_rows : given.a);
             const int first = fits ? (int)(all_pages - more) : 0;
-            a.past[i] = (int)w.keep;
-            a.keys[i] = keys;
-            a.row_off[i + 1] = end;
+            (kAll ? a.past : a.ws_past)[i] = (int)w.keep;
+            (kAll ? a.keys : a.ws_keys)[i] = keys;
+            (kAll ? a.row_off : a.ws_off)[i + 1] = end;
             if constexpr (kAll) {
                 in[3] = first;
                 s_info[i] = in;
@@ -223,18 +239,20 @@ __global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
         pages_before += total.b;
     }
     if (tid == 0) {
-        a.row_off[0] = 0;
-        if (kAll) s_off[0] = 0;
-        *a.free_left = (int)(avail - given.b);
-        if (!kAll) {
+        if constexpr (kAll) {
+            a.row_off[0] = 0;
+            s_off[0] = 0;
+            *a.free_left = (int)(avail - given.b);
+        } else {
+            a.ws_off[0] = 0;
             a.stack[0] = avail;
-            a.stack[1] = n_free;
+            a.stack[1] = avail - given.b;
         }
     }
     if constexpr (kAll) {
         __syncthreads();
         if (back > 0) {                                      // uniform
-            give_back(a, s_info, tid >> 6, PT / 64, avail, n_free);
+            for (int i = tid >> 6; i < a.n_sess; i += kPlanWaves) give_back(a, i, s_info[i], avail, n_free);
             __syncthreads();
         }
         hand_out(a, s_info, s_keys, tid >> 6, PT / 64, avail);
@@ -242,29 +260,36 @@ __global__ void __launch_bounds__(PT) plan_kernel(PlanArgs a) {
     }
 }
 
-__global__ void __launch_bounds__(FT) plan_back_kernel(PlanArgs a) {
-    give_back(a, a.info, (int)(blockIdx.x * (FT / 64) + (threadIdx.x >> 6)), (int)gridDim.x * (FT / 64), a.stack[0], a.stack[1]);
-}
-
-// workgroups below row_wgs: rows; the others: tables
+// workgroups below row_wgs: rows; the others: tables and what the sessions have now
 __global__ void __launch_bounds__(FT) plan_rows_kernel(PlanArgs a, int row_wgs) {
     __shared__ int32_t s_off[kOffsets + 1];
     const int64_t avail = a.stack[0];
     if ((int)blockIdx.x >= row_wgs) {
-        const int wgs = (int)gridDim.x - row_wgs;
-        hand_out(a, a.info, a.keys, ((int)blockIdx.x - row_wgs) * (FT / 64) + (int)(threadIdx.x >> 6), wgs * (FT / 64), avail);
+        const int wgs = (int)gridDim.x - row_wgs, w = (int)blockIdx.x - row_wgs;
+        for (int i = w * FT + (int)threadIdx.x; i <= a.n_sess; i += wgs * FT) {
+            a.row_off[i] = a.ws_off[i];
+            if (i == a.n_sess) *a.free_left = (int)a.stack[1];
+            else {
+                a.past[i] = a.ws_past[i];
+                a.keys[i] = a.ws_keys[i];
+            }
+        }
+        hand_out(a, a.info, a.ws_keys, w * (FT / 64) + (int)(threadIdx.x >> 6), wgs * (FT / 64), avail);
         return;
     }
     const bool here = a.n_sess <= kOffsets;
     if (here)
-        for (int i = threadIdx.x; i <= a.n_sess; i += FT) s_off[i] = a.row_off[i];
+        for (int i = threadIdx.x; i <= a.n_sess; i += FT) s_off[i] = a.ws_off[i];
     __syncthreads();
-    for (int r = blockIdx.x * FT + threadIdx.x; r < a.max_rows; r += row_wgs * FT) place_row(a, a.info, a.past, here ? s_off : a.row_off, r, avail);
+    for (int r = blockIdx.x * FT + threadIdx.x; r < a.max_rows; r += row_wgs * FT) place_row(a, a.info, a.ws_past, here ? s_off : a.ws_off, r, avail);
 }
 
 constexpr int kWgs = 1024;                     // of the larger launches
 
+// workspace: the stack's two numbers, then the sessions'
 size_t info_at() { return 256; }
+size_t past_at(int n_sess) { return info_at() + (size_t)n_sess * sizeof(i4); }
+size_t bytes(int n_sess) { return past_at(n_sess) + (3 * (size_t)n_sess + 1) * sizeof(int32_t); }
 
 }  // namespace
 }  // namespace nova
@@ -275,7 +300,7 @@ extern "C" {
 
 size_t kv_step_plan_workspace_bytes(int n_sess) {
     NOVA_REQUIRE(n_sess >= 1 && n_sess <= 65535);
-    return info_at() + (size_t)n_sess * sizeof(i4);
+    return bytes(n_sess);
 }
 
 void launch_kv_step_plan(int32_t* tables, int table_stride, const int32_t* n_have, const int32_t* n_keep,
@@ -289,20 +314,20 @@ void launch_kv_step_plan(int32_t* tables, int table_stride, const int32_t* n_hav
     NOVA_REQUIRE((pos && slots) || max_rows == 0);
     NOVA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
     char* ws = static_cast<char*>(workspace);
+    int32_t* ws_past = reinterpret_cast<int32_t*>(ws + past_at(n_sess));
     const PlanArgs a{tables,  table_stride, n_have, n_keep,  n_new, n_sess, max_rows,    nb,
                      free_pages, n_free,       n_past, n_keys, row_off, pos,   slots,  n_free_left,
-                     reinterpret_cast<i4*>(ws + info_at()), reinterpret_cast<int64_t*>(ws)};
+                     reinterpret_cast<i4*>(ws + info_at()), ws_past, ws_past + n_sess, ws_past + 2 * n_sess,
+                     reinterpret_cast<int64_t*>(ws)};
     const hipStream_t st = reinterpret_cast<hipStream_t>(s);
     if (max_rows <= kSmallRows && n_sess <= kSmallSessions) {
         hipLaunchKernelGGL(plan_kernel<true>, dim3(1), dim3(PT), 0, st, a);
         NOVA_LAUNCHED();
         return;
     }
-    hipLaunchKernelGGL(plan_kernel<false>, dim3(1), dim3(PT), 0, st, a);
+    hipLaunchKernelGGL(plan_kernel<false>, dim3(1 + kBackWgs), dim3(PT), 0, st, a);
     NOVA_LAUNCHED();
     const int sess_wgs = std::min((n_sess + FT / 64 - 1) / (FT / 64), kWgs);
-    hipLaunchKernelGGL(plan_back_kernel, dim3(sess_wgs), dim3(FT), 0, st, a);
-    NOVA_LAUNCHED();
     const int row_wgs = std::min((max_rows + FT - 1) / FT, kWgs);
     hipLaunchKernelGGL(plan_rows_kernel, dim3(row_wgs + sess_wgs), dim3(FT), 0, st, a, row_wgs);
     NOVA_LAUNCHED();

@@ -58,10 +58,11 @@ def test_plan(name):
 
 
 @pytest.mark.parametrize("n,stride,most_new,max_rows,spare", [
-    (256, 30, 7, 2048, 300), (257, 30, 7, 2049, 300), (1024, 12, 40, 30000, 1500), (1025, 12, 40, 1 << 15, 4000), (5000, 4, 3, 9000, 3000),
-    (3, 3000, 30000, 60001, 5000), (1, 9000, 100000, 100000, 9000)])
+    (256, 30, 3, 1024, 300), (100, 30, 9, 1025, 300), (2, 30, 400, 1024, 90), (256, 30, 7, 2048, 300), (257, 30, 7, 2049, 300),
+    (1024, 12, 40, 30000, 1500), (1025, 12, 40, 1 << 15, 4000), (5000, 4, 3, 9000, 3000),
+    (65535, 2, 2, 70000, 9000), (3, 3000, 30000, 60001, 5000), (1, 9000, 100000, 100000, 9000)])
 def test_large_plans(n, stride, most_new, max_rows, spare):
-    """one launch and three, sessions past a workgroup's threads and past what LDS holds, a stack that runs out"""
+    """one launch and two, sessions past a workgroup's threads and past what LDS holds, a stack that runs out"""
     print(f"[case] plan of {n}", flush=True)
     rng = np.random.default_rng(n)
     have = rng.integers(0, stride * KB - min(most_new, stride * 8), n)
