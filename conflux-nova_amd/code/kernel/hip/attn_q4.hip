@@ -70,6 +70,7 @@ constexpr float kLow = 2.f, kSet = 10.f, kHigh = 15.9f;   // log2 of a tile's la
 constexpr float kLazy = 8.f;                   // and at most in bf16 terms: 2^21 products of the largest values stay inside fp32
 constexpr float kDrop = 80.f;
 constexpr int kSoloPages = 64;                 // tables that take one launch, see launch()
+static_assert(kSoloPages <= 64, "a lane per page of a short table");
 constexpr int kSpread = 8;                     // powers of two of a tile in fp16: this many in a row
 constexpr int kLeastHalf = 127 - 23, kMostHalf = 127 + 13;   // exponent bytes whose values fp16 holds exactly
 constexpr int kTerms = 5;                      // of the query
@@ -391,7 +392,9 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int kvh = blockIdx.x % NKV, slot = blockIdx.x / NKV;
     Part p;
+    int row = 0;                                             // a short table's whole row, requested beside the length
     if (solo) {                                              // a slot per session
+        row = a.tables[slot * a.table_stride + min(lane, (int)a.table_stride - 1)];
         p = Part{slot, 0, 1, uniform(session_of<kCausal>(a, slot))};
         if (p.s.rows <= 0) return;
     } else {
@@ -408,6 +411,10 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
 
     // lane (g, c) reads K rows and exponents of page c >> 2, V columns and exponents of page g
     Pages pages(a, p.sess, p.s.keys);
+    if (solo) {
+        pages.win = 0;
+        pages.held = row;
+    }
     const uint8_t *k_at = nullptr, *v_at = nullptr;
     i4 kr[4], vr[4];
     int ke = 0, ve = 0;
