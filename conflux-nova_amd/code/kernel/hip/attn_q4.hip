@@ -69,8 +69,7 @@ typedef float f32v __attribute__((ext_vector_type(32)));
 constexpr float kLow = 2.f, kSet = 10.f, kHigh = 15.9f;   // log2 of a tile's largest weight in fp16 terms: at least, where it is put, at most
 constexpr float kLazy = 8.f;                   // and at most in bf16 terms: 2^21 products of the largest values stay inside fp32
 constexpr float kDrop = 80.f;
-constexpr int kSoloPages = 64;                 // tables that take one launch, see launch()
-static_assert(kSoloPages <= 64, "a lane per page of a short table");
+constexpr int kCus = kAimWgs / 2;
 constexpr int kSpread = 8;                     // powers of two of a tile in fp16: this many in a row
 constexpr int kLeastHalf = 127 - 23, kMostHalf = 127 + 13;   // exponent bytes whose values fp16 holds exactly
 constexpr int kTerms = 5;                      // of the query
@@ -383,18 +382,19 @@ __device__ __forceinline__ Session uniform(const Session& s) {
 // share them and each takes its own keys, 64 at a time, so K and V are read once.  The
 // operands come straight from the pages; the next tile's loads go out behind the products
 // that have read their registers.  kOnce: non-temporal loads, for pools that no cache
-// holds until the next step (see launch()).
-template <int NB, bool kCausal, bool kOnce>
-__global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a, bool solo) {
+// holds until the next step; solo: a workgroup per session (see launch()).
+template <int NB, bool kCausal, bool kOnce, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a, bool solo) {
     constexpr int COLS = 16 * NB;
-    __shared__ __attribute__((aligned(16))) float s_acc[WAVES][16][kAccRow];
-    __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
+    __shared__ __attribute__((aligned(16))) float s_acc[kWaves][16][kAccRow];
+    __shared__ float s_m[kWaves][COLS], s_l[kWaves][COLS];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int kvh = blockIdx.x % NKV, slot = blockIdx.x / NKV;
     Part p;
-    int row = 0;                                             // a short table's whole row, requested beside the length
+    const bool whole = solo && a.table_stride <= 64;         // a lane per page of the table:
+    int row = 0;                                             // its row, requested beside the length
     if (solo) {                                              // a slot per session
-        row = a.tables[slot * a.table_stride + min(lane, (int)a.table_stride - 1)];
+        if (whole) row = a.tables[slot * a.table_stride + min(lane, (int)a.table_stride - 1)];
         p = Part{slot, 0, 1, uniform(session_of<kCausal>(a, slot))};
         if (p.s.rows <= 0) return;
     } else {
@@ -406,12 +406,12 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
     // the part's tiles, and this wave's of them
     const int tiles = (p.s.keys + TILE - 1) / TILE;
     const int t_lo = (int)((int64_t)tiles * p.index / p.parts), t_hi = (int)((int64_t)tiles * (p.index + 1) / p.parts);
-    const int t0 = t_lo + (t_hi - t_lo) * wave / WAVES, t1 = t_lo + (t_hi - t_lo) * (wave + 1) / WAVES;
+    const int t0 = t_lo + (t_hi - t_lo) * wave / kWaves, t1 = t_lo + (t_hi - t_lo) * (wave + 1) / kWaves;
     const int clear_keys = min(p.s.past + 1, p.s.keys);      // keys below: seen by all columns
 
     // lane (g, c) reads K rows and exponents of page c >> 2, V columns and exponents of page g
     Pages pages(a, p.sess, p.s.keys);
-    if (solo) {
+    if (whole) {
         pages.win = 0;
         pages.held = row;
     }
@@ -433,22 +433,21 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
 #pragma unroll
         for (int b = 0; b < 4; ++b) vr[b] = page_load<kOnce>(v_at + kQ4VOff + 256 * b + 16 * c);
     };
-    f4 x[NB][8];               // the queries first: they have come when the first pages are on their way
-    int seen[NB];              // keys that the column sees
-#pragma unroll
-    for (int b = 0; b < NB; ++b) load_q(a, p.s, kvh, 16 * b + c, x[b], seen[b]);
-    if (t0 < t1) {
-        load_k(t0);
-        load_v();
-    }
     QTerms q[NB];
     State st[NB];
+    int seen[NB];              // keys that the column sees
     Window win;
     win.clear();
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        q_terms(x[b], q[b]);
-        st[b].clear();
+    for (int b = 0; b < NB; ++b) st[b].clear();
+    if (t0 < t1) {             // the queries first: they have come when the first pages are on their way
+        f4 x[NB][8];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) load_q(a, p.s, kvh, 16 * b + c, x[b], seen[b]);
+        load_k(t0);
+        load_v();
+#pragma unroll
+        for (int b = 0; b < NB; ++b) q_terms(x[b], q[b]);
     }
     auto step = [&](auto mask_tag, int t) {
         constexpr bool kMask = decltype(mask_tag)::value;
@@ -513,7 +512,7 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
     for (int t = t0; t < t_clear; ++t) step(std::false_type{}, t);
     for (int t = t_clear; t < t1; ++t) step(std::true_type{}, t);
 
-    // the four waves' states joined in LDS; a lone part writes the output
+    // the waves' states joined in LDS; a lone part writes the output
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const float l = rows_sum(st[b].l);
@@ -530,16 +529,16 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q4_few_kernel(AttnAr
 #pragma unroll
             for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(&s_acc[wave][c][16 * d + 4 * g]) = st[b].acc[d];
         __syncthreads();
-        for (int e = tid; e < 16 * (HD / 4); e += THREADS) {
+        for (int e = tid; e < 16 * (HD / 4); e += 64 * kWaves) {
             const int cc = e / (HD / 4), d4 = e % (HD / 4), col = 16 * b + cc;
             if (col >= n_cols) continue;
             float m = s_m[0][col];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) m = fmaxf(m, s_m[w][col]);
+            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][col]);
             f4 sum = f4{0.f, 0.f, 0.f, 0.f};
             float l = 0.f;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
+            for (int w = 0; w < kWaves; ++w) {
                 const Factor f(s_m[w][col] - m);
                 sum += f * *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]);
                 l += f * s_l[w][col];
@@ -827,19 +826,27 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
             return;
         }
     }
-    // Tables this short: a workgroup per session and kv head, nothing to find and nothing to join.  One
-    // launch against two (us, one after another in a graph), 1 / 16 / 64 sessions of 7B: of 300 keys 7.1, 7.2, 7.4
-    // against 9.4, 9.9, 13.0; of 1024 9.4, 9.8, 11.6 against 9.6, 10.3, 16.3; of 1280 10.6, 11.2, 13.4 against 9.6, 12.1, 18.4.
-    const bool solo = a.table_stride <= kSoloPages;
+    // Short tables: a workgroup per session and kv head, nothing to find and nothing to join.  Up to 64 pages, or
+    // 40 with 17 to 32 columns; where the workgroups are 64 and more, up to 96, as parts of the sessions
+    // would share CUs.  One launch against two (us, one after another in a graph), 1 / 8 / 32 sessions of 7B: of 300
+    // keys 6.6, 6.8, 6.9 against 9.2, 9.3, 10.0; of 1024 8.9, 9.2, 9.5 against 9.4, 9.6, 12.6; of 1040 10.5, 10.8, 11.2
+    // against 9.5, 9.8, 14.0; of 1536 11.4, 11.7, 12.4 against 9.5, 9.8, 14.7.  With 4 rows: of 500 12.2, 12.5, 12.7
+    // against 14.0, 14.8, 21.3; of 764 14.7, 15.1, 15.5 against 14.0, 15.2, 29.6.
+    const int wgs = a.n_sess * NKV;
+    const bool solo = a.table_stride <= (wgs >= kCus / 4 ? 96 : f.cols == 16 ? 64 : 40);
+    // With a CU for each of them, eight waves instead of four (7.1 and 9.6 us for 16 sessions of 300 and 1024 keys of
+    // 7B with four, 6.8 and 9.2 with eight); 32 columns take the registers of one wave a SIMD.
+    const bool wide = solo && f.cols == 16 && wgs <= kCus;
     const dim3 grid(NKV * (solo ? a.n_sess : f.slots));      // (slots may be past what a second dimension holds)
     // The pages of a pool larger than the 256 MB memory-side cache (all layers of it,
     // as a step walks through them) come from HBM.
     const bool once = (int64_t)Model::L * a.nb * kQ4Page > (int64_t)256 << 20;
     auto run = [&](auto once_tag) {
         constexpr bool kOnce = decltype(once_tag)::value;
-        if (f.cols == 16) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce>), grid, dim3(THREADS), 0, s, a, solo);
+        if (wide) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, 8>), grid, dim3(512), 0, s, a, true);
+        else if (f.cols == 16) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, solo);
         if constexpr (kCausal)
-            if (f.cols == 32) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce>), grid, dim3(THREADS), 0, s, a, solo);
+            if (f.cols == 32) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, solo);
     };
     if (once) run(std::true_type{});
     else run(std::false_type{});

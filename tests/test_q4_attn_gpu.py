@@ -106,12 +106,17 @@ def test_short_tables(n_keys):
 
 
 @pytest.mark.parametrize("model", MODELS)
-@pytest.mark.parametrize("stride", [64, 65])
-def test_tables_at_the_one_launch_limit(model, stride):
-    """tables of up to 64 pages take one launch, with sessions of no keys and no rows among them"""
-    d = Call(model, [1024, 0, 1023, 1, 700], seed=75)
-    c = Call(model, [1020, 9, 0, 500, 1000], [3, 0, 1, 2, 0], seed=76, behind=2)
-    for x in (d, c):
+@pytest.mark.parametrize("stride", [40, 41, 64, 65, 96, 97])
+def test_tables_at_the_one_launch_limits(model, stride):
+    """few sessions and enough for longer tables, with some of no keys and no rows"""
+    most = stride * KB
+    lengths = [most, 0, most - 1, 1, 700 % most]
+    d = Call(model, lengths, seed=75)
+    c = Call(model, [most - 4, 9, 0, 500, most - 20], [3, 0, 1, 2, 0], seed=76, behind=2)
+    many = 64 // d.nova.nkv
+    e = Call(model, (lengths * many)[:many], seed=77)
+    f = Call(model, [most - 4] + [40 + i for i in range(many - 1)], [3] + [i % 3 for i in range(many - 1)], seed=78, behind=2)
+    for x in (d, c, e, f):
         assert x.table.shape[1] >= stride
         x.table = np.ascontiguousarray(x.table[:, :stride])
         x.upload()
