@@ -382,27 +382,29 @@ __device__ __forceinline__ Session uniform(const Session& s) {
 // share them and each takes its own keys, 64 at a time, so K and V are read once.  The
 // operands come straight from the pages; the next tile's loads go out behind the products
 // that have read their registers.  kOnce: non-temporal loads, for pools that no cache
-// holds until the next step; solo: a workgroup per session (see launch()).
+// holds until the next step.  solo: 0, or the workgroups of a session, 16 columns each (see launch()).
 template <int NB, bool kCausal, bool kOnce, int kWaves>
-__global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a, bool solo) {
+__global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a, int solo) {
     constexpr int COLS = 16 * NB;
     __shared__ __attribute__((aligned(16))) float s_acc[kWaves][16][kAccRow];
     __shared__ float s_m[kWaves][COLS], s_l[kWaves][COLS];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x % NKV, slot = blockIdx.x / NKV;
+    const int kvh = blockIdx.x % NKV, unit = blockIdx.x / NKV;
+    const int slot = NB == 1 && solo ? unit / solo : unit;
+    const int col0 = NB == 1 && solo ? 16 * (unit - slot * solo) : 0;        // the first of the workgroup's columns
     Part p;
     const bool whole = solo && a.table_stride <= 64;         // a lane per page of the table:
     int row = 0;                                             // its row, requested beside the length
     if (solo) {                                              // a slot per session
         if (whole) row = a.tables[slot * a.table_stride + min(lane, (int)a.table_stride - 1)];
         p = Part{slot, 0, 1, uniform(session_of<kCausal>(a, slot))};
-        if (p.s.rows <= 0) return;
+        if (p.s.rows * G <= col0) return;
     } else {
         p = find_part<kCausal>(a, slot);
         if (p.sess < 0) return;
     }
-    if (kvh == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
-    const int n_cols = p.s.rows * G;
+    if (!solo && kvh == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
+    const int n_cols = p.s.rows * G - col0;
     // the part's tiles, and this wave's of them
     const int tiles = (p.s.keys + TILE - 1) / TILE;
     const int t_lo = (int)((int64_t)tiles * p.index / p.parts), t_hi = (int)((int64_t)tiles * (p.index + 1) / p.parts);
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
     if (t0 < t1) {             // the queries first: they have come when the first pages are on their way
         f4 x[NB][8];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) load_q(a, p.s, kvh, 16 * b + c, x[b], seen[b]);
+        for (int b = 0; b < NB; ++b) load_q(a, p.s, kvh, col0 + 16 * b + c, x[b], seen[b]);
         load_k(t0);
         load_v();
 #pragma unroll
@@ -544,7 +546,7 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
                 l += f * s_l[w][col];
             }
             if (p.parts == 1) {
-                const int r = col / G, hh = col - r * G;
+                const int r = (col0 + col) / G, hh = col0 + col - r * G;
                 const float n = p.s.keys > 0 ? 1.0f / l : 0.f;
                 *reinterpret_cast<f4*>(a.o + ((int64_t)(p.s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d4) = sum * n;
             } else {
@@ -826,27 +828,26 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
             return;
         }
     }
-    // Short tables: a workgroup per session and kv head, nothing to find and nothing to join.  Up to 64 pages, or
-    // 40 with 17 to 32 columns; where the workgroups are 64 and more, up to 96, as parts of the sessions
-    // would share CUs.  One launch against two (us, one after another in a graph), 1 / 8 / 32 sessions of 7B: of 300
+    // Short tables: a workgroup per session, kv head and 16 columns, nothing to find and nothing to join.  Up to
+    // 64 pages; where the workgroups are 64 and more, up to 96, as parts of the sessions would share CUs.  One launch against two (us, one after another in a graph), 1 / 8 / 32 sessions of 7B: of 300
     // keys 6.6, 6.8, 6.9 against 9.2, 9.3, 10.0; of 1024 8.9, 9.2, 9.5 against 9.4, 9.6, 12.6; of 1040 10.5, 10.8, 11.2
     // against 9.5, 9.8, 14.0; of 1536 11.4, 11.7, 12.4 against 9.5, 9.8, 14.7.  With 4 rows: of 500 12.2, 12.5, 12.7
     // against 14.0, 14.8, 21.3; of 764 14.7, 15.1, 15.5 against 14.0, 15.2, 29.6.
-    const int wgs = a.n_sess * NKV;
-    const bool solo = a.table_stride <= (wgs >= kCus / 4 ? 96 : f.cols == 16 ? 64 : 40);
+    const int halves = f.cols / 16, wgs = a.n_sess * NKV * halves;
+    const bool solo = a.table_stride <= (wgs >= kCus / 4 ? 96 : 64);
     // With a CU for each of them, eight waves instead of four (7.1 and 9.6 us for 16 sessions of 300 and 1024 keys of
-    // 7B with four, 6.8 and 9.2 with eight); 32 columns take the registers of one wave a SIMD.
-    const bool wide = solo && f.cols == 16 && wgs <= kCus;
-    const dim3 grid(NKV * (solo ? a.n_sess : f.slots));      // (slots may be past what a second dimension holds)
+    // 7B with four, 6.8 and 9.2 with eight).
+    const bool wide = solo && wgs <= kCus;
+    const dim3 grid(solo ? wgs : NKV * f.slots);             // (slots may be past what a second dimension holds)
     // The pages of a pool larger than the 256 MB memory-side cache (all layers of it,
     // as a step walks through them) come from HBM.
     const bool once = (int64_t)Model::L * a.nb * kQ4Page > (int64_t)256 << 20;
     auto run = [&](auto once_tag) {
         constexpr bool kOnce = decltype(once_tag)::value;
-        if (wide) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, 8>), grid, dim3(512), 0, s, a, true);
-        else if (f.cols == 16) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, solo);
-        if constexpr (kCausal)
-            if (f.cols == 32) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, solo);
+        if (wide) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, 8>), grid, dim3(512), 0, s, a, halves);
+        else if (solo || halves == 1)
+            hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, solo ? halves : 0);
+        else if constexpr (kCausal) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, 0);
     };
     if (once) run(std::true_type{});
     else run(std::false_type{});
