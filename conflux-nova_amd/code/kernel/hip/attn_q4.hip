@@ -378,20 +378,20 @@ __device__ __forceinline__ Session uniform(const Session& s) {
 
 // ---- few columns ----
 //
-// Up to 16 NB columns (query rows x heads of a kv head) of a session: the workgroup's waves
-// share them and each takes its own keys, 64 at a time, so K and V are read once.  The
-// operands come straight from the pages; the next tile's loads go out behind the products
-// that have read their registers.  kOnce: non-temporal loads, for pools that no cache
-// holds until the next step.  solo: 0, or the workgroups of a session, 16 columns each (see launch()).
-template <int NB, bool kCausal, bool kOnce, int kWaves>
-__global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(AttnArgs a, int solo) {
-    constexpr int COLS = 16 * NB;
+// 16 columns (query rows x heads of a kv head) of a session's `blocks` times 16: the workgroup's
+// waves share them and each takes its own keys, 64 at a time.  The operands come straight
+// from the pages; the next tile's loads go out behind the products that have read their
+// registers.  Blocks of 16 are workgroups of their own, which find each other's K and V in the
+// caches: two blocks in one take the registers of one wave a SIMD and, at 4 rows of 7B, 18.5 us
+// instead of 15.6 behind 8 x 2000 keys, 34.8 instead of 23.6 behind 4 x 16000.  kOnce: non-temporal
+// loads, for pools that no cache holds until the next step; solo: no cuts (see launch()).
+template <bool kCausal, bool kOnce, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, 2) q4_few_kernel(AttnArgs a, int blocks, bool solo) {
     __shared__ __attribute__((aligned(16))) float s_acc[kWaves][16][kAccRow];
-    __shared__ float s_m[kWaves][COLS], s_l[kWaves][COLS];
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int kvh = blockIdx.x % NKV, unit = blockIdx.x / NKV;
-    const int slot = NB == 1 && solo ? unit / solo : unit;
-    const int col0 = NB == 1 && solo ? 16 * (unit - slot * solo) : 0;        // the first of the workgroup's columns
+    const int slot = unit / blocks, col0 = 16 * (unit - slot * blocks);      // the first of the workgroup's columns
     Part p;
     const bool whole = solo && a.table_stride <= 64;         // a lane per page of the table:
     int row = 0;                                             // its row, requested beside the length
@@ -401,15 +401,15 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
         if (p.s.rows * G <= col0) return;
     } else {
         p = find_part<kCausal>(a, slot);
-        if (p.sess < 0) return;
+        if (p.sess < 0 || p.s.rows * G <= col0) return;
     }
-    if (!solo && kvh == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
-    const int n_cols = p.s.rows * G - col0;
+    if (!solo && kvh == 0 && col0 == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
+    const int n_cols = min(p.s.rows * G - col0, 16);
     // the part's tiles, and this wave's of them
     const int tiles = (p.s.keys + TILE - 1) / TILE;
     const int t_lo = (int)((int64_t)tiles * p.index / p.parts), t_hi = (int)((int64_t)tiles * (p.index + 1) / p.parts);
     const int t0 = t_lo + (t_hi - t_lo) * wave / kWaves, t1 = t_lo + (t_hi - t_lo) * (wave + 1) / kWaves;
-    const int clear_keys = min(p.s.past + 1, p.s.keys);      // keys below: seen by all columns
+    const int clear_keys = min(p.s.past + col0 / G + 1, p.s.keys);           // keys below: seen by all its columns
 
     // lane (g, c) reads K rows and exponents of page c >> 2, V columns and exponents of page g
     Pages pages(a, p.sess, p.s.keys);
@@ -435,21 +435,18 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
 #pragma unroll
         for (int b = 0; b < 4; ++b) vr[b] = page_load<kOnce>(v_at + kQ4VOff + 256 * b + 16 * c);
     };
-    QTerms q[NB];
-    State st[NB];
-    int seen[NB];              // keys that the column sees
+    QTerms q;
+    State st;
+    int seen;                  // keys that the column sees
     Window win;
     win.clear();
-#pragma unroll
-    for (int b = 0; b < NB; ++b) st[b].clear();
+    st.clear();
     if (t0 < t1) {             // the queries first: they have come when the first pages are on their way
-        f4 x[NB][8];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) load_q(a, p.s, kvh, col0 + 16 * b + c, x[b], seen[b]);
+        f4 x[8];
+        load_q(a, p.s, kvh, col0 + c, x, seen);
         load_k(t0);
         load_v();
-#pragma unroll
-        for (int b = 0; b < NB; ++b) q_terms(x[b], q[b]);
+        q_terms(x, q);
     }
     auto step = [&](auto mask_tag, int t) {
         constexpr bool kMask = decltype(mask_tag)::value;
@@ -463,19 +460,16 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
         auto rest = [&](auto half_tag, uint32_t nan) {
             constexpr bool kHalf = decltype(half_tag)::value;
             constexpr int kN = kParts<kHalf>;
-            u4 w[NB][2][kN];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                f4 z[4];
-                float e[2][8];
-                scores(kr, q[b], ke, st[b].m, z);
-                if (kMask) hide(z, key0, seen[b]);
-                follow<kHalf>(z, st[b]);
-                weights<kHalf>(z, nan, e);
-                st[b].l += sum_of(e);
-                split<kHalf>(e[0], w[b][0]);
-                split<kHalf>(e[1], w[b][1]);
-            }
+            u4 w[2][kN];
+            f4 z[4];
+            float e[2][8];
+            scores(kr, q, ke, st.m, z);
+            if (kMask) hide(z, key0, seen);
+            follow<kHalf>(z, st);
+            weights<kHalf>(z, nan, e);
+            st.l += sum_of(e);
+            split<kHalf>(e[0], w[0]);
+            split<kHalf>(e[1], w[1]);
             const bool more = t + 1 < t1;
             if (more) load_k(t + 1);
             each<4>([&](auto b) {
@@ -486,12 +480,10 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
                     u4 lower, upper;
                     values_of<kHalf>((uint32_t)vr[b][2 * h], (uint32_t)vr[b][2 * h + 1], e[2 * h], e[2 * h + 1], lower, upper);
 #pragma unroll
-                    for (int n = 0; n < NB; ++n)
-#pragma unroll
-                        for (int k = kN - 1; k >= 0; --k) {
-                            st[n].acc[2 * b] = add_up<kHalf>(lower, w[n][h][k], st[n].acc[2 * b]);
-                            st[n].acc[2 * b + 1] = add_up<kHalf>(upper, w[n][h][k], st[n].acc[2 * b + 1]);
-                        }
+                    for (int k = kN - 1; k >= 0; --k) {
+                        st.acc[2 * b] = add_up<kHalf>(lower, w[h][k], st.acc[2 * b]);
+                        st.acc[2 * b + 1] = add_up<kHalf>(upper, w[h][k], st.acc[2 * b + 1]);
+                    }
                 });
             });
             if (more) load_v();
@@ -515,45 +507,36 @@ __global__ void __launch_bounds__(64 * kWaves, NB == 1 ? 2 : 1) q4_few_kernel(At
     for (int t = t_clear; t < t1; ++t) step(std::true_type{}, t);
 
     // the waves' states joined in LDS; a lone part writes the output
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const float l = rows_sum(st[b].l);
-        if (g == 0) {
-            s_m[wave][16 * b + c] = st[b].reference();
-            s_l[wave][16 * b + c] = l;
-        }
+    const float sum_l = rows_sum(st.l);
+    if (g == 0) {
+        s_m[wave][c] = st.reference();
+        s_l[wave][c] = sum_l;
     }
+    if (c < n_cols)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        if (16 * b >= n_cols) break;                         // uniform
-        if (b > 0) __syncthreads();
-        if (16 * b + c < n_cols)
+        for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(&s_acc[wave][c][16 * d + 4 * g]) = st.acc[d];
+    __syncthreads();
+    for (int e = tid; e < n_cols * (HD / 4); e += 64 * kWaves) {
+        const int cc = e / (HD / 4), d4 = e % (HD / 4), col = col0 + cc;
+        float m = s_m[0][cc];
 #pragma unroll
-            for (int d = 0; d < DB; ++d) *reinterpret_cast<f4*>(&s_acc[wave][c][16 * d + 4 * g]) = st[b].acc[d];
-        __syncthreads();
-        for (int e = tid; e < 16 * (HD / 4); e += 64 * kWaves) {
-            const int cc = e / (HD / 4), d4 = e % (HD / 4), col = 16 * b + cc;
-            if (col >= n_cols) continue;
-            float m = s_m[0][col];
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][cc]);
+        f4 sum = f4{0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][col]);
-            f4 sum = f4{0.f, 0.f, 0.f, 0.f};
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const Factor f(s_m[w][col] - m);
-                sum += f * *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]);
-                l += f * s_l[w][col];
-            }
-            if (p.parts == 1) {
-                const int r = (col0 + col) / G, hh = col0 + col - r * G;
-                const float n = p.s.keys > 0 ? 1.0f / l : 0.f;
-                *reinterpret_cast<f4*>(a.o + ((int64_t)(p.s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d4) = sum * n;
-            } else {
-                const int64_t at = ((int64_t)kvh * a.slots + slot) * COLS + col;
-                *reinterpret_cast<f4*>(a.acc + at * HD + 4 * d4) = sum;
-                if (d4 == 0) a.ml[at] = f2{m, l};
-            }
+        for (int w = 0; w < kWaves; ++w) {
+            const Factor f(s_m[w][cc] - m);
+            sum += f * *reinterpret_cast<const f4*>(&s_acc[w][cc][4 * d4]);
+            l += f * s_l[w][cc];
+        }
+        if (p.parts == 1) {
+            const int r = col / G, hh = col - r * G;
+            const float n = p.s.keys > 0 ? 1.0f / l : 0.f;
+            *reinterpret_cast<f4*>(a.o + ((int64_t)(p.s.row0 + r) * NH + kvh * G + hh) * HD + 4 * d4) = sum * n;
+        } else {
+            const int64_t at = ((int64_t)kvh * a.slots + slot) * (16 * blocks) + col;
+            *reinterpret_cast<f4*>(a.acc + at * HD + 4 * d4) = sum;
+            if (d4 == 0) a.ml[at] = f2{m, l};
         }
     }
 }
@@ -819,8 +802,19 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
     a.ml = reinterpret_cast<f2*>(ws + w.ml);
     a.acc = reinterpret_cast<float*>(ws + w.acc);
     const unsigned join_wgs = (unsigned)std::min<int64_t>((int64_t)a.rows.n_rows * NH, kJoinWgs);
+    // Up to 64 columns of short tables: a workgroup per session, kv head and 16 columns, nothing to find and
+    // nothing to join.  Up to 64 pages; where the workgroups are 64 and more, up to 96, as parts of the sessions
+    // would share CUs.  One launch against two (us, one after another in a graph), 1 / 8 / 32 sessions of 7B: of 300
+    // keys 6.6, 6.8, 6.9 against 9.2, 9.3, 10.0; of 1024 8.9, 9.2, 9.5 against 9.4, 9.6, 12.6; of 1040 10.5, 10.8, 11.2
+    // against 9.5, 9.8, 14.0; of 1536 11.4, 11.7, 12.4 against 9.5, 9.8, 14.7.
+    // 33 to 64 columns against the form of many: 8 rows behind 1 / 16 / 64 x 500 keys 8.1, 8.8, 21.3 and 16.6, 20.6,
+    // 28.8; 64 x 1400 40.4 and 39.7; without the limit, 16 x 3000 of 5 rows, in parts, 28.4 and 25.3.
+    const int64_t cols = (int64_t)a.max_q * G;
+    const int blocks = cols <= 64 ? (int)(cols + 15) / 16 : 1;
+    const int64_t wgs = (int64_t)a.n_sess * NKV * blocks;
+    const bool solo = cols <= 64 && a.table_stride <= (wgs >= kCus / 4 ? 96 : 64);
     if constexpr (kCausal) {
-        if (f.many) {
+        if (f.many && !solo) {
             hipLaunchKernelGGL(q4_many_kernel, dim3(NKV, a.gw), dim3(THREADS), 0, s, a);
             NOVA_LAUNCHED();
             hipLaunchKernelGGL(many_join_kernel, dim3(join_wgs), dim3(THREADS), 0, s, a);
@@ -828,26 +822,18 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
             return;
         }
     }
-    // Short tables: a workgroup per session, kv head and 16 columns, nothing to find and nothing to join.  Up to
-    // 64 pages; where the workgroups are 64 and more, up to 96, as parts of the sessions would share CUs.  One launch against two (us, one after another in a graph), 1 / 8 / 32 sessions of 7B: of 300
-    // keys 6.6, 6.8, 6.9 against 9.2, 9.3, 10.0; of 1024 8.9, 9.2, 9.5 against 9.4, 9.6, 12.6; of 1040 10.5, 10.8, 11.2
-    // against 9.5, 9.8, 14.0; of 1536 11.4, 11.7, 12.4 against 9.5, 9.8, 14.7.  With 4 rows: of 500 12.2, 12.5, 12.7
-    // against 14.0, 14.8, 21.3; of 764 14.7, 15.1, 15.5 against 14.0, 15.2, 29.6.
-    const int halves = f.cols / 16, wgs = a.n_sess * NKV * halves;
-    const bool solo = a.table_stride <= (wgs >= kCus / 4 ? 96 : 64);
     // With a CU for each of them, eight waves instead of four (7.1 and 9.6 us for 16 sessions of 300 and 1024 keys of
     // 7B with four, 6.8 and 9.2 with eight).
     const bool wide = solo && wgs <= kCus;
-    const dim3 grid(solo ? wgs : NKV * f.slots);             // (slots may be past what a second dimension holds)
+    a.gw /= blocks;
+    const dim3 grid((unsigned)(solo ? wgs : (int64_t)NKV * f.slots * blocks));   // (past what a second dimension holds)
     // The pages of a pool larger than the 256 MB memory-side cache (all layers of it,
     // as a step walks through them) come from HBM.
     const bool once = (int64_t)Model::L * a.nb * kQ4Page > (int64_t)256 << 20;
     auto run = [&](auto once_tag) {
         constexpr bool kOnce = decltype(once_tag)::value;
-        if (wide) hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, 8>), grid, dim3(512), 0, s, a, halves);
-        else if (solo || halves == 1)
-            hipLaunchKernelGGL((q4_few_kernel<1, kCausal, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, solo ? halves : 0);
-        else if constexpr (kCausal) hipLaunchKernelGGL((q4_few_kernel<2, true, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, 0);
+        if (wide) hipLaunchKernelGGL((q4_few_kernel<kCausal, kOnce, 8>), grid, dim3(512), 0, s, a, blocks, solo);
+        else hipLaunchKernelGGL((q4_few_kernel<kCausal, kOnce, WAVES>), grid, dim3(THREADS), 0, s, a, blocks, solo);
     };
     if (once) run(std::true_type{});
     else run(std::false_type{});
