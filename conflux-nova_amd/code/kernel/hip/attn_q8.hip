@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, NB == 1 ? 2 : 1) q8_few_kernel(AttnAr
     __shared__ __attribute__((aligned(16))) float s_acc[WAVES][16][kAccRow];
     __shared__ float s_m[WAVES][COLS], s_l[WAVES][COLS];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x, slot = blockIdx.y;
+    const int kvh = blockIdx.x % NKV, slot = blockIdx.x / NKV;
     const Part p = find_part<kCausal>(a, slot);
     if (p.sess < 0) return;
     if (kvh == 0 && p.index == 0 && tid == 0) a.info[p.sess] = i4{slot, p.parts, p.s.rows, p.s.row0};
@@ -664,7 +664,7 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
     // sessions of up to 600 keys, 7B: 9.6 us instead of 10.7 in two launches).
     const bool solo = a.table_stride <= kSoloPages;
     if (solo) a.min_share = kSoloPages;
-    const dim3 grid(NKV, solo ? a.n_sess : f.slots);
+    const dim3 grid((unsigned)(NKV * (solo ? a.n_sess : f.slots)));          // (slots may pass what a second dimension holds)
     // The pages of a pool larger than the 256 MB memory-side cache (all layers of it,
     // as a step walks through them) come from HBM: non-temporal loads, 8 x 32768 keys
     // of the 14B model 103 -> 90 us, 16 ragged sessions of the 7B model whose pages
