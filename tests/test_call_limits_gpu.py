@@ -4,6 +4,7 @@ import pytest
 
 import q8ref
 from q8ref import HD, Q8Pool
+from test_q4_store_gpu import _angles, _turn
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,41 @@ def test_8_bit_attention_of_as_many_sessions_as_a_call_takes(rows, stride):
         k, v = q8ref.values(pool.rec, table[i], int(keys[i]))
         ref, tol = q8ref.attention(q[a:b], k, v, int(past[i]) + (1 if rows else 0), nova.group)
         q8ref.assert_within(got[a:b], ref, tol, f"session {i}")
+
+
+def test_rotation_of_more_rows_than_workgroups():
+    """rows past the grid's workgroups, some of them empty, into other buffers and in place"""
+    nova, rows, rot = _nova("qwen25_1p5b"), 65536 + 41, 96
+    print(f"[case] rope rows {rows}", flush=True)
+    rng = np.random.default_rng(rows)
+    q, k = (rng.standard_normal((rows, n, HD), np.float32) for n in (nova.nh, nova.nkv))
+    c, s = _angles(rng, rows, rot)
+    pos = np.arange(rows, dtype=np.int32)
+    pos[[7, 65535, 65536 + 7, 65536 + 40]] = -1
+    dq, dk, dc, ds, dp = (nova.upload(x) for x in (q, k, c, s, pos))
+    oq, ok = (nova.upload(np.full(x.shape, 7, np.float32)) for x in (q, k))
+    some = np.concatenate([np.arange(40), np.arange(65500, rows)])
+    for to_q, to_k, rest in ((oq, ok, None), (dq, dk, 0)):
+        nova.launch_rope_rows(dq.ptr, dk.ptr, dp.ptr, dc.ptr, ds.ptr, rows, rot, 0, to_q.ptr, to_k.ptr, None)
+        nova.dev_sync()
+        for to, x in ((to_q, q), (to_k, k)):
+            want = _turn(x[some], c[some], s[some], rot, 0)
+            want[pos[some] < 0] = 7 if rest is None else x[some][pos[some] < 0]
+            assert np.array_equal(to.numpy(x.shape, np.float32)[some], want)
+
+
+def test_rotation_of_as_many_rows_as_a_call_takes():
+    """2^24 rows, all but the first of them empty"""
+    nova, rows, rot = _nova("qwen25_1p5b"), 1 << 24, 128
+    print(f"[case] rope rows {rows}", flush=True)
+    rng = np.random.default_rng(1)
+    q, k = (rng.standard_normal((3, n, HD), np.float32) for n in (nova.nh, nova.nkv))
+    c, s = _angles(rng, 3, rot)
+    pos = np.full(rows, -1, np.int32)
+    pos[:2] = 5
+    dq, dk, dc, ds, dp = (nova.upload(x) for x in (q, k, c, s, pos))     # (empty rows are not read)
+    nova.launch_rope_rows(dq.ptr, dk.ptr, dp.ptr, dc.ptr, ds.ptr, rows, rot, 0, dq.ptr, dk.ptr, None)
+    nova.dev_sync()
+    for dev, x in ((dq, q), (dk, k)):
+        got = dev.numpy(x.shape, np.float32)
+        assert np.array_equal(got[:2], _turn(x, c, s, rot, 0)[:2]) and np.array_equal(got[2], x[2])
