@@ -97,7 +97,16 @@ template <bool kRope>
 constexpr int kUnits = NKV + (kRope ? NH / kHeads : 0);
 static_assert(kUnits<true> % 8 != 0, "units spread over the XCDs");
 
-// grid: pages of the call (an upper bound) times kUnits
+// Workgroups of a call: its pages (an upper bound) times kUnits.  A launch has fewer than 2^32 threads, which the
+// rotation and append of the 14B shape would pass from 13 million rows on (370 GB of them).
+template <bool kRope>
+unsigned store_wgs(const RowArgs& a) {
+    const uint64_t wgs = (uint64_t)page_bound(a) * kUnits<kRope>;
+    NOVA_REQUIRE(wgs * QT <= UINT32_MAX);
+    return (unsigned)wgs;
+}
+
+// grid: store_wgs
 template <bool kRope, RopeForm kForm>
 __global__ void __launch_bounds__(QT) q4_store_kernel(StoreArgs a) {
     const PageItem it = page_item(a, blockIdx.x / kUnits<kRope>);
@@ -217,7 +226,7 @@ void launch_kv_q4_store_batch(uint8_t* pool, const int32_t* tables, int table_st
     if (n_rows == 0) return;
     a.k = k;
     a.v = v;
-    hipLaunchKernelGGL((q4_store_kernel<false, kRopeApart4>), dim3(page_bound(a) * kUnits<false>), dim3(QT), 0,
+    hipLaunchKernelGGL((q4_store_kernel<false, kRopeApart4>), dim3(store_wgs<false>(a)), dim3(QT), 0,
                        reinterpret_cast<hipStream_t>(s), a);
     NOVA_LAUNCHED();
 }
@@ -237,7 +246,7 @@ void launch_rope_rows_kv_q4_store_batch(const float* q, const float* k, const fl
     a.cs = cs;
     a.sn = sn;
     rope_forms(rot_dim, beside != 0, [&](auto form) {
-        hipLaunchKernelGGL((q4_store_kernel<true, decltype(form)::value>), dim3(page_bound(a) * kUnits<true>), dim3(QT), 0,
+        hipLaunchKernelGGL((q4_store_kernel<true, decltype(form)::value>), dim3(store_wgs<true>(a)), dim3(QT), 0,
                            reinterpret_cast<hipStream_t>(s), a);
         NOVA_LAUNCHED();
     });

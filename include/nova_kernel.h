@@ -416,7 +416,8 @@ void launch_kv_q4_store_batch(uint8_t* pool, const int32_t* tables, int table_st
 /* Rotation and append in one launch: q's rows turn into q_out (which may be q), k's rows turn and
  * are quantised with v's (k's buffer is left as passed).  cs, sn: the rows' angles from
  * launch_rope_angles; rot_dim and beside as in launch_rope_rows, whose bits the turned
- * rows have. */
+ * rows have.  Of the 14B shape at most about 13 million rows a call (as many as a launch has
+ * threads for), else 2^24 as everywhere. */
 void launch_rope_rows_kv_q4_store_batch(const float* q, const float* k, const float* v, const float* cs, const float* sn,
                                         int rot_dim, int beside, uint8_t* pool, const int32_t* tables, int table_stride,
                                         const int32_t* n_past, const int32_t* row_off, int n_sess, int n_rows, int layer,
