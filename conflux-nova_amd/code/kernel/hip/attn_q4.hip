@@ -232,7 +232,7 @@ __device__ __forceinline__ uint32_t take_nan(uint32_t& w) {
 // The window of exponent bytes that tiles in fp16 lie in: `base` to base + kSpread - 1.
 struct Window {
     uint32_t add, want, fill;  // per byte: what is added to a byte of the window gives `want` in its upper five bits
-    bool closed;               // a value past fp16 has been seen: no more fp16, so that the reference's drop keeps the sums finite
+    bool closed;               // a value past fp16 is in the sums: no more fp16, so that the reference's drop keeps them finite
     __device__ __forceinline__ void at(int base) {
         const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane(base), up = -b & (kSpread - 1);
         add = up * 0x01010101u;
@@ -692,6 +692,7 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
             load_k(start);
             q_terms(x, q);
             st.clear();
+            win.closed = false;                              // (the window stays: it says nothing about the sums)
         }
         // One tile: its scores and weights, then the barrier that V waits for, then its
         // products.  True: V of the next tile is in LDS as well, in fp16 (what almost all are).

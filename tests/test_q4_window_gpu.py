@@ -1,0 +1,26 @@
+"""Attention over 4-bit pages: which of its two forms a tile of 64 keys takes is a matter of that
+tile's own values and of what the same rows have met before, and of nothing else."""
+import numpy as np
+import pytest
+
+from q4ref import KB, Call
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("model", ["qwen25_1p5b", "qwen25_7b", "qwen25_14b"])
+@pytest.mark.parametrize("rows,past", [(70, 100), (70, 20), (12, 2000)])
+def test_values_past_fp16_stay_with_their_session(model, rows, past):
+    """Every other session's values are 2^20 times as large, past fp16: the sessions between them, which
+    share workgroups with them, have the bits that they have beside values of their own size."""
+    n = 60
+    c = Call(model, [past + 3 * (i % 5) for i in range(n)], [rows] * n, seed=21, behind=0, scale=0.5)
+    still = c.run().reshape(n, -1)
+    p = c.parts()
+    for i in range(1, n, 2):
+        p[3][c.table[i, :-(-int(c.keys[i]) // KB)]] += 20
+    c.set_parts(p)
+    loud = c.run().reshape(n, -1)
+    changed = [i for i in range(0, n, 2) if not np.array_equal(still[i], loud[i])]
+    assert not changed, f"sessions {changed}"
+    assert not any(np.array_equal(still[i], loud[i]) for i in range(1, n, 2))
