@@ -12,7 +12,7 @@
 // lie close together (a window of eight, kSpread) is exact in fp16, and a weight goes in as
 // two fp16 terms, to 2^-22 of itself or, where fp16 ends first, to 2^-24.  The largest weight
 // of that row in the tile stands at 2^kLow or more, so 2^-24 is 2^-26 of that weight.  Any other
-// tile (powers far apart, blocks of zeros, NaN, values past fp16) takes V as bf16 with its
+// tile (powers far apart, blocks of zeros, NaN, values past fp16's normal numbers) takes V as bf16 with its
 // power of two, exact too, and a weight as the exact sum of three bf16 terms (8 bits each).
 // Sums are fp32.
 //
@@ -71,7 +71,11 @@ constexpr float kLazy = 8.f;                   // and at most in bf16 terms: 2^2
 constexpr float kDrop = 80.f;
 constexpr int kCus = kAimWgs / 2;
 constexpr int kSpread = 8;                     // powers of two of a tile in fp16: this many in a row
-constexpr int kLeastHalf = 127 - 23, kMostHalf = 127 + 13;   // exponent bytes whose values fp16 holds exactly
+// Exponent bytes whose values (1/2 to 6 times the power) are normal numbers of fp16.  Subnormal ones would be
+// exact too, but the matrix unit adds products up at the place of their operands' exponents, which it takes as
+// fp16's least there: weights lose a bit for each power below (values of 2^-24, one after another: the result was
+// off by 2^-12 of itself; of 2^-14 by 2^-20, as at any larger power).
+constexpr int kLeastHalf = 127 - 13, kMostHalf = 127 + 13;
 constexpr int kTerms = 5;                      // of the query
 constexpr int kLeastExp = -100;                // of a query block: its last term's power is a normal number
 

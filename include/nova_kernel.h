@@ -429,8 +429,8 @@ void launch_kv_q4_load_batch(const uint8_t* pool, const int32_t* tables, int tab
 /* Decode and chunk attention: the calls of the 8-bit pages, with the same arguments.
  * Precision: fp32 over the values of the codes, but for two roundings.  A query (times
  * 1/sqrt(HD) log2 e) is held to 2^-24 of the largest of each 32 of its dims, or to 2^-124.  In
- * a tile (64 keys from a multiple of 64) whose V powers of two lie within 2^7 of each other, a key's
- * weight is held to 2^-22 of itself, or to 2^-26 of the row's largest weight in that tile, or to 2^-104 of
+ * a tile (64 keys from a multiple of 64) whose V powers of two lie within 2^7 of each other, and from
+ * 2^-13 to 2^13, a key's weight is held to 2^-22 of itself, or to 2^-26 of the row's largest weight in that tile, or to 2^-104 of
  * the row's largest; in any other tile it goes in whole.  Scores have to be finite in fp32.  Keys that a
  * row does not see do not enter it, whatever they hold (only, their powers may decide which of the two
  * a tile is). */

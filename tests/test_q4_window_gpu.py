@@ -24,3 +24,19 @@ def test_values_past_fp16_stay_with_their_session(model, rows, past):
     changed = [i for i in range(0, n, 2) if not np.array_equal(still[i], loud[i])]
     assert not changed, f"sessions {changed}"
     assert not any(np.array_equal(still[i], loud[i]) for i in range(1, n, 2))
+
+
+@pytest.mark.parametrize("byte", [104, 107, 110, 113, 114, 120, 140, 141])
+@pytest.mark.parametrize("rows,keys", [(0, 40), (0, 900), (4, 300), (70, 900)])
+def test_a_mean_of_equal_values_is_the_value(rows, keys, byte):
+    """Every value is half of one power of two, those that fp16 holds as subnormal numbers among them.  Numerator and
+    denominator are sums of the same weights.  In the numerator a weight is held to 2^-22 of itself or to 2^-26 of
+    the largest of its 64, at most 2^-20 of their sum; each sum runs through chains of at most 3 n / 32 + 64
+    additions of 2^-24; the quotient and its product take 2^-23."""
+    c = Call("qwen25_7b", [keys - rows] * 3, [rows] * 3 if rows else None, seed=22, behind=0, poison=False)
+    p = c.parts()
+    p[2][:], p[3][:] = 1, byte
+    c.set_parts(p)
+    off = c.run() / 2.0 ** (byte - 128) - 1
+    bound = 2.0 ** -22 + 2.0 ** -20 + 2 * (3 * keys / 32 + 64) * 2.0 ** -24 + 2.0 ** -23
+    assert np.abs(off).max() <= bound, np.abs(off).max() / bound
