@@ -261,15 +261,16 @@ struct Window {
 };
 static_assert(kSpread == 8, "upper five bits");
 
-// smallest and largest of a lane's bytes, into the running ones
-__device__ __forceinline__ void byte_range(uint32_t w, int& least, int& most) {
+// smallest and largest of a lane's bytes that `keep` keeps, into the running ones
+__device__ __forceinline__ void byte_range(uint32_t w, uint32_t keep, int& least, int& most) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const int b = (int)(w >> (8 * k) & 255u);
-        least = min(least, b);
-        most = max(most, b);
+        least = min(least, (int)((w | ~keep) >> (8 * k) & 255u));
+        most = max(most, (int)((w & keep) >> (8 * k) & 255u));
     }
 }
+// of the exponents of four tokens, those of the first `rest`: slots behind the last key may hold anything
+__device__ __forceinline__ uint32_t tokens_of(int rest) { return rest >= 4 ? ~0u : rest <= 0 ? 0u : (1u << (8 * rest)) - 1u; }
 __device__ __forceinline__ void wave_range(int& least, int& most) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -455,10 +456,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2) q4_few_kernel(AttnArgs a, int 
     auto step = [&](auto mask_tag, int t) {
         constexpr bool kMask = decltype(mask_tag)::value;
         const int key0 = t * TILE + 16 * g;
-        uint32_t ex = (uint32_t)ve;                          // the lane's: tokens 4 (c & 3) .. of block c >> 2
-        if (kMask) {                                         // a slot behind the last key may hold anything
-            const int rest = p.s.keys - key0 - 4 * (c & 3);
-            const uint32_t keep = rest >= 4 ? ~0u : rest <= 0 ? 0u : (1u << (8 * rest)) - 1u;
+        uint32_t ex = (uint32_t)ve, keep = ~0u;              // the lane's: tokens 4 (c & 3) .. of block c >> 2
+        if (kMask) {
+            keep = tokens_of(p.s.keys - key0 - 4 * (c & 3));
             ex = (ex & keep) | (win.fill & ~keep);
         }
         auto rest = [&](auto half_tag, uint32_t nan) {
@@ -497,9 +497,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2) q4_few_kernel(AttnArgs a, int 
         if (!half) {                                         // rare: another window, or none
             nan = take_nan(ex) << (4 * (c & 3));
             int least = 255, most = 0;
-            byte_range(ex, least, most);
+            byte_range(ex, keep, least, most);
             wave_range(least, most);
             half = win.move(least, most);                    // (not with NaN in it, whose bytes are 0 now)
+            if (kMask) ex = (ex & keep) | (win.fill & ~keep);
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) nan |= (uint32_t)__shfl_xor((int)nan, o, 64);
         }
@@ -626,8 +627,7 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
         // the exponents of tokens from..from + 3 with those of slots behind the last key, which
         // may hold anything, replaced
         auto cut = [&](uint32_t x, int from) {
-            const int rest = s.keys - from;
-            const uint32_t keep = rest >= 4 ? ~0u : rest <= 0 ? 0u : (1u << (8 * rest)) - 1u;
+            const uint32_t keep = tokens_of(s.keys - from);
             return (x & keep) | (win.fill & ~keep);
         };
         // V of a tile in operand order, lane (g, c) dims 32 g + c and 32 g + 16 + c of page `wave`; to LDS
@@ -647,17 +647,22 @@ __global__ void __launch_bounds__(THREADS, 2) q4_many_kernel(AttnArgs a) {
         uint32_t nan = 0;                                    // tokens of page g whose value is NaN
         // the same for any tile; true: in fp16
         auto put = [&](int t) {
-            uint32_t x = cut(vx, t * TILE + 16 * (c >> 2) + 4 * (c & 3));
+            const int from = t * TILE + 16 * (c >> 2) + 4 * (c & 3);
+            uint32_t x = cut(vx, from);
+            auto cut_own = [&] {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ve[i] = (int)cut((uint32_t)ve[i], t * TILE + 16 * wave + 4 * i);
+                for (int i = 0; i < 4; ++i) ve[i] = (int)cut((uint32_t)ve[i], t * TILE + 16 * wave + 4 * i);
+            };
+            cut_own();
             bool half = !win.closed && __builtin_amdgcn_ballot_w64(win.outside(x) != 0) == 0;
             nan = 0;
             if (!half) {                                     // another window, or none
                 const uint32_t m = take_nan(x) << (4 * (c & 3));
                 int least = 255, most = 0;
-                byte_range(x, least, most);
+                byte_range(x, tokens_of(s.keys - from), least, most);
                 wave_range(least, most);
                 half = win.move(least, most);                // (not with NaN in it, whose bytes are 0 now)
+                cut_own();
                 if (__builtin_amdgcn_ballot_w64(m != 0)) {
                     nan = m;
                     nan |= (uint32_t)__shfl_xor((int)nan, 1, 64);

@@ -40,3 +40,27 @@ def test_a_mean_of_equal_values_is_the_value(rows, keys, byte):
     off = c.run() / 2.0 ** (byte - 128) - 1
     bound = 2.0 ** -22 + 2.0 ** -20 + 2 * (3 * keys / 32 + 64) * 2.0 ** -24 + 2.0 ** -23
     assert np.abs(off).max() <= bound, np.abs(off).max() / bound
+
+
+@pytest.mark.parametrize("power", [-10, -4, 9])
+@pytest.mark.parametrize("rows,keys", [(0, 1), (0, 40), (0, 200), (4, 40), (4, 133), (12, 40), (12, 61)])
+def test_a_tile_that_keys_fill_in_part_takes_its_form_from_them(rows, keys, power):
+    """Values 2^power times as large, as exact in fp16 as they were: the result is 2^power times what it was, bit
+    by bit, as no product, sum or weight of either is rounded differently.  What fills the slots behind
+    the last key has no say in it."""
+    past = [keys - rows] * 3
+    c = Call("qwen25_7b", past, [rows] * 3 if rows else None, seed=22, behind=0, scale=0.5)
+    one = c.run()
+    p = c.parts()
+    held = np.unique(np.concatenate([c.table[i, :-(-keys // KB)] for i in range(3)]))
+    e = p[3][held]
+    # (the poison behind the last key has powers of its own)
+    live = np.ones(e.shape, bool)
+    last = [int(np.flatnonzero(held == c.table[i, (keys - 1) // KB])[0]) for i in range(3)]
+    if keys % KB:
+        live[last, :, keys % KB:] = False
+    assert 124 <= e[live].min() and e[live].max() <= 128                         # normal numbers of fp16 at -10 and 9 as well
+    e[live] = (e[live].astype(int) + power).astype(np.uint8)
+    p[3][held] = e
+    c.set_parts(p)
+    assert np.array_equal(c.run(), one * np.float32(2.0 ** power))
