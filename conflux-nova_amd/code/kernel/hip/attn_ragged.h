@@ -604,7 +604,7 @@ AttnArgs attn_args(int64_t page, const float* q, const uint8_t* pool, const int3
     NOVA_REQUIRE((int64_t)n_sess * table_stride <= (int64_t)1 << 32);
     AttnArgs a{};
     a.q = q;
-    a.pool = pool + layer * nb * page;
+    a.pool = pool + (int64_t)layer * nb * page;
     a.tables = tables;
     a.table_stride = table_stride;
     a.n_keys = n_keys;
