@@ -463,6 +463,8 @@ void launch_kv_q4_zero_pages(uint8_t* pool, int nb, const int32_t* pages, int n_
  *     row of `tables`.  The first session with which the step's rows would pass max_rows
  *     or its pages would pass the free ones gets no rows, nor does any after it; one whose
  *     table is too short for keep + new gets none and the others are served.
+ *     Rows stand without gaps: behind a session that got none, the others' stand further up, by
+ *     row_off, and not where sums of n_new or the session's index would put them.
  * Lengths below 0 count as 0, n_have past the table as full, n_keep past n_have as n_have.
  * Out (device): n_past[i] = keep, n_keys[i] = keep + rows granted, row_off [n_sess+1] their sums, and
  * for each row r of max_rows its position pos[r] and its place in the cache slots[r] =
