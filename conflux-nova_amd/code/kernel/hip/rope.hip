@@ -175,15 +175,16 @@ __global__ void __launch_bounds__(RT) rope_angles_kernel(const int32_t* __restri
     sn[e] = (float)(s * magnitude);
 }
 
-// A workgroup per row, all heads of q and k, kRowWgs of them in the grid's first dimension (which holds fewer
-// than 2^32 threads: 2^24 rows would pass that).  HBM-bound elementwise work: 4096 rows of 7B, 134 MB, 26 us,
-// 5.1 TB/s, the rate of a large copy; 16 rows 3.1 us, a launch and its loads.
-constexpr int kRowWgs = 65536;
+// A workgroup per row, all heads of q and k.  HBM-bound elementwise work: 4096 rows of 7B, 134 MB, 26 us,
+// 5.1 TB/s, the rate of a large copy; 16 rows 3.1 us, a launch and its loads.  A launch takes up to kRowsPerLaunch rows:
+// it has fewer than 2^32 threads, which 2^24 rows would pass.  (A loop over rows in the kernel, or rows in the grid's
+// second dimension, cost the small calls up to 3%.)
+constexpr int kRowsPerLaunch = 1 << 20;
 template <RopeForm kForm>
 __global__ void __launch_bounds__(RT) rope_rows_kernel(const float* q, const float* k, const int32_t* pos, const float* cs,
-                                                       const float* sn, int n_rows, int rot, float* q_out, float* k_out) {
-    const int64_t row = (int64_t)blockIdx.y * kRowWgs + blockIdx.x;
-    if (row >= n_rows || (pos && pos[row] < 0)) return;
+                                                       const float* sn, int rot, float* q_out, float* k_out) {
+    const int64_t row = blockIdx.x;
+    if (pos && pos[row] < 0) return;
     const int units = rope_units<kForm>(rot);
     const float *c = cs + row * (rot / 2), *s = sn + row * (rot / 2);
     for (int u = threadIdx.x; u < (NH + NKV) * units; u += RT) {
@@ -314,12 +315,16 @@ void launch_rope_rows(const float* q, const float* k, const int32_t* pos, const 
     NOVA_REQUIRE(rot_dim >= 2 && rot_dim <= HD && rot_dim % 2 == 0);
     NOVA_REQUIRE(aligned16(q) && aligned16(k) && aligned16(cs) && aligned16(sn) && aligned16(q_out) && aligned16(k_out));
     if (n_rows == 0) return;
-    const dim3 grid((unsigned)std::min(n_rows, kRowWgs), (unsigned)((n_rows + kRowWgs - 1) / kRowWgs));
-    rope_forms(rot_dim, beside != 0, [&](auto form) {
-        hipLaunchKernelGGL(rope_rows_kernel<decltype(form)::value>, grid, dim3(RT), 0, reinterpret_cast<hipStream_t>(s), q, k,
-                           pos, cs, sn, n_rows, rot_dim, q_out, k_out);
-        NOVA_LAUNCHED();
-    });
+    for (int64_t row = 0; row < n_rows; row += kRowsPerLaunch) {
+        const int n = (int)std::min<int64_t>(n_rows - row, kRowsPerLaunch);
+        const int64_t in_q = row * NH * HD, in_k = row * NKV * HD, angle = row * (rot_dim / 2);
+        rope_forms(rot_dim, beside != 0, [&](auto form) {
+            hipLaunchKernelGGL(rope_rows_kernel<decltype(form)::value>, dim3((unsigned)n), dim3(RT), 0,
+                               reinterpret_cast<hipStream_t>(s), q + in_q, k + in_k, pos ? pos + row : nullptr, cs + angle,
+                               sn + angle, rot_dim, q_out + in_q, k_out + in_k);
+            NOVA_LAUNCHED();
+        });
+    }
 }
 
 }  // extern "C"

@@ -55,8 +55,8 @@ def test_8_bit_attention_of_as_many_sessions_as_a_call_takes(rows, stride):
         q8ref.assert_within(got[a:b], ref, tol, f"session {i}")
 
 
-def test_rotation_of_more_rows_than_workgroups():
-    """rows past the grid's workgroups, some of them empty, into other buffers and in place"""
+def test_rotation_of_many_rows():
+    """rows past 65536, some of them empty, into other buffers and in place"""
     nova, rows, rot = _nova("qwen25_1p5b"), 65536 + 41, 96
     print(f"[case] rope rows {rows}", flush=True)
     rng = np.random.default_rng(rows)
@@ -91,3 +91,34 @@ def test_rotation_of_as_many_rows_as_a_call_takes():
     for dev, x in ((dq, q), (dk, k)):
         got = dev.numpy(x.shape, np.float32)
         assert np.array_equal(got[:2], _turn(x, c, s, rot, 0)[:2]) and np.array_equal(got[2], x[2])
+
+
+@pytest.mark.parametrize("rot", [128, 6])
+def test_rotation_of_more_rows_than_a_launch_takes(rot):
+    """2^20 rows and 41, of which the first ones and those around 2^20 turn, in place; the others are empty"""
+    nova, border = _nova("qwen25_1p5b"), 1 << 20
+    rows = border + 41
+    print(f"[case] rope rows {rows} rot={rot}", flush=True)
+    rng = np.random.default_rng(rot)
+    some = np.concatenate([np.arange(3), np.arange(border - 4, border + 41)])
+    c, s = _angles(rng, len(some), rot)
+    pos = np.full(rows, -1, np.int32)
+    pos[some] = 9
+    pos[[border - 2, border + 3, rows - 1]] = -1
+    dp = nova.upload(pos)
+    dc, ds = (nova.alloc(rows * rot // 2 * 4) for _ in range(2))
+    dev = {n: nova.alloc(rows * n * HD * 4) for n in (nova.nh, nova.nkv)}
+    host = {n: rng.standard_normal((len(some), n, HD), np.float32) for n in dev}
+    # (the rows that turn lie in two runs)
+    for lo, hi, at in ((0, 3, 0), (3, len(some), border - 4)):
+        for d, x in ((dc, c), (ds, s), *((dev[n], host[n]) for n in dev)):
+            part = np.ascontiguousarray(x[lo:hi])
+            nova.dev_upload(d.ptr + at * part[0].nbytes, part.ctypes.data, part.nbytes)
+    q, k = dev[nova.nh].ptr, dev[nova.nkv].ptr
+    nova.launch_rope_rows(q, k, dp.ptr, dc.ptr, ds.ptr, rows, rot, 0, q, k, None)
+    nova.dev_sync()
+    for n, x in host.items():
+        want = np.where((pos[some] >= 0)[:, None, None], _turn(x, c, s, rot, 0), x)
+        got = np.concatenate([nova.download(dev[n], (hi - lo, n, HD), np.float32, at * n * HD * 4)
+                              for lo, hi, at in ((0, 3, 0), (3, len(some), border - 4))])
+        assert np.array_equal(got, want)
