@@ -368,12 +368,19 @@ typedef struct {
     double factor;         /* >= 1; not read by NOVA_ROPE_PLAIN */
     int train_len;         /* BY_PARTS: the model's own context */
     double slow_turns;     /* BY_PARTS: pairs that turn fewer times over train_len are stretched ... */
-    double fast_turns;     /* ... and those that turn more often stay; between, by degrees */
+    double fast_turns;     /* ... and those that turn more often stay; between, linear in the turns */
 } nova_rope_cfg;
 /* The pairs' rates in fp32 (host array of rot_dim/2; made in 64 bits) and the factor on
  * cos and sin, once per model.  LINEAR: freq / factor.  BASE: base * factor^(rot_dim /
- * (rot_dim - 2)).  BY_PARTS: freq of the fast pairs, freq / factor of the slow ones, and
- * a magnitude of 0.1 ln(factor) + 1 (else 1).  Returns rot_dim / 2. */
+ * (rot_dim - 2)).  BY_PARTS: a pair turns t = train_len * freq / 2 pi times over the model's own
+ * context; its rate is freq from fast_turns on, freq / factor up to slow_turns, and between them
+ * freq * (k + (1 - k) / factor), k = (t - slow_turns) / (fast_turns - slow_turns): a ramp that is linear
+ * in the turns; the magnitude is 0.1 ln(factor) + 1 (else 1).  Returns rot_dim / 2.
+ * There are models whose ramp is linear in the pair's index instead, between the rounded indices
+ * of the pairs that turn fast_turns and slow_turns times.  Their rates in between are others (base 10^6,
+ * 128 dims, train_len 32768, factor 4, turns 1 to 32: by more than 5% in 15 of 64 pairs, by 42% in
+ * one).  launch_rope_angles takes any rates and any magnitude, so such a model's program
+ * makes its own, and one that goes without the magnitude passes 1. */
 int nova_rope_freqs(const nova_rope_cfg* cfg, float* freq, double* magnitude);
 /* The angles of a step's rows, for all layers: cs, sn [n_rows][rot_dim/2] =
  * fp32(cos(pos[r] * freq[i]) * magnitude), and sin, in 64 bits before the one rounding; the angle
@@ -399,7 +406,8 @@ void launch_rope_rows(const float* q, const float* k, const int32_t* pos, const 
  *     V code       at 1024 + (d>>5)*256 + (d&15)*16 + t, the low half where bit 4 of d is clear
  *     K exponent   at 2048 + (t&3)*16 + (d>>5)*4 + (t>>2)
  *     V exponent   at 2112 + (d>>5)*16 + t
- * An exponent byte b stands for 2^(b - 127), 255 for NaN.  All-zero memory is a page of zeros.
+ * An exponent byte b stands for 2^(b - 127), 255 for NaN; 0 stands beside codes of zero only.  All-zero
+ * memory is a page of zeros.
  *
  * Quantiser, per 32 values with largest |x| = a: the power is the smallest 2^e with
  * a <= 7 * 2^e, the codes the values nearest to x / 2^e, ties to the even code, so that no
