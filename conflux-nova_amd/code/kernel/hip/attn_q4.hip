@@ -27,12 +27,16 @@
 // MB: 51 us, 5.6 TB/s, where a large read reaches 6.1; the joining launch takes 4 more), a chain of
 // latencies where they are few (16 ragged sessions of 512 to 8192 keys, 7B, 34 MB: 16 us and 4; of
 // a workgroup's 11: 1.3 until it knows its part, 1.7 until the queries are in terms, 4.7 for 2 or 3
-// tiles a wave, 1.9 for the end).  Many columns: vector and matrix instructions, which a SIMD
+// tiles a wave, 1.9 for the end, the rest and the launch's other 5 not taken apart).  Pages that no cache holds cost
+// little: the same call over 28 layers of a pool of 1 GB in turn 18.2 us instead of 17.6.  Many columns: vector and matrix instructions, which a SIMD
 // hardly overlaps (8 x 512 rows behind up to 4096 keys, 7B, 122 GFLOP of scores and outputs: 241
 // us, 506 TFLOP/s; per tile and wave 216 vector and 52 matrix instructions and 110 others take 960 ns
 // of a SIMD, where the vector and matrix ones alone, on registers, take 678).  Left out one by
 // one, the barrier is worth 4% of the time, three quarters of the LDS reads 2%, of K's loads nothing,
-// 16 of the 52 products or the conversion of V 9% each.  Three waves a SIMD, and the next tile's
+// 16 of the 52 products or the conversion of V 9% each.  Tiles in bf16: one in each session costs 2% of the many
+// columns and nothing of the decodes; all of them (a token 2^-12 as large as the others in each) 8 x 512
+// rows 366 us instead of 238, 8 x 32768 keys 68 instead of 62, 16 ragged sessions 19.3 instead of 17.5, 1 to 8 rows
+// of 16 sessions 40.2 instead of 31.9.  Three waves a SIMD, and the next tile's
 // scores under the softmax, are slower for want of registers.
 #include <hip/hip_runtime.h>
 #include <cstdint>
@@ -813,7 +817,8 @@ void launch(AttnArgs a, void* workspace, hipStream_t s) {
     a.acc = reinterpret_cast<float*>(ws + w.acc);
     const unsigned join_wgs = (unsigned)std::min<int64_t>((int64_t)a.rows.n_rows * NH, kJoinWgs);
     // Up to 64 columns of short tables: a workgroup per session, kv head and 16 columns, nothing to find and
-    // nothing to join.  Up to 64 pages; where the workgroups are 64 and more, up to 96, as parts of the sessions
+    // nothing to join.  The table's width counts, as the host knows no lengths: 8 sessions of 300 keys (7B) 6.9 us over a
+    // table of up to 64 pages, 9.5 over a wider one.  Up to 64 pages; where the workgroups are 64 and more, up to 96, as parts of the sessions
     // would share CUs.  One launch against two (us, one after another in a graph), 1 / 8 / 32 sessions of 7B: of 300
     // keys 6.6, 6.8, 6.9 against 9.2, 9.3, 10.0; of 1024 8.9, 9.2, 9.5 against 9.4, 9.6, 12.6; of 1040 10.5, 10.8, 11.2
     // against 9.5, 9.8, 14.0; of 1536 11.4, 11.7, 12.4 against 9.5, 9.8, 14.7.

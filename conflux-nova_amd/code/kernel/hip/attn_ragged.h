@@ -3,7 +3,8 @@
 // that join the pieces.
 //
 // Two kernels per format, by the columns (query rows x heads of a kv head) that a session
-// may have.  "few": up to 32, a workgroup's waves share them and split the keys.  "many": 64
+// may have.  "few": a workgroup's waves share its columns and split the keys; up to 32 columns, all in one
+// workgroup (8-bit pages), or 16 to a workgroup and up to 64 over short tables (4-bit pages).  "many": 64
 // columns a workgroup, all waves over the same keys.  A piece of a session's (or group's)
 // work leaves {reference m, sum of 2^(s - m)} and the weighted sum of values per column in
 // the workspace.
@@ -36,8 +37,9 @@ constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int TILE = 64;                       // keys of a wave's step: four pages
 constexpr int kTilePages = TILE / kKvBlock;
-// Workgroups aimed at: two per CU.  (Of the form with two blocks of columns one runs per
-// CU, as it takes the registers of both, so its parts go through in two rounds.)
+// Workgroups aimed at: two per CU (4-bit pages with four: 16 ragged sessions 21.6 us instead of 17.9, drafts 41.3,
+// 32.3, short mixed prompts 49.6, 35.5, 8 x 512 rows 255, 238).  Of the 8-bit form with two blocks of columns
+// one runs per CU, as it takes the registers of both, so its parts go through in two rounds.
 constexpr int kAimWgs = 512;
 constexpr int DB = HD / 16;                    // 16-dim blocks of the output
 constexpr int kManyCols = 16 * WAVES;          // columns of a workgroup where there are many
@@ -562,7 +564,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // 37.3; 16 x 600: 19.8, 17.5; 32 x 100: 14.0, 11.5); the host knows the columns, not the keys.
 constexpr int kFewCols = 32;
 // Tiles of a workgroup that shares a session: one per wave.  Many columns, 12 prompts
-// of up to 300 tokens (1.5B): 2 42.9 us, 4 43.1, 6 44.3, 8 57.4.
+// of up to 300 tokens (1.5B), 8-bit pages: 2 42.9 us, 4 43.1, 6 44.3, 8 57.4; 4-bit: 2 and 4 35.5.
 constexpr int kMinShare = 4;
 // A joining launch that fills the chip (4096: 16 sessions of 1 to 8 rows, 7B, 34.8 us instead
 // of 34.4; 12 prompts of up to 300 tokens, 1.5B, 38.5, 37.4).

@@ -18,8 +18,10 @@
 // otherwise: no byte holds two tokens, so the page's other tokens stay as they are.
 //
 // What bounds it: HBM (4096 rows of 7B, rotation and append, 138 MB: 32 us, 4.3 TB/s, where a large
-// copy reaches 5.1; their read back, 19 MB, 8.3 us) or, for a step's few rows, a launch and three
-// loads that wait for each other (16 rows 3.8 us).
+// copy reaches 5.1; one call after another, whose rows the caches still have, 25) or, for a step's few rows, a launch
+// and three loads that wait for each other (16 rows 3.8 us).  The append alone: 4096 rows, 19 MB, 4.1 us from the
+// caches, 16 rows 2.8.  The read back of 4096 rows, 19 MB, takes 7.5: twice what their bytes need; V comes out of
+// LDS byte by byte, with bank conflicts (0.46 M).
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <type_traits>
